@@ -54,6 +54,7 @@ extern "C" {
 #define TG_U8 6
 #define TG_F8E4M3 7
 #define TG_I8 8 /* not in the reference table (its cuTile-rs FFI has no int8 operator); used by the group quantiser */
+#define TG_F64 9 /* extension: rotary frequencies */
 
 typedef struct TgTensorDesc {
   uint64_t ptr;       /* device address */
@@ -363,6 +364,59 @@ TG_API const char* tg_last_error_string(void);
  * the choice is a cost model, waves x (k-blocks per unit + split tail), exposed for inspection and tests. */
 TG_API int32_t tg_plan_splits(int32_t kind, int64_t M, int64_t N, int64_t K, int32_t num_sms, int32_t* tile_cols,
                               int32_t* splits);
+
+/* ---- Decoder operators around the GEMMs -------------------------------------------------------------------
+ * RMS norm with the residual's addition in front and the 1 x 128 activation quantiser behind it:
+ *   h = round(x + residual),  y = h * rsqrt(mean(h^2) + eps) * (w + weight_offset),  s = amax / 448 per 128 values of y
+ *   (1 for an all-zero block),  Y = e4m3(y / s).
+ * X, R [T, hidden] bf16 / f16 with any row pitch (a multiple of 16 bytes); hidden a multiple of 128 up to 65536; W [hidden]
+ * in X's type or f32; Y [T, hidden] e4m3, S [T, hidden / 128] f32, H [T, hidden] contiguous.  R and H go together (both
+ * null: h = x).  H may be the memory of X or of R. */
+TG_API int32_t tg_rms_norm_quant(const TgTensorDesc* Y, const TgTensorDesc* S, const TgTensorDesc* H, const TgTensorDesc* X,
+                                 const TgTensorDesc* R, const TgTensorDesc* W, float eps, float weight_offset, int32_t device_id,
+                                 uint64_t stream);
+
+/* Rotary positions of Q [T, heads, D] and K [T, heads, D] (K / Ko may be null), bf16 / f16, D a multiple of 16 up to 512,
+ * any token and head pitch that keeps 16-byte alignment; the outputs may be the inputs.  inv_freq: f64 [R / 2] radians per
+ * position, R <= D a multiple of 16; elements from R on are copied.  interleaved 0: pairs (i, i + R / 2), 1: (2 i, 2 i + 1).
+ * positions: int32 / int64 [T], any value.  cos and sin are multiplied by `magnitude`. */
+TG_API int32_t tg_apply_rope(const TgTensorDesc* Qo, const TgTensorDesc* Ko, const TgTensorDesc* Q, const TgTensorDesc* K,
+                             const TgTensorDesc* positions, const TgTensorDesc* inv_freq, int32_t interleaved, float magnitude,
+                             int32_t device_id, uint64_t stream);
+
+/* Paged key / value cache in e4m3.  Kc [pages, heads, 128, D], Vc [pages, heads, D, 128] (values lie [dim][token]), D 64 or
+ * 128, Ks / Vs f32 [pages, heads]: one power-of-two scale per page and head.  block_table int32 [seqs, pages per sequence],
+ * seq_lens int32 [seqs]: tokens of each sequence INCLUDING the new ones; cu_seqlens int32 [seqs + 1]: sequence b's new
+ * tokens are rows [cu[b], cu[b + 1]) of the batch, its last positions (null: one row per sequence).  Entries of these
+ * tables are read on the device: pages outside [0, pages) and positions below 0 or past the table are neither read nor
+ * written.  A page that is written belongs to one sequence.
+ *
+ * write: K, V [T, heads, D] bf16 / f16.  Scale of a (page, head): smallest 2^e, -60 <= e <= 60, with amax / 2^e <= 448 over
+ * the finite new values; a page that holds earlier tokens keeps the larger of its scale and the new one, and moves its
+ * bytes if that grew.  inv_freq not null: keys are rotated at their positions and rounded to 16 bits first, and Q (may be
+ * null) is rotated into Qo.
+ * read: Ko, Vo [seqs, max_len, heads, D] contiguous, bf16 / f16; rows behind a sequence's length are zero. */
+TG_API int32_t tg_kv_cache_write(const TgTensorDesc* Kc, const TgTensorDesc* Vc, const TgTensorDesc* Ks, const TgTensorDesc* Vs,
+                                 const TgTensorDesc* K, const TgTensorDesc* V, const TgTensorDesc* block_table,
+                                 const TgTensorDesc* seq_lens, const TgTensorDesc* cu_seqlens, const TgTensorDesc* Qo,
+                                 const TgTensorDesc* Q, const TgTensorDesc* inv_freq, int32_t interleaved, float magnitude,
+                                 int32_t device_id, uint64_t stream);
+TG_API int32_t tg_kv_cache_read(const TgTensorDesc* Ko, const TgTensorDesc* Vo, const TgTensorDesc* Kc, const TgTensorDesc* Vc,
+                                const TgTensorDesc* Ks, const TgTensorDesc* Vs, const TgTensorDesc* block_table,
+                                const TgTensorDesc* seq_lens, int32_t device_id, uint64_t stream);
+
+/* Causal attention of the new tokens over the cache (which already holds them): Q, O [T, q_heads, D] bf16 / f16, q_heads a
+ * multiple of the cache's heads (at most 64 times).  A token at position i sees j <= i, and under a window (> 0) of those
+ * only j > i - window or j < sinks.  A token that sees nothing gets zeros.  max_q_len: no sequence has more new tokens than
+ * this (rows beyond it are not computed).  workspace: at least tg_paged_attention_workspace_bytes() bytes, 16-byte
+ * aligned, contents immaterial; calls that may overlap need one each. */
+TG_API uint64_t tg_paged_attention_workspace_bytes(int64_t tokens, int64_t q_heads, int64_t kv_heads, int64_t head_dim,
+                                                   int64_t seqs, int32_t max_q_len, int32_t num_sms);
+TG_API int32_t tg_paged_attention(const TgTensorDesc* O, const TgTensorDesc* Q, const TgTensorDesc* Kc, const TgTensorDesc* Vc,
+                                  const TgTensorDesc* Ks, const TgTensorDesc* Vs, const TgTensorDesc* block_table,
+                                  const TgTensorDesc* seq_lens, const TgTensorDesc* cu_seqlens, int32_t max_q_len, float scale,
+                                  int32_t window, int32_t sinks, uint64_t workspace, uint64_t workspace_bytes, int32_t device_id,
+                                  uint64_t stream);
 
 /* Library version, e.g. 100 for 0.1.0. */
 TG_API int32_t tg_version(void);

@@ -5,7 +5,8 @@ Public surface (same names and signatures as the reference operators):
     gemm_alpha_beta                                    (tilegym.suites.flashinfer.ops)
     matmul, bmm                                        (tilegym.ops)
 plus the per-tensor pieces the reference lacks (fp8_scaled_mm, fp8_block_scaled_mm, quant_per_tensor,
-weight_quant_block, FP8Linear) and apply_tilegym_kernel_to_llama / _deepseek_v2.
+weight_quant_block, FP8Linear), the decoder operators around the GEMMs (rms_norm_quant, apply_rope, kv_cache_write,
+kv_cache_read, paged_attention on an FP8KVCache) and apply_tilegym_kernel_to_llama / _deepseek_v2.
 """
 
 from .ops import (  # noqa: F401
@@ -22,12 +23,21 @@ from .ops import (  # noqa: F401
     matmul,
     quant_per_tensor,
     reset_workspaces,
+    rms_norm_quant,
     set_static_weights,
     w8a8_block_fp8_matmul,
     weight_dequant,
     weight_quant_block,
 )
 
+from .attention import (  # noqa: E402,F401
+    FP8KVCache,
+    apply_rope,
+    kv_cache_read,
+    kv_cache_write,
+    paged_attention,
+    rope_frequencies,
+)
 from .moe import FP8MoE, fused_experts_impl, fused_moe, moe_align_block_size  # noqa: E402,F401
 
 __version__ = "0.1.0"

@@ -42,6 +42,7 @@ DTYPE_CODES = {
     torch.uint8: 6,
     torch.float8_e4m3fn: 7,
     torch.int8: 8,  # extension: the reference table stops at 7
+    torch.float64: 9,  # extension: rotary frequencies
 }
 
 
@@ -147,6 +148,27 @@ SIGNATURES = {
         [_P, ctypes.c_uint64, _P, ctypes.c_uint64, ctypes.c_int32, ctypes.c_uint64],
     ),
     "tg_weight_quant_block": (ctypes.c_int32, [_P, _P, _P, ctypes.c_int32, ctypes.c_int32, ctypes.c_uint64]),
+    "tg_rms_norm_quant": (
+        ctypes.c_int32,
+        [_P, _P, _P, _P, _P, _P, ctypes.c_float, ctypes.c_float, ctypes.c_int32, ctypes.c_uint64],
+    ),
+    "tg_apply_rope": (
+        ctypes.c_int32,
+        [_P, _P, _P, _P, _P, _P, ctypes.c_int32, ctypes.c_float, ctypes.c_int32, ctypes.c_uint64],
+    ),
+    "tg_kv_cache_write": (
+        ctypes.c_int32,
+        [_P] * 12 + [ctypes.c_int32, ctypes.c_float, ctypes.c_int32, ctypes.c_uint64],
+    ),
+    "tg_kv_cache_read": (ctypes.c_int32, [_P] * 8 + [ctypes.c_int32, ctypes.c_uint64]),
+    "tg_paged_attention_workspace_bytes": (
+        ctypes.c_uint64, [ctypes.c_int64] * 5 + [ctypes.c_int32, ctypes.c_int32],
+    ),
+    "tg_paged_attention": (
+        ctypes.c_int32,
+        [_P] * 9 + [ctypes.c_int32, ctypes.c_float, ctypes.c_int32, ctypes.c_int32, ctypes.c_uint64, ctypes.c_uint64,
+                    ctypes.c_int32, ctypes.c_uint64],
+    ),
     "tg_device_status": (ctypes.c_int32, [ctypes.c_int32, ctypes.POINTER(ctypes.c_int32)]),
     "tg_reload_env": (None, []),
     "tg_set_wait_limit_us": (ctypes.c_uint32, [ctypes.c_uint32]),

@@ -1,0 +1,155 @@
+// Attention over the paged e4m3 key / value cache.
+//
+//   o_i = sum_j softmax_j(scale * q_i . k_j) v_j,  j <= pos_i  and  (j > pos_i - window  or  j < sinks)
+//
+// The simple form: one block per (new token, query head) walks the pages that the token sees, one thread per cached token
+// for the products with q, one thread per element of the head for the sums with v; running maximum and sum in 32 bits.
+#include <cstdio>
+
+#include "tg_attention.cuh"
+
+namespace tg {
+namespace {
+
+__device__ __forceinline__ float2 e4m3_two(uint32_t two) {
+  const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(two & 0xffffu), __NV_E4M3);
+  return __half22float2(*reinterpret_cast<const __half2*>(&h));
+}
+
+template <typename T, int DIM>
+__global__ void __launch_bounds__(128) tg_attention_simple_kernel(const AttentionParams p) {
+  __shared__ __align__(16) float q[DIM];
+  __shared__ float prob[kPage], red[4];
+  const int tok = blockIdx.x, head = blockIdx.y, tid = threadIdx.x;
+  griddep_wait();
+  griddep_launch_dependents();
+  int first, lo, hi;
+  const int b = find_sequence(p.c.cu, p.c.seqs, tok, 1, 0, first);
+  new_rows(p.c.cu, b, p.tokens, lo, hi);
+  if (tok < lo || tok >= hi) return;  // rows behind the last sequence
+  const int len = min(p.c.seq_lens[b], p.c.max_pages * kPage);
+  const int pos = p.c.seq_lens[b] - hi + tok;
+  const T* src = static_cast<const T*>(p.q) + tok * p.q_tok + head * p.q_head;
+  T* dst = static_cast<T*>(p.o) + tok * p.o_tok + head * p.o_head;
+  if (tid < DIM) q[tid] = static_cast<float>(src[tid]) * p.scale * 1.4426950408889634f;
+  __syncthreads();
+  const int kv = head / p.group;
+  const int64_t from = p.window > 0 ? max(static_cast<int64_t>(pos) - p.window + 1, int64_t(0)) : 0;
+  float m = -INFINITY, l = 0.f, acc = 0.f;
+  for (int page = 0; page * kPage < len && page * kPage <= pos; ++page) {
+    if ((page + 1) * static_cast<int64_t>(kPage) <= from && page * kPage >= p.sinks) continue;
+    const int phys = p.c.table[b * p.c.table_pitch + page];
+    if (phys < 0 || phys >= p.c.pages) continue;
+    const int64_t block = static_cast<int64_t>(phys) * p.c.heads + kv;
+    const int j = page * kPage + tid;
+    const bool seen = j < len && j <= pos && (j >= from || j < p.sinks);
+    float s = -INFINITY;
+    if (seen) {
+      const uint4* row = reinterpret_cast<const uint4*>(p.c.k + (block * kPage + tid) * DIM);
+      float dot = 0.f;
+#pragma unroll
+      for (int i = 0; i < DIM / 16; ++i) {
+        const uint4 w4 = row[i];
+        const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const float2 f = e4m3_two(w[k >> 1] >> (16 * (k & 1)));
+          dot = fmaf(f.x, q[i * 16 + 2 * k], dot);
+          dot = fmaf(f.y, q[i * 16 + 2 * k + 1], dot);
+        }
+      }
+      s = dot * p.c.ks[block];
+    }
+    float mx = s;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+    if ((tid & 31) == 0) red[tid >> 5] = mx;
+    __syncthreads();
+    const float m_new = fmaxf(m, fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3])));
+    const float base = m_new == -INFINITY ? 0.f : m_new;
+    const float shrink = exp2f(m - base);
+    m = m_new;
+    prob[tid] = seen ? exp2f(s - base) : 0.f;
+    __syncthreads();
+    const float vs = p.c.vs[block];
+    float sum = 0.f, part = 0.f;
+    const int j0 = page * kPage;
+    for (int t = 0; t < kPage; ++t) {
+      const int at = j0 + t;
+      if (at >= len || at > pos || !(at >= from || at < p.sinks)) continue;
+      sum += prob[t];
+      if (tid < DIM) part = fmaf(prob[t], e4m3_two(p.c.v[(block * DIM + tid) * kPage + t]).x, part);
+    }
+    l = l * shrink + sum;
+    acc = acc * shrink + part * vs;
+    __syncthreads();
+  }
+  if (tid < DIM) dst[tid] = static_cast<T>(l > 0.f || l != l ? acc / l : 0.f);
+}
+
+}  // namespace
+}  // namespace tg
+
+using namespace tg;
+
+extern "C" TG_API uint64_t tg_paged_attention_workspace_bytes(int64_t, int64_t, int64_t, int64_t, int64_t, int32_t, int32_t) { return 0; }
+
+extern "C" TG_API int32_t tg_paged_attention(const TgTensorDesc* O, const TgTensorDesc* Q, const TgTensorDesc* Kc, const TgTensorDesc* Vc,
+                                             const TgTensorDesc* Ks, const TgTensorDesc* Vs, const TgTensorDesc* block_table,
+                                             const TgTensorDesc* seq_lens, const TgTensorDesc* cu_seqlens, int32_t max_q_len, float scale,
+                                             int32_t window, int32_t sinks, uint64_t workspace, uint64_t workspace_bytes, int32_t device_id,
+                                             uint64_t stream) {
+  AttentionParams p = {};
+  int32_t rc;
+  if ((rc = check_cache(&p.c, Kc, Vc, Ks, Vs, block_table, seq_lens, cu_seqlens)) != TG_OK) return rc;
+  if (Q == nullptr || O == nullptr) return api_fail(TG_ERR_NULL, "q or output descriptor is null");
+  if (!is_16bit(Q->dtype)) return api_fail(TG_ERR_DTYPE, "q must be bf16 or f16");
+  if (Q->ndim != 3) return api_fail(TG_ERR_ARGS, "q must be [tokens, heads, head_dim]");
+  const int64_t T = Q->shape[0], heads = Q->shape[1], D = p.c.dim;
+  if (T > (1 << 28)) return api_fail(TG_ERR_ARGS, "too many tokens");
+  if (cu_seqlens == nullptr && T != p.c.seqs) return api_fail(TG_ERR_ARGS, "without cu_seqlens there is one new token per sequence");
+  if (heads < 1 || heads % p.c.heads != 0 || heads / p.c.heads > 64)
+    return api_fail(TG_ERR_ARGS, "the query heads must be a multiple of the cache's heads, at most 64 times as many");
+  if ((rc = check_heads(Q, "q: [tokens, heads, head_dim of the cache], 16-byte aligned", T, heads, D, Q->dtype)) != TG_OK) return rc;
+  if ((rc = check_heads(O, "output: shape and type of q, 16-byte aligned", T, heads, D, Q->dtype)) != TG_OK) return rc;
+  if (max_q_len < 1) return api_fail(TG_ERR_ARGS, "max_q_len must be at least 1");
+  if (window < 0 || sinks < 0) return api_fail(TG_ERR_ARGS, "window and sinks must not be negative");
+  if (sinks > 0 && window == 0) return api_fail(TG_ERR_ARGS, "sinks only mean something under a window");
+  if (!(scale > 0.f) || scale > 3.0e38f) return api_fail(TG_ERR_ARGS, "scale must be positive and finite");
+  if (T == 0 || p.c.seqs == 0) return TG_OK;
+  ScopedDevice guard(device_id);
+  if (guard.err != cudaSuccess) {
+    cudaGetLastError();
+    return api_fail(TG_ERR_DEVICE, "cannot select the CUDA device");
+  }
+  int num_sms = 0;
+  int32_t* status = nullptr;
+  if ((rc = api_init_device(device_id, &num_sms, &status)) != TG_OK) return rc;
+  p.q = reinterpret_cast<const void*>(Q->ptr);
+  p.o = reinterpret_cast<void*>(O->ptr);
+  p.q_tok = Q->strides[0];
+  p.q_head = Q->strides[1];
+  p.o_tok = O->strides[0];
+  p.o_head = O->strides[1];
+  p.tokens = static_cast<int32_t>(T);
+  p.q_heads = static_cast<int32_t>(heads);
+  p.group = static_cast<int32_t>(heads / p.c.heads);
+  p.scale = scale;
+  p.window = window;
+  p.sinks = sinks;
+  const cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  const dim3 grid(static_cast<unsigned>(T), static_cast<unsigned>(heads)), block(128);
+  cudaError_t e;
+  if (Q->dtype == TG_BF16)
+    e = D == 128 ? launch_pdl(tg_attention_simple_kernel<__nv_bfloat16, 128>, grid, block, 0, st, p)
+                 : launch_pdl(tg_attention_simple_kernel<__nv_bfloat16, 64>, grid, block, 0, st, p);
+  else
+    e = D == 128 ? launch_pdl(tg_attention_simple_kernel<__half, 128>, grid, block, 0, st, p)
+                 : launch_pdl(tg_attention_simple_kernel<__half, 64>, grid, block, 0, st, p);
+  if (e != cudaSuccess) {
+    char msg[160];
+    snprintf(msg, sizeof(msg), "paged_attention launch failed: %s", cudaGetErrorString(e));
+    return api_fail(TG_ERR_LAUNCH, msg);
+  }
+  return TG_OK;
+}

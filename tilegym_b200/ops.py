@@ -315,6 +315,68 @@ def per_token_group_quant_8bit(
     return x_q, x_s
 
 
+def _no_grad_inputs(*tensors: Optional[torch.Tensor]) -> None:
+    """The package has forward kernels only: a result that silently cuts the graph is refused."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise RuntimeError("tilegym_b200 operators have no backward: call them under torch.no_grad() or detach the inputs")
+
+
+def rms_norm_quant(
+    x: torch.Tensor,
+    weight: torch.Tensor,
+    eps: float = 1e-6,
+    residual: Optional[torch.Tensor] = None,
+    weight_offset: float = 0.0,
+    inplace: bool = False,
+) -> Tuple[torch.Tensor, ...]:
+    """RMS norm fused with the residual's addition and `act_quant`: (y e4m3, s f32 per 128 values[, h]).
+
+    h = x + residual rounded to x's type (the residual stream's next value; without a residual h = x and is not
+    returned), y = h * rsqrt(mean(h^2) + eps) * (weight + weight_offset) in fp32, then quantised per 1 x 128 block with
+    `act_quant`'s rule (scale amax / 448, 1.0 for an all-zero block) without being rounded to 16 bits on the way.  What
+    `fp8_block_scaled_mm` takes as A / As.  x, residual (..., hidden) bf16 or f16, hidden a multiple of 128 up to
+    65536; weight (hidden,) in x's type or fp32.  With inplace=True h is written over `residual`.
+    """
+    dev = _need_cuda(x, weight, residual)
+    _no_grad_inputs(x, residual)
+    hidden = x.shape[-1]
+    if x.dtype not in (torch.bfloat16, torch.float16):
+        raise _lib.TileGymB200Error(-2, f"rms_norm_quant takes bf16 or f16, got {x.dtype}")
+    assert hidden % 128 == 0 and hidden > 0, "the hidden size must be a multiple of 128"
+    assert weight.shape == (hidden,), "weight must hold one value per hidden element"
+    x2 = _rows16(x.reshape(-1, hidden))
+    T = x2.shape[0]
+    y = torch.empty(x.shape, dtype=_FP8, device=dev)
+    s = torch.empty(x.shape[:-1] + (hidden // 128,), dtype=torch.float32, device=dev)
+    r2 = h = None
+    if residual is not None:
+        assert residual.shape == x.shape and residual.dtype == x.dtype, "residual must have x's shape and type"
+        if inplace:
+            assert residual.is_contiguous() and residual.data_ptr() % 16 == 0, "an in-place residual must be contiguous and 16-byte aligned"
+            h = residual
+        else:
+            h = torch.empty(x.shape, dtype=x.dtype, device=dev)
+        r2 = _rows16(residual.reshape(-1, hidden))
+    else:
+        assert not inplace, "inplace=True writes the sum over the residual: there is none"
+    if not weight.is_contiguous() or weight.data_ptr() % 16:
+        weight = weight.clone(memory_format=torch.contiguous_format)
+    rc = _lib.lib().tg_rms_norm_quant(
+        _lib.desc2d(y.data_ptr(), T, hidden, hidden, _FP8), _lib.desc2d(s.data_ptr(), T, hidden // 128, hidden // 128, torch.float32),
+        _lib.desc2d(h.data_ptr(), T, hidden, hidden, h.dtype) if h is not None else None, _lib.desc(x2), _lib.desc(r2),
+        _lib.desc(weight), float(eps), float(weight_offset), dev.index, _stream(dev),
+    )
+    _lib.check_rc(rc)
+    return (y, s) if h is None else (y, s, h)
+
+
+def _rows16(x2: torch.Tensor) -> torch.Tensor:
+    """A 2-D tensor whose rows are dense and start on 16-byte boundaries (itself, or a copy)."""
+    if x2.stride(1) != 1 or x2.data_ptr() % 16 or x2.stride(0) * x2.element_size() % 16:
+        return x2.clone(memory_format=torch.contiguous_format)
+    return x2
+
+
 def weight_dequant(
     x: torch.Tensor, s: torch.Tensor, block_size: int = 128, dtype: torch.dtype = torch.bfloat16
 ) -> torch.Tensor:
