@@ -81,10 +81,10 @@ def cache_values(cache, block_table_row, length):
 
 
 def ref_attention(q, cache, block_table, seq_lens, cu, scale=None, window=0, sinks=0):
-    """(o, sum of p |v|, largest scale * sum |q k| of what a row sees) [tokens, heads, dim] (the last: dim 1) in f64; rows
-    outside cu are zero."""
+    """(o, sum of p |v|, largest scale * sum |q k| of what a row sees [.., 1], largest p * v_scale times the sum of the
+    bytes' |v|) [tokens, heads, dim] in f64; rows outside cu are zero."""
     T, Hq, D = q.shape
-    o, mag, size = (torch.zeros(T, Hq, n, dtype=torch.float64) for n in (D, D, 1))
+    o, mag, size, coarse = (torch.zeros(T, Hq, n, dtype=torch.float64) for n in (D, D, 1, D))
     scale = D**-0.5 if scale is None else scale
     for b, length in enumerate(seq_lens.tolist()):
         lo, hi = int(cu[b]), int(cu[b + 1])
@@ -112,4 +112,7 @@ def ref_attention(q, cache, block_table, seq_lens, cu, scale=None, window=0, sin
             mag[lo:hi].view(hi - lo, H, g, D)[:, h] = (p @ vv.abs()).transpose(0, 1)
             a = (rows.abs() @ k[h].abs().T * scale).masked_fill(~seen, 0.0).amax(-1, keepdim=True)
             size[lo:hi].view(hi - lo, H, g, 1)[:, h] = a.transpose(0, 1)
-    return o, mag, size
+            vs = cache[3][block_table[b, : -(-length // PAGE)].long(), h].double().repeat_interleave(PAGE)[:length]
+            top = (p * vs).amax(-1, keepdim=True) * (seen.double() @ (vv.abs() / vs[:, None]))
+            coarse[lo:hi].view(hi - lo, H, g, D)[:, h] = top.transpose(0, 1)
+    return o, mag, size, coarse

@@ -320,25 +320,28 @@ def test_read(dev, heads, dim, dtype):
 
 
 # ------------------------------------------------------------------ paged_attention
-#: what the probabilities may be off by, relative, before they meet the values
-P_ERROR = {BF: 0.0, HF: 0.0}
+#: What the probabilities may be off by, relative, before they meet the values: the kernels split them into e4m3 terms, each
+#: rounding half a step (2^-4) of what the one before left: two for bf16, three for f16.
+P_ERROR = {BF: 2.0**-8, HF: 2.0**-12}
 
 
-def allowed(dtype, o, mag, size):
+def allowed(dtype, o, mag, size, coarse):
     """Half a step of o, and of sum p |v|: the probabilities' rounding, and 32-bit noise.  A logit is a sum of 128 products in
     32 bits, off by at most 128 * 2^-24 of the sum of their magnitudes (`size`), which moves a probability by as much,
     relative; numerator and denominator: 2^-16 * size.  exp, sums and the running maximum's rescaling: 2^-14.
+    The terms end at half of e4m3's smallest step, 2^-10, where the row's largest p * v_scale is 2^7 or more: 2^-17 of that
+    times the values' bytes (`coarse`).
     A probability under 2^-126 of the largest is 0 in 32 bits: 2^-126 * 448 * 2^12 (the largest scale here) * 1000 tokens."""
     tiny = 2.0**-25 if dtype == HF else 2.0**-95
-    return half_step(dtype) * o.abs() + (P_ERROR[dtype] + 2.0**-16 * size + 2.0**-14) * mag + tiny
+    return half_step(dtype) * o.abs() + (P_ERROR[dtype] + 2.0**-16 * size + 2.0**-14) * mag + 2.0**-17 * coarse + tiny
 
 
 def check_attention(dev, q, ref, table, lens, new, got=None, **kw):
     cu = cumulative(new)
     if got is None:
         got = tg.paged_attention(q.to(dev), on(dev, ref), table.to(dev), i32(lens).to(dev), cu.to(dev), max_q_len=max(new + [1]), **kw)
-    o, mag, size = D.ref_attention(q, ref, table, i32(lens), cu, **{k: v for k, v in kw.items() if k in ("scale", "window", "sinks")})
-    bound = allowed(q.dtype, o, mag, size)
+    o, mag, *rest = D.ref_attention(q, ref, table, i32(lens), cu, **{k: v for k, v in kw.items() if k in ("scale", "window", "sinks")})
+    bound = allowed(q.dtype, o, mag, *rest)
     n = int(cu[-1])
     diff = (got.cpu().double() - o).abs()[:n]
     assert bool((diff <= bound[:n]).all()), float((diff / (mag[:n] + 1e-30)).max())
@@ -416,6 +419,8 @@ def test_attention_nan_stays_with_those_who_see_it(dev):
         got = tg.paged_attention(q.to(dev), on(dev, ref), table.to(dev), i32(lens).to(dev), i32([0, 1, 141]).to(dev), max_q_len=140, **kw)
         bad = got.isnan().cpu()
         assert bool(bad[0].all()) == (not kw) and bool(bad[0].any()) == (not kw)
+        small = tg.paged_attention(q[:5].to(dev), on(dev, ref), table[1:].to(dev), i32([323]).to(dev), i32([0, 5]).to(dev), max_q_len=5, **kw)
+        assert bool(small[2:, :, 7].isnan().all()) and int(small.isnan().sum()) == 3 * 4  # positions 318 .. 322
         want = torch.zeros_like(bad[1:])
         want[60:, :, 7] = True  # positions 260 .. 399: rows from 320 on see it
         assert torch.equal(bad[1:], want)

@@ -388,6 +388,17 @@ int32_t api_check_output(const TgTensorDesc* C, int64_t M, int64_t N) { return c
 int32_t api_make_map(CUtensorMap* map, uint64_t ptr, int64_t rows, int64_t K, int64_t pitch, int box_rows) {
   return make_map(map, ptr, rows, K, pitch, box_rows);
 }
+int32_t api_make_page_map(CUtensorMap* map, uint64_t ptr, int64_t rows, int cols, int box_rows) {
+  cuuint64_t dims[2] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows)};
+  cuuint64_t strides[1] = {static_cast<cuuint64_t>(cols)};
+  cuuint32_t box[2] = {static_cast<cuuint32_t>(cols), static_cast<cuuint32_t>(box_rows)};
+  cuuint32_t estr[2] = {1u, 1u};
+  CUresult r = g_encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, reinterpret_cast<void*>(ptr), dims, strides, box, estr,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, cols == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
+                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(TG_ERR_ARGS, "cuTensorMapEncodeTiled (cache) failed with CUresult %d", static_cast<int>(r));
+  return TG_OK;
+}
 uint32_t api_wait_limit_us() { return g_wait_limit_us; }
 int32_t api_init_device(int dev, int* num_sms, int32_t** status) {
   int32_t rc = init_device(dev);

@@ -92,7 +92,21 @@ __global__ void __launch_bounds__(128) tg_attention_simple_kernel(const Attentio
 
 using namespace tg;
 
-extern "C" TG_API uint64_t tg_paged_attention_workspace_bytes(int64_t, int64_t, int64_t, int64_t, int64_t, int32_t, int32_t) { return 0; }
+// Rows of a unit in the kernel for few rows, 0 where the batch has too many for it.
+static int few_rows_of(int64_t q_heads, int64_t kv_heads, int32_t max_q_len) {
+  if (q_heads < 1 || kv_heads < 1 || max_q_len < 1) return 0;
+  const int64_t rows = q_heads / kv_heads * max_q_len;
+  return rows <= kFewRowsMax ? few_rows_padded(static_cast<int>(rows)) : 0;
+}
+
+extern "C" TG_API uint64_t tg_paged_attention_workspace_bytes(int64_t, int64_t q_heads, int64_t kv_heads, int64_t head_dim, int64_t,
+                                                              int32_t max_q_len, int32_t num_sms) {
+  const int rows = few_rows_of(q_heads, kv_heads, max_q_len);
+  if (rows == 0) return 0;
+  const int dim = head_dim == 64 ? 64 : 128;
+  // the larger of the two types' block counts
+  return few_rows_workspace(dim, rows, few_rows_blocks(dim, rows, true, num_sms));
+}
 
 extern "C" TG_API int32_t tg_paged_attention(const TgTensorDesc* O, const TgTensorDesc* Q, const TgTensorDesc* Kc, const TgTensorDesc* Vc,
                                              const TgTensorDesc* Ks, const TgTensorDesc* Vs, const TgTensorDesc* block_table,
@@ -117,6 +131,7 @@ extern "C" TG_API int32_t tg_paged_attention(const TgTensorDesc* O, const TgTens
   if (sinks > 0 && window == 0) return api_fail(TG_ERR_ARGS, "sinks only mean something under a window");
   if (!(scale > 0.f) || scale > 3.0e38f) return api_fail(TG_ERR_ARGS, "scale must be positive and finite");
   if (T == 0 || p.c.seqs == 0) return TG_OK;
+  if (p.c.pages < 1) return api_fail(TG_ERR_ARGS, "the cache has no page");
   ScopedDevice guard(device_id);
   if (guard.err != cudaSuccess) {
     cudaGetLastError();
@@ -137,7 +152,29 @@ extern "C" TG_API int32_t tg_paged_attention(const TgTensorDesc* O, const TgTens
   p.scale = scale;
   p.window = window;
   p.sinks = sinks;
+  p.max_q_len = max_q_len;
+  p.status = status;
+  p.wait_limit_us = api_wait_limit_us();
   const cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  if (const int rows = few_rows_of(heads, p.c.heads, max_q_len); rows > 0) {
+    const int blocks = few_rows_blocks(p.c.dim, rows, Q->dtype == TG_BF16, num_sms);
+    if (workspace == 0) return api_fail(TG_ERR_NULL, "the workspace is null");
+    if (workspace & 15u) return api_fail(TG_ERR_ALIGN, "the workspace must be 16-byte aligned");
+    if (workspace_bytes < few_rows_workspace(p.c.dim, rows, blocks)) return api_fail(TG_ERR_ARGS, "the workspace is too small");
+    const uint64_t parts = 2ull * blocks * rows;
+    p.part_o = reinterpret_cast<float*>(workspace);
+    p.part_ml = reinterpret_cast<float2*>(workspace + parts * p.c.dim * 4);
+    p.record = reinterpret_cast<int4*>(workspace + parts * p.c.dim * 4 + parts * 8);
+    CUtensorMap tmK, tmV;
+    const int64_t page_heads = static_cast<int64_t>(p.c.pages) * p.c.heads;
+    if ((rc = api_make_page_map(&tmK, Kc->ptr, page_heads * kPage, p.c.dim, kPage)) != TG_OK) return rc;
+    if ((rc = api_make_page_map(&tmV, Vc->ptr, page_heads * p.c.dim, kPage, p.c.dim)) != TG_OK) return rc;
+    const cudaError_t e = launch_attention_few_rows(tmK, tmV, p, rows, blocks, Q->dtype == TG_BF16, st);
+    if (e == cudaSuccess) return TG_OK;
+    char msg[160];
+    snprintf(msg, sizeof(msg), "paged_attention launch failed: %s", cudaGetErrorString(e));
+    return api_fail(TG_ERR_LAUNCH, msg);
+  }
   const dim3 grid(static_cast<unsigned>(T), static_cast<unsigned>(heads)), block(128);
   cudaError_t e;
   if (Q->dtype == TG_BF16)

@@ -1,0 +1,732 @@
+// Attention over the paged e4m3 cache for few rows: R = (new tokens of a sequence) * (query heads of a cache head) <= 64.
+//
+// The cache's bytes are read once and are nearly all of the work, so the kernel is built to keep copies in flight, and the
+// cached bytes ARE the tensor core's operands: no conversion, no transposition.
+//
+//   S^T [128 tokens, R]  = K [128, dim] . Q^T           kind::f8f6f4, q = q1 + q2 (+ q3) in e4m3, summed by the accumulator
+//   p = 2^(S * scale * log2 e + log2 v_scale - ref)     thread = token; v_scale of the page rides in the exponent
+//   O^T [dim, R]        += V^T [dim, 128] . P           p = p1 + p2 (+ p3) in e4m3, the same way
+//
+// The two factors that are not in the cache are split into sums of e4m3 values (split_e4m3): two terms hold a bf16 q exactly
+// and p to 2^-8, three (f16) both to 2^-12.  `ref` is a running maximum of the
+// exponent that is only moved when it would grow by more than one (a power of two of headroom is left for that under
+// e4m3's 448), which rescales O^T in TMEM.  Keeping v_scale in the exponent keeps p at one magnitude whatever the pages'
+// scales are.
+//
+// Work: the pages that the units (sequence, cache head) see are numbered through, and every block takes an equal range of
+// them, wherever that begins and ends: no batch is too ragged.  A block that ends inside a unit leaves a partial result and
+// a record; the joining kernel adds the parts of such a unit in block order, so results do not depend on timing.
+// Warp 0 copies pages (TMA, a ring of page pairs), warp 1 issues the products, warps 2-5 do the softmax.
+#include <cstdio>
+
+#include "tg_attention.cuh"
+
+namespace tg {
+namespace {
+
+constexpr int kThreads = 192;
+constexpr float kHeadroom = 7.f;  // p is kept times 2^7; it may reach 2^8 before ref moves
+
+template <typename T>
+constexpr int kTermsOf = std::is_same<T, __half>::value ? 3 : 2;
+
+template <int DIM, int N, int TERMS>
+struct Shape {
+  static constexpr int kTile = DIM * kPage;  // bytes of a key or value page
+  static constexpr int kP = TERMS * N * kPage;
+  static constexpr int kQ = TERMS * N * DIM;
+  // two blocks share an SM where each still has a ring of three page pairs
+  static constexpr int kBlocksPerSm = N == 16 && !(TERMS == 3 && DIM == 128) ? 2 : 1;
+  static constexpr int kMisc = 4096;
+  // dim 64: the value operand is read as 128 rows, 64 of them whatever follows the page
+  static constexpr int kBudget = (kBlocksPerSm == 2 ? 113 : 226) * 1024 - 1024 - 2 * kP - kQ - kMisc;
+  static constexpr int kStages = kBudget / (2 * kTile) > 8 ? 8 : kBudget / (2 * kTile);
+  static constexpr int kSmem = 1024 + kStages * 2 * kTile + 2 * kP + kQ + kMisc;
+  static constexpr int kTmem = N == 16 ? 64 : N == 32 ? 128 : 256;  // S^T twice and O^T, a power of two
+  static_assert(kStages >= 3, "the ring is too short to hide the latency of a page");
+  static_assert(2 * kP + kQ >= 8192, "the value operand of dim 64 reads 8 KB behind its page");
+};
+
+struct TileInfo {
+  float ks, lv, inv_vs;
+  int base;  // position of the page's first token; -1: no such page
+};
+
+// A bounded wait whose outcome is the same for the whole warp, which is converged behind it.
+template <bool kHint = false>
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile uint32_t* abort_flag) {
+  return __all_sync(0xffffffffu, mbar_wait<kHint>(bar, parity, abort_flag));
+}
+
+// The units are numbered sequence by sequence, the cache heads of a sequence next to one another.
+struct Cursor {
+  int b, h;
+  SeqView v;
+};
+__device__ __forceinline__ bool next_unit(const AttentionParams& p, Cursor& c) {
+  if (++c.h < p.c.heads) return true;
+  c.h = 0;
+  do {
+    if (++c.b >= p.c.seqs) return false;
+    c.v = view_sequence(p, c.b, 0, p.max_q_len);
+  } while (c.v.tiles == 0);
+  return true;
+}
+
+template <typename T, int DIM, int N>
+__global__ void __launch_bounds__(kThreads, (Shape<DIM, N, kTermsOf<T>>::kBlocksPerSm))
+    tg_attention_few_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const AttentionParams p) {
+  constexpr int kTerms = kTermsOf<T>;
+  using Sh = Shape<DIM, N, kTerms>;
+  constexpr int kStages = Sh::kStages;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* p_smem = smem + kStages * 2 * Sh::kTile;
+  uint8_t* q_smem = p_smem + 2 * Sh::kP;
+  uint8_t* misc = q_smem + Sh::kQ;
+  // misc: barriers, tile notes, row factors, exchanged maxima
+  uint64_t* bars = reinterpret_cast<uint64_t*>(misc);
+  TileInfo* info = reinterpret_cast<TileInfo*>(misc + 512);
+  volatile uint32_t* abort_flag = reinterpret_cast<volatile uint32_t*>(misc + 512 + 8 * sizeof(TileInfo));
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(misc + 512 + 8 * sizeof(TileInfo) + 16);
+  int64_t* sched = reinterpret_cast<int64_t*>(misc + 512 + 8 * sizeof(TileInfo) + 32);  // 0 total, 1 prefix, 2 sequence, 3.. warp sums
+  float* rowmul = reinterpret_cast<float*>(misc + 1024);
+  float4* wmax = reinterpret_cast<float4*>(misc + 2048);  // [2][N] of four warps' maxima; also the sums' exchange
+
+  const uint32_t bar0 = smem_u32(bars);
+  const uint32_t b_full = bar0, b_empty = bar0 + 8 * kStages, b_sfull = b_empty + 8 * kStages, b_sempty = b_sfull + 16,
+                 b_pready = b_sempty + 16, b_pvdone = b_pready + 16, b_qready = b_pvdone + 16, b_xchg = b_qready + 8;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  if (warp == 0) {
+    if (elect_one()) {
+      prefetch_tmap(&tmK);
+      prefetch_tmap(&tmV);
+    }
+    if (lane == 0) {
+      for (int i = 0; i < kStages; ++i) {
+        mbar_init(b_full + 8 * i, 1);
+        mbar_init(b_empty + 8 * i, 1);
+      }
+      for (int i = 0; i < 2; ++i) {
+        mbar_init(b_sfull + 8 * i, 1);
+        mbar_init(b_sempty + 8 * i, 4);
+        mbar_init(b_pready + 8 * i, 4);
+        mbar_init(b_pvdone + 8 * i, 1);
+        mbar_init(b_xchg + 8 * i, 4);
+      }
+      mbar_init(b_qready, 4);
+      init_abort_flag(abort_flag, p.wait_limit_us);
+      fence_mbar_init();
+    }
+  } else if (warp == 1) {
+    tmem_alloc(smem_u32(tmem_slot), Sh::kTmem);
+    tmem_relinquish();
+  }
+  // rows of P that no query has stay zero, and so do their columns of O^T
+  for (int i = threadIdx.x; i < (2 * Sh::kP + Sh::kQ) / 16; i += kThreads) reinterpret_cast<uint4*>(p_smem)[i] = make_uint4(0, 0, 0, 0);
+  fence_proxy_async_smem();
+  griddep_wait();
+  griddep_launch_dependents();
+
+  // ---- this block's range of pages
+  {
+    int64_t sum = 0;
+    for (int b = threadIdx.x; b < p.c.seqs; b += kThreads) sum += view_sequence(p, b, 0, p.max_q_len).tiles;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (lane == 0) sched[3 + warp] = sum;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      int64_t t = 0;
+      for (int w = 0; w < kThreads / 32; ++w) t += sched[3 + w];
+      sched[0] = t * p.c.heads;
+      sched[1] = 0;
+      sched[2] = -1;
+    }
+    __syncthreads();
+  }
+  const int64_t total = sched[0];
+  const int64_t blocks = min(static_cast<int64_t>(gridDim.x), total);  // the others have nothing to do
+  const bool mine_any = blockIdx.x < blocks;
+  const int64_t begin = mine_any ? total * blockIdx.x / blocks : 0, end = mine_any ? total * (blockIdx.x + 1) / blocks : 0;
+  if (begin < end) {
+    const int64_t target = begin / p.c.heads;
+    int64_t before = 0;
+    for (int base = 0; base < p.c.seqs; base += kThreads) {
+      const int b = base + threadIdx.x;
+      const int mine = b < p.c.seqs ? view_sequence(p, b, 0, p.max_q_len).tiles : 0;
+      int64_t incl = mine;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int64_t up = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += up;
+      }
+      __syncthreads();
+      if (lane == 31) sched[3 + warp] = incl;
+      __syncthreads();
+      int64_t off = before, all = before;
+      for (int w = 0; w < kThreads / 32; ++w) {
+        if (w < warp) off += sched[3 + w];
+        all += sched[3 + w];
+      }
+      if (mine > 0 && off + incl - mine <= target && target < off + incl) {
+        sched[1] = off + incl - mine;
+        sched[2] = b;
+      }
+      before = all;
+      if (before > target) break;  // the same for every thread
+    }
+    __syncthreads();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  const uint32_t t_o = tmem + 2 * N;
+
+  Cursor cur;
+  cur.b = static_cast<int>(sched[2]);
+  int t0 = 0;
+  const bool work = begin < end && cur.b >= 0;
+  if (work) {
+    cur.v = view_sequence(p, cur.b, 0, p.max_q_len);
+    const int64_t rem = begin - sched[1] * p.c.heads;
+    cur.h = static_cast<int>(rem / cur.v.tiles);
+    t0 = static_cast<int>(rem - static_cast<int64_t>(cur.h) * cur.v.tiles);
+  } else if (threadIdx.x == 0) {
+    p.record[blockIdx.x] = make_int4(-1, 0, 0, 0);
+  }
+  int64_t left = work ? end - begin : 0;
+  bool ok = true;
+  int site = 0;
+
+  if (warp == 0) {
+    // ------------------------------------------------------------------------------------------ copies
+    const uint64_t policy = policy_evict_first();
+    const int rows_k = p.c.pages * p.c.heads * kPage, rows_v = p.c.pages * p.c.heads * DIM;
+    int it = 0;
+    while (left > 0 && ok) {
+      const int t1 = static_cast<int>(min(static_cast<int64_t>(cur.v.tiles), t0 + left));
+      left -= t1 - t0;
+      for (int base = t0; base < t1 && ok; base += 32) {
+        // 32 pages at a time: numbers first, so that copies start before the scales are here
+        const int t = base + lane;
+        const int page = t < t1 ? cur.v.page_of(t) : p.c.max_pages;
+        int phys = page < p.c.max_pages ? p.c.table[cur.b * p.c.table_pitch + page] : -1;
+        if (phys < 0 || phys >= p.c.pages) phys = -1;
+        const int64_t block = static_cast<int64_t>(phys) * p.c.heads + cur.h;
+        float ks = 0.f, vs = 1.f;
+        if (phys >= 0) {
+          ks = p.c.ks[block];
+          vs = p.c.vs[block];
+        }
+        for (int i = 0; i < min(32, t1 - base); ++i, ++it) {
+          const int stage = it % kStages, round = it / kStages;
+          if (!warp_wait<true>(b_empty + 8 * stage, (round & 1) ^ 1, abort_flag)) {
+            ok = false;
+            site = 1;
+            break;
+          }
+          const int ph = __shfl_sync(0xffffffffu, phys, i);
+          // a page that is not there: a box behind the end of the cache, which reads as zeros
+          const int yk = ph >= 0 ? (ph * p.c.heads + cur.h) * kPage : rows_k;
+          const int yv = ph >= 0 ? (ph * p.c.heads + cur.h) * DIM : rows_v;
+          const uint32_t dst = smem_u32(smem + stage * 2 * Sh::kTile);
+          if (elect_one()) {
+            tma_load_2d_hint(dst, &tmK, b_full + 8 * stage, 0, yk, policy);
+            tma_load_2d_hint(dst + Sh::kTile, &tmV, b_full + 8 * stage, 0, yv, policy);
+          }
+          __syncwarp();
+          const float k1 = __shfl_sync(0xffffffffu, ks, i), v1 = __shfl_sync(0xffffffffu, vs, i);
+          if (elect_one()) {
+            info[stage] = TileInfo{k1, log2f(v1), 1.0f / v1, ph >= 0 ? cur.v.page_of(base + i) * kPage : -1};
+            mbar_arrive_expect_tx(b_full + 8 * stage, 2 * Sh::kTile);
+          }
+          __syncwarp();
+        }
+      }
+      t0 = 0;
+      if (left > 0 && !next_unit(p, cur)) break;
+    }
+    if (!ok) {
+      if (lane == 0) *p.status = kRoleProducer * 1000 + site;
+      // copies still in flight land before the block leaves (a bounded number of parked tries each)
+      for (int i = max(it - kStages, 0); i < it; ++i)
+        for (int tries = 0; tries < 1000 && !mbar_try_wait(b_full + 8 * (i % kStages), (i / kStages) & 1); ++tries) {
+        }
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------------------------------------ products
+    constexpr uint32_t idesc = make_idesc_e4m3_f32(128, N);
+    const uint32_t q_addr = smem_u32(q_smem), p_addr = smem_u32(p_smem);
+    int it = 0, unit = 0;
+    auto issue_pv = [&](int i, bool first) {
+      const int stage = i % kStages, buf = i & 1;
+      if (!warp_wait(b_pready + 8 * buf, (i >> 1) & 1, abort_flag)) return false;
+      tc_fence_after();
+      if (elect_one()) {
+        const uint64_t a = make_kmajor_sw128_desc(smem_u32(smem + stage * 2 * Sh::kTile + Sh::kTile));
+#pragma unroll
+        for (int term = 0; term < kTerms; ++term) {
+          const uint64_t b = make_kmajor_sw128_desc(p_addr + buf * Sh::kP + term * N * kPage);
+#pragma unroll
+          for (int k = 0; k < kPage / 32; ++k) mma_f8f6f4(t_o, a + 2 * k, b + 2 * k, idesc, !(first && term == 0 && k == 0));
+        }
+        tc_commit(b_empty + 8 * stage);
+        tc_commit(b_pvdone + 8 * buf);
+      }
+      __syncwarp();
+      return true;
+    };
+    while (left > 0 && ok) {
+      const int t1 = static_cast<int>(min(static_cast<int64_t>(cur.v.tiles), t0 + left));
+      left -= t1 - t0;
+      if (!warp_wait(b_qready, unit & 1, abort_flag)) {
+        ok = false;
+        site = 1;
+        break;
+      }
+      ++unit;
+      for (int t = t0; t < t1; ++t, ++it) {
+        const int stage = it % kStages, buf = it & 1;
+        if (!warp_wait(b_full + 8 * stage, (it / kStages) & 1, abort_flag) ||
+            !warp_wait(b_sempty + 8 * buf, ((it >> 1) & 1) ^ 1, abort_flag)) {
+          ok = false;
+          site = 2;
+          break;
+        }
+        tc_fence_after();
+        if (elect_one()) {
+          const uint64_t a = rows_desc<DIM>(smem_u32(smem + stage * 2 * Sh::kTile));
+#pragma unroll
+          for (int term = 0; term < kTerms; ++term) {
+            const uint64_t b = rows_desc<DIM>(q_addr + term * N * DIM);
+#pragma unroll
+            for (int k = 0; k < DIM / 32; ++k) mma_f8f6f4(tmem + buf * N, a + 2 * k, b + 2 * k, idesc, term + k > 0);
+          }
+          tc_commit(b_sfull + 8 * buf);
+        }
+        __syncwarp();
+        if (t > t0 && !issue_pv(it - 1, t - 1 == t0)) {
+          ok = false;
+          site = 3;
+          break;
+        }
+      }
+      // the unit's last product does not wait for the next unit's queries
+      if (ok && !issue_pv(it - 1, t1 - 1 == t0)) {
+        ok = false;
+        site = 4;
+      }
+      t0 = 0;
+      if (left > 0 && !next_unit(p, cur)) break;
+    }
+    if (!ok && lane == 0) *p.status = kRoleMma * 1000 + site;
+  } else {
+    // ------------------------------------------------------------------------------------------ softmax
+    const int quarter = warp & 3, token = quarter * 32 + lane, st = (warp - 2) * 32 + lane;
+    const uint32_t lane_off = static_cast<uint32_t>(quarter * 32) << 16;
+    int it = 0, xchg = 0;
+    int64_t tile_at = begin;
+    float ref[N], l[N];
+    // one arrival per warp, then all wait: bounded, unlike a named barrier
+    auto meet = [&]() {
+      __syncwarp();
+      const uint32_t bar = b_xchg + 8 * (xchg & 1);
+      if (lane == 0) mbar_arrive(bar);
+      const bool r = warp_wait(bar, (xchg >> 1) & 1, abort_flag);
+      ++xchg;
+      return r;
+    };
+    while (left > 0 && ok) {
+      const int t1 = static_cast<int>(min(static_cast<int64_t>(cur.v.tiles), t0 + left));
+      left -= t1 - t0;
+      const SeqView v = cur.v;
+      const int rows = v.n * p.group;
+      // ---- queries: eight elements per thread, split into e4m3 terms under a power-of-two scale of their row
+      {
+        constexpr int kLanes = DIM / 8;
+        const int e = (st % kLanes) * 8;
+        for (int r0 = 0; r0 < rows; r0 += 128 / kLanes) {
+          const int r = r0 + st / kLanes;
+          uint4 w = make_uint4(0, 0, 0, 0);
+          if (r < rows) {
+            const int i = r / p.group;
+            w = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.q) + (v.lo + i) * p.q_tok +
+                                                (cur.h * p.group + r - i * p.group) * p.q_head + e);
+          }
+          const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
+          float f[8];
+          uint32_t top = 0;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float2 u = unpack_pair<T>(ww[j]);
+            f[2 * j] = u.x;
+            f[2 * j + 1] = u.y;
+            top = max(top, max(__float_as_uint(u.x) & 0x7fffffffu, __float_as_uint(u.y) & 0x7fffffffu));
+          }
+#pragma unroll
+          for (int o = kLanes / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+          const float s = cache_scale(__uint_as_float(top)), inv = pow2_reciprocal(s);
+          uint32_t out[kTerms][2];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            uint32_t term[kTerms];
+            float a = f[2 * j] * inv, c = f[2 * j + 1] * inv;
+            split_e4m3<kTerms>(a, c, term);
+#pragma unroll
+            for (int x = 0; x < kTerms; ++x) out[x][j >> 1] = (j & 1) ? out[x][j >> 1] | (term[x] << 16) : term[x];
+          }
+          if (r < rows) {
+#pragma unroll
+            for (int x = 0; x < kTerms; ++x)
+              *reinterpret_cast<uint2*>(q_smem + x * N * DIM + swizzled<DIM>(r, e)) = make_uint2(out[x][0], out[x][1]);
+            // a row that holds an infinity or NaN has no answer
+            if (e == 0) rowmul[r] = top >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : s * p.scale * 1.4426950408889634f;
+          }
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(b_qready);
+        if (!meet()) {
+          ok = false;
+          site = 1;
+          break;
+        }
+      }
+#pragma unroll
+      for (int r = 0; r < N; ++r) {
+        ref[r] = -INFINITY;
+        l[r] = 0.f;
+      }
+      uint64_t nan_rows = 0;  // rows that see a NaN in element `token` of a value
+      for (int t = t0; t < t1; ++t, ++it) {
+        const int stage = it % kStages, buf = it & 1;
+        if (!warp_wait(b_full + 8 * stage, (it / kStages) & 1, abort_flag)) {
+          ok = false;
+          site = 2;
+          break;
+        }
+        const TileInfo ti = info[stage];
+        const bool page_ok = ti.base >= 0;
+        int see_lo, see_hi;
+        rows_that_see(p, v, ti.base + token, page_ok, see_lo, see_hi);
+        see_lo *= p.group;
+        see_hi *= p.group;
+        // every row sees every token of the page: the ends' columns need no look
+        int f_lo, f_hi, g_lo, g_hi;
+        rows_that_see(p, v, ti.base, page_ok, f_lo, f_hi);
+        rows_that_see(p, v, ti.base + kPage - 1, page_ok, g_lo, g_hi);
+        const bool whole = f_lo == 0 && g_lo == 0 && f_hi == v.n && g_hi == v.n && page_ok;
+        if (!whole && token < DIM) {
+          // values that nobody sees are whatever memory held, NaN among it, and 0 * NaN is NaN: they become zeros; a NaN
+          // that only some rows see is kept from the product and given to those rows at the end
+          uint8_t* row = smem + stage * 2 * Sh::kTile + Sh::kTile + token * kPage;
+          // tokens of the page that some row sees: t < any_hi and (t >= any_lo or t < any_sink)
+          const int any_hi = page_ok ? min(max(min(v.len, v.pos0 + v.n) - ti.base, 0), kPage) : 0;
+          const int any_lo = p.window > 0 ? static_cast<int>(min(max(static_cast<int64_t>(v.pos0) - p.window + 1 - ti.base, int64_t(0)), int64_t(kPage))) : 0;
+          const int any_sink = min(max(p.sinks - ti.base, 0), kPage);
+          for (int c = 0; c < kPage / 16; ++c) {
+            uint4* at = reinterpret_cast<uint4*>(row + ((c ^ (token & 7)) << 4));
+            const int t16 = c * 16;
+            if (t16 >= any_hi || (t16 >= any_sink && t16 + 16 <= any_lo)) {
+              *at = make_uint4(0, 0, 0, 0);
+              continue;
+            }
+            const bool all = t16 + 16 <= any_hi && (t16 >= any_lo || t16 + 16 <= any_sink);
+            uint4 w = *at;
+            uint32_t ww[4] = {w.x, w.y, w.z, w.w};
+            if (!all) {
+#pragma unroll
+              for (int x = 0; x < 16; ++x) {
+                const int tt = t16 + x;
+                if (!(tt < any_hi && (tt >= any_lo || tt < any_sink))) ww[x >> 2] &= ~(255u << (8 * (x & 3)));
+              }
+            }
+            uint32_t nan = 0;
+#pragma unroll
+            for (int x = 0; x < 4; ++x) nan |= ((ww[x] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
+            if (nan) {
+#pragma unroll
+              for (int x = 0; x < 16; ++x) {
+                if (((ww[x >> 2] >> (8 * (x & 3))) & 127u) == 127u) {
+                  int lo, hi;
+                  rows_that_see(p, v, ti.base + t16 + x, page_ok, lo, hi);
+                  const int a = lo * p.group, z = hi * p.group;
+                  if (a < z) nan_rows |= (z >= 64 ? ~uint64_t(0) : (uint64_t(1) << z) - 1) & ~((uint64_t(1) << a) - 1);
+                  ww[x >> 2] &= ~(255u << (8 * (x & 3)));
+                }
+              }
+            }
+            if (nan || !all) *at = make_uint4(ww[0], ww[1], ww[2], ww[3]);
+          }
+        }
+        if (!warp_wait(b_sfull + 8 * buf, (it >> 1) & 1, abort_flag)) {
+          ok = false;
+          site = 3;
+          break;
+        }
+        tc_fence_after();
+        const uint32_t t_s = tmem + buf * N + lane_off;
+        const int span = see_hi - see_lo;
+        float4* wm = wmax + (xchg & 1) * N;
+#pragma unroll
+        for (int c = 0; c < N; c += 16) {
+          if (c >= rows) break;
+          uint32_t s[16];
+          tmem_ld_32x16(t_s + c, s);
+          tmem_ld_wait();
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            if (c + (j & ~3) >= rows) break;
+            const float x = static_cast<unsigned>(c + j - see_lo) < static_cast<unsigned>(max(span, 0))
+                                ? fmaf(__uint_as_float(s[j]), rowmul[c + j] * ti.ks, ti.lv) : -INFINITY;
+            const float m = redux_max(x);
+            if (lane == 0) reinterpret_cast<float*>(wm + c + j)[quarter] = m;
+          }
+        }
+        if (!meet()) {
+          ok = false;
+          site = 4;
+          break;
+        }
+        // ---- move the reference where a row's exponent has outgrown it
+        bool moved = false;
+#pragma unroll
+        for (int r = 0; r < N; ++r) {
+          if ((r & ~3) >= rows) break;
+          const float4 w = wm[r];
+          const float m = fmaxf(fmaxf(w.x, w.y), fmaxf(w.z, w.w));
+          moved = moved || m > ref[r] + 1.f;
+        }
+        if (moved) {
+          if (t > t0 && !warp_wait(b_pvdone + 8 * ((it - 1) & 1), ((it - 1) >> 1) & 1, abort_flag)) {
+            ok = false;
+            site = 5;
+            break;
+          }
+          tc_fence_after();
+#pragma unroll
+          for (int c = 0; c < N; c += 16) {
+            if (c >= rows) break;
+            float f[16];
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+              f[j] = 1.f;
+              if (c + (j & ~3) < rows) {
+                const float4 w = wm[c + j];
+                const float m = fmaxf(fmaxf(w.x, w.y), fmaxf(w.z, w.w));
+                if (m > ref[c + j] + 1.f) {
+                  f[j] = exp2_approx(ref[c + j] - m);
+                  ref[c + j] = m;
+                  l[c + j] *= f[j];
+                }
+              }
+            }
+            if (t > t0) {
+              uint32_t o[16];
+              tmem_ld_32x16(t_o + lane_off + c, o);
+              tmem_ld_wait();
+#pragma unroll
+              for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * f[j]);
+              tmem_st_32x16(t_o + lane_off + c, o);
+              tmem_st_wait();
+            }
+          }
+        }
+        // ---- P; its buffer is free once the product before the last has read it
+        if (!warp_wait(b_pvdone + 8 * buf, ((it >> 1) & 1) ^ 1, abort_flag)) {
+          ok = false;
+          site = 6;
+          break;
+        }
+        uint8_t* pb = p_smem + buf * Sh::kP;
+#pragma unroll
+        for (int c = 0; c < N; c += 16) {
+          if (c >= rows) break;
+          uint32_t s[16];
+          tmem_ld_32x16(t_s + c, s);
+          tmem_ld_wait();
+#pragma unroll
+          for (int j = 0; j < 16; j += 2) {
+            if (c + (j & ~3) >= rows) break;
+            float e[2];
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+              const int r = c + j + x;
+              const bool seen = static_cast<unsigned>(r - see_lo) < static_cast<unsigned>(max(span, 0));
+              const float z = fmaf(__uint_as_float(s[j + x]), rowmul[r] * ti.ks, ti.lv) - ref[r] + kHeadroom;
+              e[x] = seen ? exp2_approx(z) : 0.f;
+            }
+            // the sums take p as it is: a page whose values are tiny beside the others' still counts in full
+            l[c + j] = fmaf(e[0], ti.inv_vs, l[c + j]);
+            l[c + j + 1] = fmaf(e[1], ti.inv_vs, l[c + j + 1]);
+            uint32_t term[kTerms];
+            split_e4m3<kTerms>(e[0], e[1], term);
+#pragma unroll
+            for (int x = 0; x < kTerms; ++x) {
+              if (c + j < rows) pb[x * N * kPage + swizzled<128>(c + j, token)] = static_cast<uint8_t>(term[x]);
+              if (c + j + 1 < rows) pb[x * N * kPage + swizzled<128>(c + j + 1, token)] = static_cast<uint8_t>(term[x] >> 8);
+            }
+          }
+        }
+        fence_proxy_async_smem();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(b_sempty + 8 * buf);
+          mbar_arrive(b_pready + 8 * buf);
+        }
+      }
+      if (!ok) break;
+      // ---- the unit's (or this block's part of its) result: thread = element of the head
+#pragma unroll
+      for (int r = 0; r < N; ++r) {
+        if ((r & ~3) >= rows) break;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) l[r] += __shfl_xor_sync(0xffffffffu, l[r], o);
+      }
+      float4* sums = wmax + (xchg & 1) * N;
+#pragma unroll
+      for (int r = 0; r < N; ++r) {
+        if ((r & ~3) >= rows) break;
+        if (lane == 0) reinterpret_cast<float*>(sums + r)[quarter] = l[r];
+      }
+      if (!meet() || !warp_wait(b_pvdone + 8 * ((it - 1) & 1), ((it - 1) >> 1) & 1, abort_flag)) {
+        ok = false;
+        site = 7;
+        break;
+      }
+      tc_fence_after();
+      const bool whole_unit = t0 == 0 && t1 == v.tiles;
+      const int64_t slot = 2 * static_cast<int64_t>(blockIdx.x) + (t0 > 0 ? 0 : 1);
+#pragma unroll
+      for (int c = 0; c < N; c += 16) {
+        if (c >= rows) break;
+        uint32_t o[16];
+        tmem_ld_32x16(t_o + lane_off + c, o);
+        tmem_ld_wait();
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          const int r = c + j;
+          if (r >= rows) break;
+          const float4 w = sums[r];
+          const float sum = (w.x + w.y) + (w.z + w.w);
+          float x = __uint_as_float(o[j]);
+          if ((nan_rows >> r) & 1u) x = __uint_as_float(0x7fc00000u);
+          if (whole_unit) {
+            const int i = r / p.group;
+            if (token < DIM)
+              static_cast<T*>(p.o)[(v.lo + i) * p.o_tok + (cur.h * p.group + r - i * p.group) * p.o_head + token] =
+                  static_cast<T>(sum == 0.f ? 0.f : x / sum);
+          } else {
+            if (token < DIM) p.part_o[(slot * N + r) * DIM + token] = x;
+            if (token == 0) p.part_ml[slot * N + r] = make_float2(ref[r], sum);
+          }
+        }
+      }
+      tc_fence_before();
+      if (left == 0 && st == 0) {
+        // does the unit go on behind this block, and did it begin here?
+        int4 rec = make_int4(-1, 0, 0, 0);
+        if (t0 == 0 && t1 < v.tiles) {
+          const int64_t unit_end = tile_at + v.tiles;
+          rec = make_int4(v.lo, cur.h, v.n, static_cast<int>((unit_end * blocks - 1) / total));
+        }
+        p.record[blockIdx.x] = rec;
+      }
+      tile_at += t1 - t0;
+      t0 = 0;
+      if (left > 0 && !next_unit(p, cur)) break;
+    }
+    if (!ok && lane == 0) *p.status = kRoleEpilogue * 1000 + site;
+    if (!ok && st == 0) p.record[blockIdx.x] = make_int4(-1, 0, 0, 0);
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, Sh::kTmem);
+  }
+}
+
+// Adds the parts of a unit that was cut by a block's range, in block order.  Block (i, y): rows 4 y .. 4 y + 3 of the unit that
+// block i of the kernel above left unfinished.
+template <typename T, int DIM>
+__global__ void __launch_bounds__(4 * DIM) tg_attention_join_kernel(const AttentionParams p, int rows_padded) {
+  griddep_wait();
+  griddep_launch_dependents();
+  const int4 rec = p.record[blockIdx.x];
+  const int r = blockIdx.y * 4 + threadIdx.x / DIM, d = threadIdx.x % DIM;
+  if (rec.x < 0 || r >= rec.z * p.group) return;
+  const int first = blockIdx.x, last = min(rec.w, static_cast<int>(gridDim.x) - 1);
+  const int64_t head = (2 * static_cast<int64_t>(first) + 1) * rows_padded + r;  // the first part: slot 1 of its block
+  float m = p.part_ml[head].x;
+#pragma unroll 8
+  for (int i = first + 1; i <= last; ++i) m = fmaxf(m, p.part_ml[2 * static_cast<int64_t>(i) * rows_padded + r].x);
+  const float base = m == -INFINITY ? 0.f : m;
+  float l = 0.f, o = 0.f;
+#pragma unroll 8
+  for (int i = first; i <= last; ++i) {
+    const int64_t at = i == first ? head : 2 * static_cast<int64_t>(i) * rows_padded + r;
+    const float2 ml = p.part_ml[at];
+    const float f = exp2f(ml.x - base);
+    l = fmaf(ml.y, f, l);
+    o = fmaf(p.part_o[at * DIM + d], f, o);
+  }
+  const int i = r / p.group;
+  static_cast<T*>(p.o)[(rec.x + i) * p.o_tok + (rec.y * p.group + r - i * p.group) * p.o_head + d] = static_cast<T>(l == 0.f ? 0.f : o / l);
+}
+
+template <typename T, int DIM, int N>
+cudaError_t launch_n(const CUtensorMap& tmK, const CUtensorMap& tmV, const AttentionParams& p, int blocks, cudaStream_t stream) {
+  constexpr int kTerms = kTermsOf<T>;
+  using Sh = Shape<DIM, N, kTerms>;
+  auto kernel = tg_attention_few_rows_kernel<T, DIM, N>;
+  static bool set[64] = {};  // per device; set again at worst
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (!set[dev & 63]) {
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Sh::kSmem);
+    if (e != cudaSuccess) return e;
+    set[dev & 63] = true;
+  }
+  e = launch_pdl(kernel, dim3(blocks), dim3(kThreads), Sh::kSmem, stream, tmK, tmV, p);
+  if (e != cudaSuccess) return e;
+  return launch_pdl(tg_attention_join_kernel<T, DIM>, dim3(blocks, (p.max_q_len * p.group + 3) / 4), dim3(4 * DIM), 0, stream, p, N);
+}
+
+template <typename T, int DIM>
+cudaError_t launch_rows(const CUtensorMap& tmK, const CUtensorMap& tmV, const AttentionParams& p, int n, int blocks, cudaStream_t stream) {
+  if (n == 16) return launch_n<T, DIM, 16>(tmK, tmV, p, blocks, stream);
+  if (n == 32) return launch_n<T, DIM, 32>(tmK, tmV, p, blocks, stream);
+  return launch_n<T, DIM, 64>(tmK, tmV, p, blocks, stream);
+}
+
+}  // namespace
+
+int few_rows_padded(int rows) { return rows <= 16 ? 16 : rows <= 32 ? 32 : 64; }
+
+int few_rows_blocks(int dim, int rows_padded, bool bf16, int num_sms) {
+  static_assert(Shape<128, 16, 2>::kBlocksPerSm == 2 && Shape<64, 16, 3>::kBlocksPerSm == 2 && Shape<128, 16, 3>::kBlocksPerSm == 1 &&
+                Shape<64, 32, 2>::kBlocksPerSm == 1, "the rule below");
+  return num_sms * (rows_padded == 16 && (bf16 || dim == 64) ? 2 : 1);
+}
+
+uint64_t few_rows_workspace(int dim, int rows_padded, int blocks) {
+  const uint64_t parts = 2ull * blocks * rows_padded;
+  return parts * dim * 4 + parts * 8 + 16ull * blocks;
+}
+
+cudaError_t launch_attention_few_rows(const CUtensorMap& tmK, const CUtensorMap& tmV, const AttentionParams& p, int rows_padded,
+                                      int blocks, bool bf16, cudaStream_t stream) {
+  if (bf16)
+    return p.c.dim == 128 ? launch_rows<__nv_bfloat16, 128>(tmK, tmV, p, rows_padded, blocks, stream)
+                          : launch_rows<__nv_bfloat16, 64>(tmK, tmV, p, rows_padded, blocks, stream);
+  return p.c.dim == 128 ? launch_rows<__half, 128>(tmK, tmV, p, rows_padded, blocks, stream)
+                        : launch_rows<__half, 64>(tmK, tmV, p, rows_padded, blocks, stream);
+}
+
+}  // namespace tg

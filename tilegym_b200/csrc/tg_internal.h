@@ -112,6 +112,8 @@ int32_t api_fail(int32_t rc, const char* msg);
 int32_t api_check_operand(const TgTensorDesc* t, const char* name);
 int32_t api_check_output(const TgTensorDesc* C, int64_t M, int64_t N);
 int32_t api_make_map(CUtensorMap* map, uint64_t ptr, int64_t rows, int64_t K, int64_t pitch, int box_rows);
+// dense rows of 64 or 128 bytes (64- or 128-byte swizzle), boxes of whole rows; for the pages of an 8-bit cache
+int32_t api_make_page_map(CUtensorMap* map, uint64_t ptr, int64_t rows, int cols, int box_rows);
 int32_t api_init_device(int dev, int* num_sms, int32_t** status);  // call with `dev` current
 uint32_t api_wait_limit_us();  // tg_set_wait_limit_us() value (0 = default), for GemmParams::wait_limit_us
 
