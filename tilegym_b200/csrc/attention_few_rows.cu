@@ -7,10 +7,11 @@
 //   p = 2^(S * scale * log2 e + log2 v_scale - ref)     thread = token; v_scale of the page rides in the exponent
 //   O^T [dim, R]        += V^T [dim, 128] . P           p = p1 + p2 (+ p3) in e4m3, the same way
 //
-// The two factors that are not in the cache are split into sums of e4m3 values (split_e4m3): two terms hold a bf16 q exactly
-// and p to 2^-8, three (f16) both to 2^-12.  `ref` is a running maximum of the
-// exponent that is only moved when it would grow by more than one (a power of two of headroom is left for that under
-// e4m3's 448), which rescales O^T in TMEM.  Keeping v_scale in the exponent keeps p at one magnitude whatever the pages'
+// The two factors that are not in the cache are split into e4m3 terms, each holding what the one before left: two hold a
+// bf16 q exactly and p to 2^-8, three (f16) both to 2^-12.  The terms of q are summed by the accumulator; those of p are
+// kept 16 times larger each (which moves the end of e4m3's range out of reach) and have columns of their own in O^T, joined
+// at the end.  `ref` is a running maximum of the exponent that is only moved when a p would leave the format (2^5 of
+// headroom), which rescales O^T in TMEM.  Keeping v_scale in the exponent keeps p at one magnitude whatever the pages'
 // scales are.
 //
 // Work: the pages that the units (sequence, cache head) see are numbered through, and every block takes an equal range of
@@ -25,7 +26,8 @@ namespace tg {
 namespace {
 
 constexpr int kThreads = 192;
-constexpr float kHeadroom = 7.f;  // p is kept times 2^7; it may reach 2^8 before ref moves
+constexpr float kNominal = 3.f, kLimit = 8.f;  // p is kept times 2^3 and may reach 2^8 (e4m3 ends at 448) before ref moves
+constexpr float kUnset = -1e30f;  // the reference of a row that has not seen a token yet
 
 template <typename T>
 constexpr int kTermsOf = std::is_same<T, __half>::value ? 3 : 2;
@@ -42,7 +44,8 @@ struct Shape {
   static constexpr int kBudget = (kBlocksPerSm == 2 ? 113 : 226) * 1024 - 1024 - 2 * kP - kQ - kMisc;
   static constexpr int kStages = kBudget / (2 * kTile) > 8 ? 8 : kBudget / (2 * kTile);
   static constexpr int kSmem = 1024 + kStages * 2 * kTile + 2 * kP + kQ + kMisc;
-  static constexpr int kTmem = N == 16 ? 64 : N == 32 ? 128 : 256;  // S^T twice and O^T, a power of two
+  static constexpr int kTmemUsed = 2 * N + TERMS * N;  // S^T twice and the terms' O^T
+  static constexpr int kTmem = kTmemUsed <= 64 ? 64 : kTmemUsed <= 128 ? 128 : kTmemUsed <= 256 ? 256 : 512;
   static_assert(kStages >= 3, "the ring is too short to hide the latency of a page");
   static_assert(2 * kP + kQ >= 8192, "the value operand of dim 64 reads 8 KB behind its page");
 };
@@ -56,6 +59,22 @@ struct TileInfo {
 template <bool kHint = false>
 __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile uint32_t* abort_flag) {
   return __all_sync(0xffffffffu, mbar_wait<kHint>(bar, parity, abort_flag));
+}
+
+// The four softmax warps meet; true if any thread says so.  Nobody waits alone here: whatever a warp found, it comes.
+__device__ __forceinline__ bool softmax_vote(bool mine) {
+  uint32_t any;
+  asm volatile(
+      "{\n\t"
+      ".reg .pred p, q;\n\t"
+      "setp.ne.u32 p, %1, 0;\n\t"
+      "barrier.cta.red.or.pred q, 1, 128, p;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t"
+      "}"
+      : "=r"(any)
+      : "r"(static_cast<uint32_t>(mine))
+      : "memory");
+  return any != 0;
 }
 
 // The units are numbered sequence by sequence, the cache heads of a sequence next to one another.
@@ -73,9 +92,57 @@ __device__ __forceinline__ bool next_unit(const AttentionParams& p, Cursor& c) {
   return true;
 }
 
+// One element's row of a value page (128 tokens) of which not every row sees every token.  Values that nobody sees are
+// whatever memory held, NaN among it, and 0 * NaN is NaN: they become zeros.  A NaN that some rows see is kept from the
+// product, which would give it to all, and noted for those rows.
+__device__ __noinline__ void clean_values(const AttentionParams& p, const SeqView& v, int base, uint8_t* row, int d, uint64_t& nan_rows) {
+  // tokens of the page that some row sees: t < hi and (t >= lo or t < sink)
+  const int hi = base >= 0 ? min(max(min(v.len, v.pos0 + v.n) - base, 0), kPage) : 0;
+  const int lo = p.window > 0 ? static_cast<int>(min(max(static_cast<int64_t>(v.pos0) - p.window + 1 - base, int64_t(0)), int64_t(kPage))) : 0;
+  const int sink = min(max(p.sinks - max(base, 0), 0), kPage);
+#pragma unroll 2
+  for (int c = 0; c < kPage / 16; ++c) {
+    uint4* at = reinterpret_cast<uint4*>(row + ((c ^ (d & 7)) << 4));
+    const int t = c * 16;
+    if (t >= hi || (t >= sink && t + 16 <= lo)) {
+      *at = make_uint4(0, 0, 0, 0);
+      continue;
+    }
+    const bool all = t + 16 <= hi && (t >= lo || t + 16 <= sink);
+    const uint4 w = *at;
+    uint32_t ww[4] = {w.x, w.y, w.z, w.w};
+    if (!all) {
+#pragma unroll
+      for (int x = 0; x < 16; ++x)
+        if (!(t + x < hi && (t + x >= lo || t + x < sink))) ww[x >> 2] &= ~(255u << (8 * (x & 3)));
+    }
+    uint32_t nan = 0;
+#pragma unroll
+    for (int x = 0; x < 4; ++x) nan |= ((ww[x] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
+    if (nan) {
+#pragma unroll 1
+      for (int x = 0; x < 16; ++x) {
+        const uint32_t word = x < 8 ? (x < 4 ? ww[0] : ww[1]) : (x < 12 ? ww[2] : ww[3]);
+        if (((word >> (8 * (x & 3))) & 127u) != 127u) continue;
+        int a, z;
+        rows_that_see(p, v, base + t + x, true, a, z);
+        a *= p.group;
+        z *= p.group;
+        if (a < z) nan_rows |= (z >= 64 ? ~uint64_t(0) : (uint64_t(1) << z) - 1) & ~((uint64_t(1) << a) - 1);
+        const uint32_t keep = ~(255u << (8 * (x & 3)));
+        if (x < 4) ww[0] &= keep;
+        else if (x < 8) ww[1] &= keep;
+        else if (x < 12) ww[2] &= keep;
+        else ww[3] &= keep;
+      }
+    }
+    if (nan || !all) *at = make_uint4(ww[0], ww[1], ww[2], ww[3]);
+  }
+}
+
 template <typename T, int DIM, int N>
 __global__ void __launch_bounds__(kThreads, (Shape<DIM, N, kTermsOf<T>>::kBlocksPerSm))
-    tg_attention_few_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const AttentionParams p) {
+    tg_attention_few_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const __grid_constant__ AttentionParams p) {
   constexpr int kTerms = kTermsOf<T>;
   using Sh = Shape<DIM, N, kTerms>;
   constexpr int kStages = Sh::kStages;
@@ -89,13 +156,14 @@ __global__ void __launch_bounds__(kThreads, (Shape<DIM, N, kTermsOf<T>>::kBlocks
   TileInfo* info = reinterpret_cast<TileInfo*>(misc + 512);
   volatile uint32_t* abort_flag = reinterpret_cast<volatile uint32_t*>(misc + 512 + 8 * sizeof(TileInfo));
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(misc + 512 + 8 * sizeof(TileInfo) + 16);
-  int64_t* sched = reinterpret_cast<int64_t*>(misc + 512 + 8 * sizeof(TileInfo) + 32);  // 0 total, 1 prefix, 2 sequence, 3.. warp sums
+  int64_t* sched = reinterpret_cast<int64_t*>(misc + 512 + 8 * sizeof(TileInfo) + 32);  // 0 tiles in front, 1 sequence, 2.. warp sums
   float* rowmul = reinterpret_cast<float*>(misc + 1024);
-  float4* wmax = reinterpret_cast<float4*>(misc + 2048);  // [2][N] of four warps' maxima; also the sums' exchange
+  float* ref = reinterpret_cast<float*>(misc + 1280);        // [2][N]
+  float* wmax = reinterpret_cast<float*>(misc + 2048);       // [2][4][N]: the four warps' maxima, or sums, by row
 
   const uint32_t bar0 = smem_u32(bars);
   const uint32_t b_full = bar0, b_empty = bar0 + 8 * kStages, b_sfull = b_empty + 8 * kStages, b_sempty = b_sfull + 16,
-                 b_pready = b_sempty + 16, b_pvdone = b_pready + 16, b_qready = b_pvdone + 16, b_xchg = b_qready + 8;
+                 b_pready = b_sempty + 16, b_pvdone = b_pready + 16, b_qready = b_pvdone + 16;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   if (warp == 0) {
@@ -113,7 +181,6 @@ __global__ void __launch_bounds__(kThreads, (Shape<DIM, N, kTermsOf<T>>::kBlocks
         mbar_init(b_sempty + 8 * i, 4);
         mbar_init(b_pready + 8 * i, 4);
         mbar_init(b_pvdone + 8 * i, 1);
-        mbar_init(b_xchg + 8 * i, 4);
       }
       mbar_init(b_qready, 4);
       init_abort_flag(abort_flag, p.wait_limit_us);
@@ -123,61 +190,57 @@ __global__ void __launch_bounds__(kThreads, (Shape<DIM, N, kTermsOf<T>>::kBlocks
     tmem_alloc(smem_u32(tmem_slot), Sh::kTmem);
     tmem_relinquish();
   }
-  // rows of P that no query has stay zero, and so do their columns of O^T
-  for (int i = threadIdx.x; i < (2 * Sh::kP + Sh::kQ) / 16; i += kThreads) reinterpret_cast<uint4*>(p_smem)[i] = make_uint4(0, 0, 0, 0);
-  fence_proxy_async_smem();
   griddep_wait();
   griddep_launch_dependents();
 
   // ---- this block's range of pages
+  int64_t total, begin = 0, end = 0, blocks;
   {
-    int64_t sum = 0;
-    for (int b = threadIdx.x; b < p.c.seqs; b += kThreads) sum += view_sequence(p, b, 0, p.max_q_len).tiles;
+    const int mine = static_cast<int>(threadIdx.x) < p.c.seqs ? view_sequence(p, threadIdx.x, 0, p.max_q_len).tiles : 0;
+    int64_t sum = mine;
+    for (int b = threadIdx.x + kThreads; b < p.c.seqs; b += kThreads) sum += view_sequence(p, b, 0, p.max_q_len).tiles;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    if (lane == 0) sched[3 + warp] = sum;
+    if (lane == 0) sched[2 + warp] = sum;
+    if (threadIdx.x == 0) sched[1] = -1;
     __syncthreads();
-    if (threadIdx.x == 0) {
-      int64_t t = 0;
-      for (int w = 0; w < kThreads / 32; ++w) t += sched[3 + w];
-      sched[0] = t * p.c.heads;
-      sched[1] = 0;
-      sched[2] = -1;
+    total = 0;
+#pragma unroll
+    for (int w = 0; w < kThreads / 32; ++w) total += sched[2 + w];
+    total *= p.c.heads;
+    blocks = min(static_cast<int64_t>(gridDim.x), total);  // the others have nothing to do
+    if (blockIdx.x < blocks) {
+      begin = total * blockIdx.x / blocks;
+      end = total * (blockIdx.x + 1) / blocks;
     }
-    __syncthreads();
-  }
-  const int64_t total = sched[0];
-  const int64_t blocks = min(static_cast<int64_t>(gridDim.x), total);  // the others have nothing to do
-  const bool mine_any = blockIdx.x < blocks;
-  const int64_t begin = mine_any ? total * blockIdx.x / blocks : 0, end = mine_any ? total * (blockIdx.x + 1) / blocks : 0;
-  if (begin < end) {
+    // the sequence in which it begins: prefix sums, as far as needed
     const int64_t target = begin / p.c.heads;
     int64_t before = 0;
-    for (int base = 0; base < p.c.seqs; base += kThreads) {
+    for (int base = 0; base < p.c.seqs && begin < end; base += kThreads) {
       const int b = base + threadIdx.x;
-      const int mine = b < p.c.seqs ? view_sequence(p, b, 0, p.max_q_len).tiles : 0;
-      int64_t incl = mine;
+      const int n = base == 0 ? mine : b < p.c.seqs ? view_sequence(p, b, 0, p.max_q_len).tiles : 0;
+      int64_t incl = n;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
         const int64_t up = __shfl_up_sync(0xffffffffu, incl, o);
         if (lane >= o) incl += up;
       }
       __syncthreads();
-      if (lane == 31) sched[3 + warp] = incl;
+      if (lane == 31) sched[2 + warp] = incl;
       __syncthreads();
       int64_t off = before, all = before;
+#pragma unroll
       for (int w = 0; w < kThreads / 32; ++w) {
-        if (w < warp) off += sched[3 + w];
-        all += sched[3 + w];
+        if (w < warp) off += sched[2 + w];
+        all += sched[2 + w];
       }
-      if (mine > 0 && off + incl - mine <= target && target < off + incl) {
-        sched[1] = off + incl - mine;
-        sched[2] = b;
+      if (n > 0 && off + incl - n <= target && target < off + incl) {
+        sched[0] = off + incl - n;
+        sched[1] = b;
       }
       before = all;
       if (before > target) break;  // the same for every thread
     }
-    __syncthreads();
   }
   tc_fence_before();
   __syncthreads();
@@ -186,12 +249,12 @@ __global__ void __launch_bounds__(kThreads, (Shape<DIM, N, kTermsOf<T>>::kBlocks
   const uint32_t t_o = tmem + 2 * N;
 
   Cursor cur;
-  cur.b = static_cast<int>(sched[2]);
+  cur.b = static_cast<int>(sched[1]);
   int t0 = 0;
   const bool work = begin < end && cur.b >= 0;
   if (work) {
     cur.v = view_sequence(p, cur.b, 0, p.max_q_len);
-    const int64_t rem = begin - sched[1] * p.c.heads;
+    const int64_t rem = begin - sched[0] * p.c.heads;
     cur.h = static_cast<int>(rem / cur.v.tiles);
     t0 = static_cast<int>(rem - static_cast<int64_t>(cur.h) * cur.v.tiles);
   } else if (threadIdx.x == 0) {
@@ -258,7 +321,7 @@ __global__ void __launch_bounds__(kThreads, (Shape<DIM, N, kTermsOf<T>>::kBlocks
     }
   } else if (warp == 1) {
     // ------------------------------------------------------------------------------------------ products
-    constexpr uint32_t idesc = make_idesc_e4m3_f32(128, N);
+    constexpr uint32_t idesc = make_idesc_e4m3_f32(128, N), idesc_pv = make_idesc_e4m3_f32(128, kTerms * N);
     const uint32_t q_addr = smem_u32(q_smem), p_addr = smem_u32(p_smem);
     int it = 0, unit = 0;
     auto issue_pv = [&](int i, bool first) {
@@ -267,12 +330,9 @@ __global__ void __launch_bounds__(kThreads, (Shape<DIM, N, kTermsOf<T>>::kBlocks
       tc_fence_after();
       if (elect_one()) {
         const uint64_t a = make_kmajor_sw128_desc(smem_u32(smem + stage * 2 * Sh::kTile + Sh::kTile));
+        const uint64_t b = make_kmajor_sw128_desc(p_addr + buf * Sh::kP);
 #pragma unroll
-        for (int term = 0; term < kTerms; ++term) {
-          const uint64_t b = make_kmajor_sw128_desc(p_addr + buf * Sh::kP + term * N * kPage);
-#pragma unroll
-          for (int k = 0; k < kPage / 32; ++k) mma_f8f6f4(t_o, a + 2 * k, b + 2 * k, idesc, !(first && term == 0 && k == 0));
-        }
+        for (int k = 0; k < kPage / 32; ++k) mma_f8f6f4(t_o, a + 2 * k, b + 2 * k, idesc_pv, !(first && k == 0));
         tc_commit(b_empty + 8 * stage);
         tc_commit(b_pvdone + 8 * buf);
       }
@@ -325,251 +385,220 @@ __global__ void __launch_bounds__(kThreads, (Shape<DIM, N, kTermsOf<T>>::kBlocks
     if (!ok && lane == 0) *p.status = kRoleMma * 1000 + site;
   } else {
     // ------------------------------------------------------------------------------------------ softmax
+    // A wait that gives up is remembered, not acted on: the four warps leave together at their next vote.
     const int quarter = warp & 3, token = quarter * 32 + lane, st = (warp - 2) * 32 + lane;
     const uint32_t lane_off = static_cast<uint32_t>(quarter * 32) << 16;
-    int it = 0, xchg = 0;
+    int it = 0, turn = 0;
     int64_t tile_at = begin;
-    float ref[N], l[N];
-    // one arrival per warp, then all wait: bounded, unlike a named barrier
-    auto meet = [&]() {
-      __syncwarp();
-      const uint32_t bar = b_xchg + 8 * (xchg & 1);
-      if (lane == 0) mbar_arrive(bar);
-      const bool r = warp_wait(bar, (xchg >> 1) & 1, abort_flag);
-      ++xchg;
-      return r;
+    float l[N];
+    int side = 0;  // which of the two copies of the references holds
+    auto wait = [&](uint32_t bar, uint32_t parity, int where) {
+      if (!warp_wait(bar, parity, abort_flag) && ok) {
+        ok = false;
+        site = where;
+      }
     };
-    while (left > 0 && ok) {
+    while (left > 0) {
       const int t1 = static_cast<int>(min(static_cast<int64_t>(cur.v.tiles), t0 + left));
       left -= t1 - t0;
       const SeqView v = cur.v;
       const int rows = v.n * p.group;
       // ---- queries: eight elements per thread, split into e4m3 terms under a power-of-two scale of their row
       {
-        constexpr int kLanes = DIM / 8;
+        constexpr int kLanes = DIM / 8, kRows = 128 / kLanes, kPasses = N / kRows, kBatch = kPasses < 4 ? kPasses : 4;
         const int e = (st % kLanes) * 8;
-        for (int r0 = 0; r0 < rows; r0 += 128 / kLanes) {
-          const int r = r0 + st / kLanes;
-          uint4 w = make_uint4(0, 0, 0, 0);
-          if (r < rows) {
-            const int i = r / p.group;
-            w = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.q) + (v.lo + i) * p.q_tok +
-                                                (cur.h * p.group + r - i * p.group) * p.q_head + e);
-          }
-          const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
-          float f[8];
-          uint32_t top = 0;
+#pragma unroll 1
+        for (int r0 = 0; r0 < rows; r0 += kRows * kBatch) {
+          uint4 w[kBatch];
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const float2 u = unpack_pair<T>(ww[j]);
-            f[2 * j] = u.x;
-            f[2 * j + 1] = u.y;
-            top = max(top, max(__float_as_uint(u.x) & 0x7fffffffu, __float_as_uint(u.y) & 0x7fffffffu));
+          for (int k = 0; k < kBatch; ++k) {
+            const int r = r0 + k * kRows + st / kLanes, i = r / p.group;
+            w[k] = make_uint4(0, 0, 0, 0);
+            if (r < rows)
+              w[k] = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.q) + (v.lo + i) * p.q_tok + (cur.h * p.group + r - i * p.group) * p.q_head + e);
           }
 #pragma unroll
-          for (int o = kLanes / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-          const float s = cache_scale(__uint_as_float(top)), inv = pow2_reciprocal(s);
-          uint32_t out[kTerms][2];
+          for (int k = 0; k < kBatch; ++k) {
+            const int r = r0 + k * kRows + st / kLanes;
+            const uint32_t ww[4] = {w[k].x, w[k].y, w[k].z, w[k].w};
+            float f[8];
+            uint32_t top = 0;
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            uint32_t term[kTerms];
-            float a = f[2 * j] * inv, c = f[2 * j + 1] * inv;
-            split_e4m3<kTerms>(a, c, term);
+            for (int j = 0; j < 4; ++j) {
+              const float2 u = unpack_pair<T>(ww[j]);
+              f[2 * j] = u.x;
+              f[2 * j + 1] = u.y;
+              top = max(top, max(__float_as_uint(u.x) & 0x7fffffffu, __float_as_uint(u.y) & 0x7fffffffu));
+            }
 #pragma unroll
-            for (int x = 0; x < kTerms; ++x) out[x][j >> 1] = (j & 1) ? out[x][j >> 1] | (term[x] << 16) : term[x];
-          }
-          if (r < rows) {
+            for (int o = kLanes / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+            const float sc = cache_scale(__uint_as_float(top)), inv = pow2_reciprocal(sc);
+            uint32_t out[kTerms][2];
 #pragma unroll
-            for (int x = 0; x < kTerms; ++x)
-              *reinterpret_cast<uint2*>(q_smem + x * N * DIM + swizzled<DIM>(r, e)) = make_uint2(out[x][0], out[x][1]);
-            // a row that holds an infinity or NaN has no answer
-            if (e == 0) rowmul[r] = top >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : s * p.scale * 1.4426950408889634f;
+            for (int j = 0; j < 4; ++j) {
+              uint32_t term[kTerms];
+              split_e4m3<kTerms>(f[2 * j] * inv, f[2 * j + 1] * inv, 1.f, term);
+#pragma unroll
+              for (int x = 0; x < kTerms; ++x) out[x][j >> 1] = (j & 1) ? out[x][j >> 1] | (term[x] << 16) : term[x];
+            }
+            if (r < N) {
+#pragma unroll
+              for (int x = 0; x < kTerms; ++x)
+                *reinterpret_cast<uint2*>(q_smem + x * N * DIM + swizzled<DIM>(r, e)) = make_uint2(out[x][0], out[x][1]);
+              // a row that holds an infinity or NaN has no answer
+              if (e == 0) rowmul[r] = top >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : sc * p.scale * 1.4426950408889634f;
+            }
           }
         }
+        // rows that fill up a group of eight: exponents of minus infinity.  The copy that nobody can still be reading.
+        side ^= 1;
+        if (st < N) ref[side * N + st] = st < rows ? kUnset : INFINITY;
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(b_qready);
-        if (!meet()) {
-          ok = false;
-          site = 1;
-          break;
-        }
+        if (softmax_vote(!ok)) break;
       }
 #pragma unroll
-      for (int r = 0; r < N; ++r) {
-        ref[r] = -INFINITY;
-        l[r] = 0.f;
-      }
+      for (int r = 0; r < N; ++r) l[r] = 0.f;
       uint64_t nan_rows = 0;  // rows that see a NaN in element `token` of a value
+      // positions that every row sees: [all_lo, all_hi), and the first tokens
+      const int all_hi = min(v.len, v.pos0 + 1);
+      const int all_lo = p.window > 0 ? static_cast<int>(max(static_cast<int64_t>(v.pos0) + v.n - p.window, int64_t(0))) : 0;
+      bool gave_up = false;
       for (int t = t0; t < t1; ++t, ++it) {
         const int stage = it % kStages, buf = it & 1;
-        if (!warp_wait(b_full + 8 * stage, (it / kStages) & 1, abort_flag)) {
-          ok = false;
-          site = 2;
-          break;
-        }
+        wait(b_full + 8 * stage, (it / kStages) & 1, 1);
         const TileInfo ti = info[stage];
-        const bool page_ok = ti.base >= 0;
-        int see_lo, see_hi;
-        rows_that_see(p, v, ti.base + token, page_ok, see_lo, see_hi);
-        see_lo *= p.group;
-        see_hi *= p.group;
-        // every row sees every token of the page: the ends' columns need no look
-        int f_lo, f_hi, g_lo, g_hi;
-        rows_that_see(p, v, ti.base, page_ok, f_lo, f_hi);
-        rows_that_see(p, v, ti.base + kPage - 1, page_ok, g_lo, g_hi);
-        const bool whole = f_lo == 0 && g_lo == 0 && f_hi == v.n && g_hi == v.n && page_ok;
-        if (!whole && token < DIM) {
-          // values that nobody sees are whatever memory held, NaN among it, and 0 * NaN is NaN: they become zeros; a NaN
-          // that only some rows see is kept from the product and given to those rows at the end
-          uint8_t* row = smem + stage * 2 * Sh::kTile + Sh::kTile + token * kPage;
-          // tokens of the page that some row sees: t < any_hi and (t >= any_lo or t < any_sink)
-          const int any_hi = page_ok ? min(max(min(v.len, v.pos0 + v.n) - ti.base, 0), kPage) : 0;
-          const int any_lo = p.window > 0 ? static_cast<int>(min(max(static_cast<int64_t>(v.pos0) - p.window + 1 - ti.base, int64_t(0)), int64_t(kPage))) : 0;
-          const int any_sink = min(max(p.sinks - ti.base, 0), kPage);
-          for (int c = 0; c < kPage / 16; ++c) {
-            uint4* at = reinterpret_cast<uint4*>(row + ((c ^ (token & 7)) << 4));
-            const int t16 = c * 16;
-            if (t16 >= any_hi || (t16 >= any_sink && t16 + 16 <= any_lo)) {
-              *at = make_uint4(0, 0, 0, 0);
-              continue;
-            }
-            const bool all = t16 + 16 <= any_hi && (t16 >= any_lo || t16 + 16 <= any_sink);
-            uint4 w = *at;
-            uint32_t ww[4] = {w.x, w.y, w.z, w.w};
-            if (!all) {
-#pragma unroll
-              for (int x = 0; x < 16; ++x) {
-                const int tt = t16 + x;
-                if (!(tt < any_hi && (tt >= any_lo || tt < any_sink))) ww[x >> 2] &= ~(255u << (8 * (x & 3)));
-              }
-            }
-            uint32_t nan = 0;
-#pragma unroll
-            for (int x = 0; x < 4; ++x) nan |= ((ww[x] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
-            if (nan) {
-#pragma unroll
-              for (int x = 0; x < 16; ++x) {
-                if (((ww[x >> 2] >> (8 * (x & 3))) & 127u) == 127u) {
-                  int lo, hi;
-                  rows_that_see(p, v, ti.base + t16 + x, page_ok, lo, hi);
-                  const int a = lo * p.group, z = hi * p.group;
-                  if (a < z) nan_rows |= (z >= 64 ? ~uint64_t(0) : (uint64_t(1) << z) - 1) & ~((uint64_t(1) << a) - 1);
-                  ww[x >> 2] &= ~(255u << (8 * (x & 3)));
-                }
-              }
-            }
-            if (nan || !all) *at = make_uint4(ww[0], ww[1], ww[2], ww[3]);
-          }
+        const bool whole = ti.base >= 0 && ti.base + kPage <= all_hi && (ti.base >= all_lo || ti.base + kPage <= p.sinks);
+        int see_lo = 0, see_hi = N;
+        if (!whole) {
+          rows_that_see(p, v, ti.base + token, ti.base >= 0, see_lo, see_hi);
+          see_lo *= p.group;
+          see_hi *= p.group;
+          if (token < DIM) clean_values(p, v, ti.base, smem + stage * 2 * Sh::kTile + Sh::kTile + token * kPage, token, nan_rows);
         }
-        if (!warp_wait(b_sfull + 8 * buf, (it >> 1) & 1, abort_flag)) {
-          ok = false;
-          site = 3;
-          break;
-        }
+        wait(b_sfull + 8 * buf, (it >> 1) & 1, 2);
         tc_fence_after();
         const uint32_t t_s = tmem + buf * N + lane_off;
-        const int span = see_hi - see_lo;
-        float4* wm = wmax + (xchg & 1) * N;
-#pragma unroll
-        for (int c = 0; c < N; c += 16) {
-          if (c >= rows) break;
-          uint32_t s[16];
-          tmem_ld_32x16(t_s + c, s);
-          tmem_ld_wait();
-#pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            if (c + (j & ~3) >= rows) break;
-            const float x = static_cast<unsigned>(c + j - see_lo) < static_cast<unsigned>(max(span, 0))
-                                ? fmaf(__uint_as_float(s[j]), rowmul[c + j] * ti.ks, ti.lv) : -INFINITY;
-            const float m = redux_max(x);
-            if (lane == 0) reinterpret_cast<float*>(wm + c + j)[quarter] = m;
-          }
-        }
-        if (!meet()) {
-          ok = false;
-          site = 4;
-          break;
-        }
-        // ---- move the reference where a row's exponent has outgrown it
-        bool moved = false;
-#pragma unroll
-        for (int r = 0; r < N; ++r) {
-          if ((r & ~3) >= rows) break;
-          const float4 w = wm[r];
-          const float m = fmaxf(fmaxf(w.x, w.y), fmaxf(w.z, w.w));
-          moved = moved || m > ref[r] + 1.f;
-        }
-        if (moved) {
-          if (t > t0 && !warp_wait(b_pvdone + 8 * ((it - 1) & 1), ((it - 1) >> 1) & 1, abort_flag)) {
-            ok = false;
-            site = 5;
-            break;
-          }
-          tc_fence_after();
+        // ---- exponents: z = S * (row's factor * page's scale) + log2 v_scale - ref + kNominal, eight rows at a time
+        float z[N];
+        const float shift = ti.lv + kNominal;
+        auto exponents = [&](bool with_ref) {
 #pragma unroll
           for (int c = 0; c < N; c += 16) {
             if (c >= rows) break;
-            float f[16];
+            uint32_t s[16];
+            tmem_ld_32x16(t_s + c, s);
+            tmem_ld_wait();
 #pragma unroll
-            for (int j = 0; j < 16; ++j) {
-              f[j] = 1.f;
-              if (c + (j & ~3) < rows) {
-                const float4 w = wm[c + j];
-                const float m = fmaxf(fmaxf(w.x, w.y), fmaxf(w.z, w.w));
-                if (m > ref[c + j] + 1.f) {
-                  f[j] = exp2_approx(ref[c + j] - m);
-                  ref[c + j] = m;
-                  l[c + j] *= f[j];
-                }
-              }
+            for (int g = 0; g < 16; g += 8) {
+              if (c + g >= rows) break;
+              float m[8], r[8];
+              *reinterpret_cast<float4*>(m) = *reinterpret_cast<const float4*>(rowmul + c + g);
+              *reinterpret_cast<float4*>(m + 4) = *reinterpret_cast<const float4*>(rowmul + c + g + 4);
+              *reinterpret_cast<float4*>(r) = *reinterpret_cast<const float4*>(ref + side * N + c + g);
+              *reinterpret_cast<float4*>(r + 4) = *reinterpret_cast<const float4*>(ref + side * N + c + g + 4);
+#pragma unroll
+              for (int j = 0; j < 8; ++j) z[c + g + j] = fmaf(__uint_as_float(s[g + j]), m[j] * ti.ks, with_ref ? shift - r[j] : shift);
+            }
+          }
+          if (!whole) {
+#pragma unroll
+            for (int r = 0; r < N; ++r)
+              if (r < see_lo || r >= see_hi) z[r] = -INFINITY;
+          }
+        };
+        bool move = t == t0;
+        if (!move) {
+          exponents(true);
+          float over = -INFINITY;
+#pragma unroll
+          for (int g = 0; g < N; g += 8) {
+            if (g >= rows) break;
+            over = fmaxf(over, fmaxf(fmaxf(fmaxf(z[g], z[g + 1]), fmaxf(z[g + 2], z[g + 3])), fmaxf(fmaxf(z[g + 4], z[g + 5]), fmaxf(z[g + 6], z[g + 7]))));
+          }
+          move = softmax_vote(over > kLimit || !ok);
+        }
+        if (move) {
+          // ---- some row's exponent has outgrown its reference (or has none yet): every row's maximum, and a new reference
+          // where it is needed; the sums and O^T go along
+          exponents(false);
+          float* wm = wmax + (turn & 1) * 4 * N;
+          ++turn;
+#pragma unroll
+          for (int g = 0; g < N; g += 8) {
+            if (g >= rows) break;
+            float m[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) m[j] = redux_max(z[g + j]);
+            if (lane == 0) {
+              *reinterpret_cast<float4*>(wm + quarter * N + g) = make_float4(m[0], m[1], m[2], m[3]);
+              *reinterpret_cast<float4*>(wm + quarter * N + g + 4) = make_float4(m[4], m[5], m[6], m[7]);
+            }
+          }
+          if (t > t0) wait(b_pvdone + 8 * ((it - 1) & 1), ((it - 1) >> 1) & 1, 3);
+          if (softmax_vote(!ok)) {
+            gave_up = true;
+            break;
+          }
+          tc_fence_after();
+          const float* old = ref + side * N;
+          float* now = ref + (side ^ 1) * N;
+#pragma unroll
+          for (int g = 0; g < N; g += 8) {
+            if (g >= rows) break;
+            float f[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              const float* w = wm + g + j;
+              const float m = fmaxf(fmaxf(w[0], w[N]), fmaxf(w[2 * N], w[3 * N])) - kNominal, was = old[g + j];
+              const float r = m > was + (kLimit - kNominal) || was == kUnset ? fmaxf(m, kUnset) : was;
+              if (st == 0) now[g + j] = r;
+              f[j] = exp2_approx(was - r);
+              l[g + j] *= f[j];
+              z[g + j] -= r;
             }
             if (t > t0) {
-              uint32_t o[16];
-              tmem_ld_32x16(t_o + lane_off + c, o);
-              tmem_ld_wait();
 #pragma unroll
-              for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * f[j]);
-              tmem_st_32x16(t_o + lane_off + c, o);
-              tmem_st_wait();
+              for (int x = 0; x < kTerms; ++x) {
+                uint32_t o[8];
+                tmem_ld_32x8(t_o + lane_off + x * N + g, o);
+                tmem_ld_wait();
+#pragma unroll
+                for (int j = 0; j < 8; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * f[j]);
+                tmem_st_32x8(t_o + lane_off + x * N + g, o);
+              }
             }
           }
+          if (t > t0) tmem_st_wait();
+          side ^= 1;  // read again behind the next vote, or this one's below
+          if (softmax_vote(!ok)) {
+            gave_up = true;
+            break;
+          }
         }
-        // ---- P; its buffer is free once the product before the last has read it
-        if (!warp_wait(b_pvdone + 8 * buf, ((it >> 1) & 1) ^ 1, abort_flag)) {
-          ok = false;
-          site = 6;
-          break;
-        }
-        uint8_t* pb = p_smem + buf * Sh::kP;
+        // ---- P.  Its buffer is free: S^T of this page was issued behind the product before the last, which read it, and the
+        // barrier that announced S^T counts every product issued before.
+        const uint32_t pb = smem_u32(p_smem) + buf * Sh::kP + token;
 #pragma unroll
-        for (int c = 0; c < N; c += 16) {
-          if (c >= rows) break;
-          uint32_t s[16];
-          tmem_ld_32x16(t_s + c, s);
-          tmem_ld_wait();
+        for (int g = 0; g < N; g += 8) {
+          if (g >= rows) break;
+          uint32_t term[4][kTerms];
 #pragma unroll
-          for (int j = 0; j < 16; j += 2) {
-            if (c + (j & ~3) >= rows) break;
-            float e[2];
-#pragma unroll
-            for (int x = 0; x < 2; ++x) {
-              const int r = c + j + x;
-              const bool seen = static_cast<unsigned>(r - see_lo) < static_cast<unsigned>(max(span, 0));
-              const float z = fmaf(__uint_as_float(s[j + x]), rowmul[r] * ti.ks, ti.lv) - ref[r] + kHeadroom;
-              e[x] = seen ? exp2_approx(z) : 0.f;
-            }
+          for (int j = 0; j < 8; j += 2) {
+            const float e0 = exp2_approx(z[g + j]), e1 = exp2_approx(z[g + j + 1]);
             // the sums take p as it is: a page whose values are tiny beside the others' still counts in full
-            l[c + j] = fmaf(e[0], ti.inv_vs, l[c + j]);
-            l[c + j + 1] = fmaf(e[1], ti.inv_vs, l[c + j + 1]);
-            uint32_t term[kTerms];
-            split_e4m3<kTerms>(e[0], e[1], term);
-#pragma unroll
-            for (int x = 0; x < kTerms; ++x) {
-              if (c + j < rows) pb[x * N * kPage + swizzled<128>(c + j, token)] = static_cast<uint8_t>(term[x]);
-              if (c + j + 1 < rows) pb[x * N * kPage + swizzled<128>(c + j + 1, token)] = static_cast<uint8_t>(term[x] >> 8);
-            }
+            l[g + j] = fmaf(e0, ti.inv_vs, l[g + j]);
+            l[g + j + 1] = fmaf(e1, ti.inv_vs, l[g + j + 1]);
+            split_e4m3<kTerms>(e0, e1, kTermStep, term[j >> 1]);
           }
+#pragma unroll
+          for (int x = 0; x < kTerms; ++x)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              const uint32_t byte = (j & 1) ? term[j >> 1][x] >> 8 : term[j >> 1][x];
+              asm volatile("st.shared.u8 [%0], %1;" ::"r"((pb ^ (j << 4)) + (x * N + g + j) * kPage), "r"(byte) : "memory");
+            }
         }
         fence_proxy_async_smem();
         tc_fence_before();
@@ -579,50 +608,70 @@ __global__ void __launch_bounds__(kThreads, (Shape<DIM, N, kTermsOf<T>>::kBlocks
           mbar_arrive(b_pready + 8 * buf);
         }
       }
-      if (!ok) break;
+      if (gave_up) break;
       // ---- the unit's (or this block's part of its) result: thread = element of the head
+      float* sums = wmax + (turn & 1) * 4 * N;
+      ++turn;
 #pragma unroll
-      for (int r = 0; r < N; ++r) {
-        if ((r & ~3) >= rows) break;
+      for (int g = 0; g < N; g += 8) {
+        if (g >= rows) break;
+        // eight sums over 32 lanes: each step halves the values a lane still carries, lane i ends with row i mod 8
+        float a[4], b2[2], c;
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) l[r] += __shfl_xor_sync(0xffffffffu, l[r], o);
-      }
-      float4* sums = wmax + (xchg & 1) * N;
+        for (int j = 0; j < 4; ++j) {
+          const float give = (lane & 4) ? l[g + j] : l[g + j + 4], keep = (lane & 4) ? l[g + j + 4] : l[g + j];
+          a[j] = keep + __shfl_xor_sync(0xffffffffu, give, 4);
+        }
 #pragma unroll
-      for (int r = 0; r < N; ++r) {
-        if ((r & ~3) >= rows) break;
-        if (lane == 0) reinterpret_cast<float*>(sums + r)[quarter] = l[r];
+        for (int j = 0; j < 2; ++j) {
+          const float give = (lane & 2) ? a[j] : a[j + 2], keep = (lane & 2) ? a[j + 2] : a[j];
+          b2[j] = keep + __shfl_xor_sync(0xffffffffu, give, 2);
+        }
+        {
+          const float give = (lane & 1) ? b2[0] : b2[1], keep = (lane & 1) ? b2[1] : b2[0];
+          c = keep + __shfl_xor_sync(0xffffffffu, give, 1);
+        }
+        c += __shfl_xor_sync(0xffffffffu, c, 8);
+        c += __shfl_xor_sync(0xffffffffu, c, 16);
+        if (lane < 8) sums[quarter * N + g + lane] = c;
       }
-      if (!meet() || !warp_wait(b_pvdone + 8 * ((it - 1) & 1), ((it - 1) >> 1) & 1, abort_flag)) {
-        ok = false;
-        site = 7;
-        break;
-      }
+      wait(b_pvdone + 8 * ((it - 1) & 1), ((it - 1) >> 1) & 1, 4);
+      if (softmax_vote(!ok)) break;
       tc_fence_after();
       const bool whole_unit = t0 == 0 && t1 == v.tiles;
       const int64_t slot = 2 * static_cast<int64_t>(blockIdx.x) + (t0 > 0 ? 0 : 1);
+      T* out = static_cast<T*>(p.o) + v.lo * p.o_tok + static_cast<int64_t>(cur.h) * p.group * p.o_head + token;
+      int in_group = 0;
 #pragma unroll
-      for (int c = 0; c < N; c += 16) {
-        if (c >= rows) break;
-        uint32_t o[16];
-        tmem_ld_32x16(t_o + lane_off + c, o);
-        tmem_ld_wait();
+      for (int g = 0; g < N; g += 8) {
+        if (g >= rows) break;
+        float o[8];
 #pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          const int r = c + j;
+        for (int x = kTerms - 1; x >= 0; --x) {
+          uint32_t part[8];
+          tmem_ld_32x8(t_o + lane_off + x * N + g, part);
+          tmem_ld_wait();
+#pragma unroll
+          for (int j = 0; j < 8; ++j) o[j] = x == kTerms - 1 ? __uint_as_float(part[j]) : fmaf(o[j], 1.f / kTermStep, __uint_as_float(part[j]));
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const int r = g + j;
           if (r >= rows) break;
-          const float4 w = sums[r];
-          const float sum = (w.x + w.y) + (w.z + w.w);
-          float x = __uint_as_float(o[j]);
+          const float* w = sums + r;
+          const float sum = (w[0] + w[N]) + (w[2 * N] + w[3 * N]);
+          float x = o[j];
           if ((nan_rows >> r) & 1u) x = __uint_as_float(0x7fc00000u);
           if (whole_unit) {
-            const int i = r / p.group;
-            if (token < DIM)
-              static_cast<T*>(p.o)[(v.lo + i) * p.o_tok + (cur.h * p.group + r - i * p.group) * p.o_head + token] =
-                  static_cast<T>(sum == 0.f ? 0.f : x / sum);
+            if (token < DIM) *out = static_cast<T>(sum == 0.f ? 0.f : __fdividef(x, sum));
+            out += p.o_head;
+            if (++in_group == p.group) {
+              in_group = 0;
+              out += p.o_tok - p.group * p.o_head;
+            }
           } else {
             if (token < DIM) p.part_o[(slot * N + r) * DIM + token] = x;
-            if (token == 0) p.part_ml[slot * N + r] = make_float2(ref[r], sum);
+            if (token == 0) p.part_ml[slot * N + r] = make_float2(ref[side * N + r], sum);
           }
         }
       }
@@ -641,7 +690,7 @@ __global__ void __launch_bounds__(kThreads, (Shape<DIM, N, kTermsOf<T>>::kBlocks
       if (left > 0 && !next_unit(p, cur)) break;
     }
     if (!ok && lane == 0) *p.status = kRoleEpilogue * 1000 + site;
-    if (!ok && st == 0) p.record[blockIdx.x] = make_int4(-1, 0, 0, 0);
+    if (abort_flag[0] && st == 0) p.record[blockIdx.x] = make_int4(-1, 0, 0, 0);
   }
   tc_fence_before();
   __syncthreads();

@@ -40,13 +40,16 @@ __device__ __forceinline__ float exp2_approx(float v) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
   return r;
 }
-__device__ __forceinline__ void tmem_st_32x16(uint32_t taddr, const uint32_t (&r)[16]) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], "
-      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15};"
-      ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
-      "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(taddr)
-      : "memory");
+__device__ __forceinline__ void tmem_ld_32x8(uint32_t taddr, uint32_t (&r)[8]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+               : "r"(taddr)
+               : "memory");
+}
+__device__ __forceinline__ void tmem_st_32x8(uint32_t taddr, const uint32_t (&r)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%8], {%0, %1, %2, %3, %4, %5, %6, %7};" ::"r"(r[0]), "r"(r[1]), "r"(r[2]),
+               "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(taddr)
+               : "memory");
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
@@ -68,19 +71,21 @@ __device__ __forceinline__ uint32_t swizzled(int r, int e) {
   else return r * 64 + ((chunk ^ ((r >> 1) & 3)) << 4) + (e & 15);
 }
 
-// Two values as a sum of TERMS pairs of e4m3 values.  e4m3 has four significant bits, what a rounding leaves is at most 2^-4
-// of the value and again has a sign: two terms hold eight bits (a bf16 exactly), three twelve, of everything above 2^-3 ..
-// (half a step of the smallest term, 2^-10, below).
+// Two values as sums of TERMS pairs of e4m3 values, each `step` times smaller than it is stored beside the one before.
+// e4m3 has four significant bits; what a rounding leaves is at most 2^-4 of the value and has a sign again, so two terms
+// hold eight bits (a bf16 exactly), three twelve, down to half of the smallest step of the last term.
+constexpr float kTermStep = 16.f;
 template <int TERMS>
-__device__ __forceinline__ void split_e4m3(float lo, float hi, uint32_t (&term)[TERMS]) {
+__device__ __forceinline__ void split_e4m3(float lo, float hi, float step, uint32_t (&term)[TERMS]) {
 #pragma unroll
   for (int i = 0; i < TERMS; ++i) {
     const __nv_fp8x2_storage_t b = __nv_cvt_float2_to_fp8x2(make_float2(lo, hi), __NV_SATFINITE, __NV_E4M3);
     term[i] = b;
+    if (i + 1 == TERMS) break;
     const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(b, __NV_E4M3);
     const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
-    lo -= f.x;
-    hi -= f.y;
+    lo = (lo - f.x) * step;
+    hi = (hi - f.y) * step;
   }
 }
 
