@@ -61,6 +61,12 @@ __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatil
   return __all_sync(0xffffffffu, mbar_wait<kHint>(bar, parity, abort_flag));
 }
 
+__device__ __forceinline__ void load8(const float* src, float (&v)[8]) {
+  const float4 a = *reinterpret_cast<const float4*>(src), b = *reinterpret_cast<const float4*>(src + 4);
+  v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+  v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+}
+
 // The four softmax warps meet; true if any thread says so.  Nobody waits alone here: whatever a warp found, it comes.
 __device__ __forceinline__ bool softmax_vote(bool mine) {
   uint32_t any;
@@ -494,10 +500,8 @@ __global__ void __launch_bounds__(kThreads, (Shape<DIM, N, kTermsOf<T>>::kBlocks
             for (int g = 0; g < 16; g += 8) {
               if (c + g >= rows) break;
               float m[8], r[8];
-              *reinterpret_cast<float4*>(m) = *reinterpret_cast<const float4*>(rowmul + c + g);
-              *reinterpret_cast<float4*>(m + 4) = *reinterpret_cast<const float4*>(rowmul + c + g + 4);
-              *reinterpret_cast<float4*>(r) = *reinterpret_cast<const float4*>(ref + side * N + c + g);
-              *reinterpret_cast<float4*>(r + 4) = *reinterpret_cast<const float4*>(ref + side * N + c + g + 4);
+              load8(rowmul + c + g, m);
+              load8(ref + side * N + c + g, r);
 #pragma unroll
               for (int j = 0; j < 8; ++j) z[c + g + j] = fmaf(__uint_as_float(s[g + j]), m[j] * ti.ks, with_ref ? shift - r[j] : shift);
             }
@@ -547,18 +551,33 @@ __global__ void __launch_bounds__(kThreads, (Shape<DIM, N, kTermsOf<T>>::kBlocks
 #pragma unroll
           for (int g = 0; g < N; g += 8) {
             if (g >= rows) break;
-            float f[8];
+            float top[8], was[8], f[8];
+            load8(wm + g, top);
+#pragma unroll
+            for (int q = 1; q < 4; ++q) {
+              float w[8];
+              load8(wm + q * N + g, w);
+#pragma unroll
+              for (int j = 0; j < 8; ++j) top[j] = fmaxf(top[j], w[j]);
+            }
+            load8(old + g, was);
+            bool any = false;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-              const float* w = wm + g + j;
-              const float m = fmaxf(fmaxf(w[0], w[N]), fmaxf(w[2 * N], w[3 * N])) - kNominal, was = old[g + j];
-              const float r = m > was + (kLimit - kNominal) || was == kUnset ? fmaxf(m, kUnset) : was;
-              if (st == 0) now[g + j] = r;
-              f[j] = exp2_approx(was - r);
+              const float m = top[j] - kNominal;
+              const bool go = m > was[j] + (kLimit - kNominal) || was[j] == kUnset;
+              const float r = go ? fmaxf(m, kUnset) : was[j];
+              any = any || go;
+              f[j] = exp2_approx(was[j] - r);
               l[g + j] *= f[j];
               z[g + j] -= r;
+              top[j] = r;
             }
-            if (t > t0) {
+            if (st == 0) {
+              *reinterpret_cast<float4*>(now + g) = make_float4(top[0], top[1], top[2], top[3]);
+              *reinterpret_cast<float4*>(now + g + 4) = make_float4(top[4], top[5], top[6], top[7]);
+            }
+            if (t > t0 && any) {
 #pragma unroll
               for (int x = 0; x < kTerms; ++x) {
                 uint32_t o[8];
@@ -645,33 +664,51 @@ __global__ void __launch_bounds__(kThreads, (Shape<DIM, N, kTermsOf<T>>::kBlocks
 #pragma unroll
       for (int g = 0; g < N; g += 8) {
         if (g >= rows) break;
-        float o[8];
+        float o[8], sum[8];
+        uint32_t part[kTerms][8];
 #pragma unroll
-        for (int x = kTerms - 1; x >= 0; --x) {
-          uint32_t part[8];
-          tmem_ld_32x8(t_o + lane_off + x * N + g, part);
-          tmem_ld_wait();
+        for (int x = 0; x < kTerms; ++x) tmem_ld_32x8(t_o + lane_off + x * N + g, part[x]);
+        load8(sums + g, sum);
 #pragma unroll
-          for (int j = 0; j < 8; ++j) o[j] = x == kTerms - 1 ? __uint_as_float(part[j]) : fmaf(o[j], 1.f / kTermStep, __uint_as_float(part[j]));
+        for (int q = 1; q < 4; ++q) {
+          float w[8];
+          load8(sums + q * N + g, w);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) sum[j] += w[j];
         }
+        tmem_ld_wait();
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          const int r = g + j;
-          if (r >= rows) break;
-          const float* w = sums + r;
-          const float sum = (w[0] + w[N]) + (w[2 * N] + w[3 * N]);
-          float x = o[j];
-          if ((nan_rows >> r) & 1u) x = __uint_as_float(0x7fc00000u);
-          if (whole_unit) {
-            if (token < DIM) *out = static_cast<T>(sum == 0.f ? 0.f : __fdividef(x, sum));
+          o[j] = __uint_as_float(part[kTerms - 1][j]);
+#pragma unroll
+          for (int x = kTerms - 2; x >= 0; --x) o[j] = fmaf(o[j], 1.f / kTermStep, __uint_as_float(part[x][j]));
+        }
+        if (nan_rows != 0) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            if ((nan_rows >> (g + j)) & 1u) o[j] = __uint_as_float(0x7fc00000u);
+        }
+        if (whole_unit) {
+          T res[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) res[j] = static_cast<T>(sum[j] == 0.f ? 0.f : __fdividef(o[j], sum[j]));
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            if (g + j < rows && token < DIM) *out = res[j];
             out += p.o_head;
             if (++in_group == p.group) {
               in_group = 0;
               out += p.o_tok - p.group * p.o_head;
             }
-          } else {
-            if (token < DIM) p.part_o[(slot * N + r) * DIM + token] = x;
-            if (token == 0) p.part_ml[slot * N + r] = make_float2(ref[side * N + r], sum);
+          }
+        } else {
+          if (token < DIM) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) p.part_o[(slot * N + g + j) * DIM + token] = o[j];
+          }
+          if (token == 0) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) p.part_ml[slot * N + g + j] = make_float2(ref[side * N + g + j], sum[j]);
           }
         }
       }
