@@ -2,93 +2,11 @@
 //
 //   o_i = sum_j softmax_j(scale * q_i . k_j) v_j,  j <= pos_i  and  (j > pos_i - window  or  j < sinks)
 //
-// The simple form: one block per (new token, query head) walks the pages that the token sees, one thread per cached token
-// for the products with q, one thread per element of the head for the sums with v; running maximum and sum in 32 bits.
+// The C entry point: checks, tensor maps of the pages, and the choice between the kernel for few rows of a (sequence, cache
+// head), where reading the cache is the work, and the one for many, where the products are.
 #include <cstdio>
 
 #include "tg_attention.cuh"
-
-namespace tg {
-namespace {
-
-__device__ __forceinline__ float2 e4m3_two(uint32_t two) {
-  const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(two & 0xffffu), __NV_E4M3);
-  return __half22float2(*reinterpret_cast<const __half2*>(&h));
-}
-
-template <typename T, int DIM>
-__global__ void __launch_bounds__(128) tg_attention_simple_kernel(const AttentionParams p) {
-  __shared__ __align__(16) float q[DIM];
-  __shared__ float prob[kPage], red[4];
-  const int tok = blockIdx.x, head = blockIdx.y, tid = threadIdx.x;
-  griddep_wait();
-  griddep_launch_dependents();
-  int first, lo, hi;
-  const int b = find_sequence(p.c.cu, p.c.seqs, tok, 1, 0, first);
-  new_rows(p.c.cu, b, p.tokens, lo, hi);
-  if (tok < lo || tok >= hi) return;  // rows behind the last sequence
-  const int len = min(p.c.seq_lens[b], p.c.max_pages * kPage);
-  const int pos = p.c.seq_lens[b] - hi + tok;
-  const T* src = static_cast<const T*>(p.q) + tok * p.q_tok + head * p.q_head;
-  T* dst = static_cast<T*>(p.o) + tok * p.o_tok + head * p.o_head;
-  if (tid < DIM) q[tid] = static_cast<float>(src[tid]) * p.scale * 1.4426950408889634f;
-  __syncthreads();
-  const int kv = head / p.group;
-  const int64_t from = p.window > 0 ? max(static_cast<int64_t>(pos) - p.window + 1, int64_t(0)) : 0;
-  float m = -INFINITY, l = 0.f, acc = 0.f;
-  for (int page = 0; page * kPage < len && page * kPage <= pos; ++page) {
-    if ((page + 1) * static_cast<int64_t>(kPage) <= from && page * kPage >= p.sinks) continue;
-    const int phys = p.c.table[b * p.c.table_pitch + page];
-    if (phys < 0 || phys >= p.c.pages) continue;
-    const int64_t block = static_cast<int64_t>(phys) * p.c.heads + kv;
-    const int j = page * kPage + tid;
-    const bool seen = j < len && j <= pos && (j >= from || j < p.sinks);
-    float s = -INFINITY;
-    if (seen) {
-      const uint4* row = reinterpret_cast<const uint4*>(p.c.k + (block * kPage + tid) * DIM);
-      float dot = 0.f;
-#pragma unroll
-      for (int i = 0; i < DIM / 16; ++i) {
-        const uint4 w4 = row[i];
-        const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          const float2 f = e4m3_two(w[k >> 1] >> (16 * (k & 1)));
-          dot = fmaf(f.x, q[i * 16 + 2 * k], dot);
-          dot = fmaf(f.y, q[i * 16 + 2 * k + 1], dot);
-        }
-      }
-      s = dot * p.c.ks[block];
-    }
-    float mx = s;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-    if ((tid & 31) == 0) red[tid >> 5] = mx;
-    __syncthreads();
-    const float m_new = fmaxf(m, fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3])));
-    const float base = m_new == -INFINITY ? 0.f : m_new;
-    const float shrink = exp2f(m - base);
-    m = m_new;
-    prob[tid] = seen ? exp2f(s - base) : 0.f;
-    __syncthreads();
-    const float vs = p.c.vs[block];
-    float sum = 0.f, part = 0.f;
-    const int j0 = page * kPage;
-    for (int t = 0; t < kPage; ++t) {
-      const int at = j0 + t;
-      if (at >= len || at > pos || !(at >= from || at < p.sinks)) continue;
-      sum += prob[t];
-      if (tid < DIM) part = fmaf(prob[t], e4m3_two(p.c.v[(block * DIM + tid) * kPage + t]).x, part);
-    }
-    l = l * shrink + sum;
-    acc = acc * shrink + part * vs;
-    __syncthreads();
-  }
-  if (tid < DIM) dst[tid] = static_cast<T>(l > 0.f || l != l ? acc / l : 0.f);
-}
-
-}  // namespace
-}  // namespace tg
 
 using namespace tg;
 
@@ -156,6 +74,10 @@ extern "C" TG_API int32_t tg_paged_attention(const TgTensorDesc* O, const TgTens
   p.status = status;
   p.wait_limit_us = api_wait_limit_us();
   const cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  CUtensorMap tmK, tmV;
+  const int64_t page_heads = static_cast<int64_t>(p.c.pages) * p.c.heads;
+  if ((rc = api_make_page_map(&tmK, Kc->ptr, page_heads * kPage, p.c.dim, kPage)) != TG_OK) return rc;
+  if ((rc = api_make_page_map(&tmV, Vc->ptr, page_heads * p.c.dim, kPage, p.c.dim)) != TG_OK) return rc;
   if (const int rows = few_rows_of(heads, p.c.heads, max_q_len); rows > 0) {
     const int blocks = few_rows_blocks(p.c.dim, rows, Q->dtype == TG_BF16, num_sms);
     if (workspace == 0) return api_fail(TG_ERR_NULL, "the workspace is null");
@@ -165,24 +87,13 @@ extern "C" TG_API int32_t tg_paged_attention(const TgTensorDesc* O, const TgTens
     p.part_o = reinterpret_cast<float*>(workspace);
     p.part_ml = reinterpret_cast<float2*>(workspace + parts * p.c.dim * 4);
     p.record = reinterpret_cast<int4*>(workspace + parts * p.c.dim * 4 + parts * 8);
-    CUtensorMap tmK, tmV;
-    const int64_t page_heads = static_cast<int64_t>(p.c.pages) * p.c.heads;
-    if ((rc = api_make_page_map(&tmK, Kc->ptr, page_heads * kPage, p.c.dim, kPage)) != TG_OK) return rc;
-    if ((rc = api_make_page_map(&tmV, Vc->ptr, page_heads * p.c.dim, kPage, p.c.dim)) != TG_OK) return rc;
     const cudaError_t e = launch_attention_few_rows(tmK, tmV, p, rows, blocks, Q->dtype == TG_BF16, st);
     if (e == cudaSuccess) return TG_OK;
     char msg[160];
     snprintf(msg, sizeof(msg), "paged_attention launch failed: %s", cudaGetErrorString(e));
     return api_fail(TG_ERR_LAUNCH, msg);
   }
-  const dim3 grid(static_cast<unsigned>(T), static_cast<unsigned>(heads)), block(128);
-  cudaError_t e;
-  if (Q->dtype == TG_BF16)
-    e = D == 128 ? launch_pdl(tg_attention_simple_kernel<__nv_bfloat16, 128>, grid, block, 0, st, p)
-                 : launch_pdl(tg_attention_simple_kernel<__nv_bfloat16, 64>, grid, block, 0, st, p);
-  else
-    e = D == 128 ? launch_pdl(tg_attention_simple_kernel<__half, 128>, grid, block, 0, st, p)
-                 : launch_pdl(tg_attention_simple_kernel<__half, 64>, grid, block, 0, st, p);
+  const cudaError_t e = launch_attention_many_rows(tmK, tmV, p, Q->dtype == TG_BF16, st);
   if (e != cudaSuccess) {
     char msg[160];
     snprintf(msg, sizeof(msg), "paged_attention launch failed: %s", cudaGetErrorString(e));

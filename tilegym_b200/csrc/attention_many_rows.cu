@@ -1,0 +1,546 @@
+// Attention over the paged e4m3 cache for many rows: prompts, whole or in chunks.
+//
+// A block owns two tiles of 128 rows of one (sequence, cache head); a row is a (token, query head of the group) pair, so a
+// key or value page that is loaded once serves the whole group.
+//
+//   S [128 rows, 128 tokens] = Q . K^T      kind::f8f6f4 on the cached bytes, q split into e4m3 terms (bf16: two hold it
+//                                           exactly) that the accumulator sums: the time of one 16-bit product, no conversion of K
+//   p = 2^(S * scale * log2 e + log2 v_scale - ref)   thread = row: no exchange between threads at all
+//   O [128 rows, dim]       += P . V        kind::f16: P in f16 from TMEM, V converted e4m3 -> f16 (exact) by two warps once
+//                                           per page for both tiles
+//
+// Per page and tile the tensor core needs 512 + 512 clocks (dim 128) and the exponentials 1024 (16 a clock), so the two
+// tiles take turns: while one is in its softmax the tensor core does the other's products.  `ref` is a running maximum that
+// moves only when a p would exceed 2^8 (f16 has room for that), which is when O is rescaled in TMEM.  TMEM is full: S of
+// both tiles (P takes the place of the S it came from) and O of both.
+// Warp 0 copies pages, warp 1 issues products, warps 2-3 convert values, warps 4-7 and 8-11 are the tiles' softmax.
+#include <cstdio>
+
+#include "tg_attention.cuh"
+
+namespace tg {
+namespace {
+
+constexpr int kThreads = 384;
+constexpr float kUnset = -1e30f;  // the reference of a row that has not seen a token yet
+constexpr float kHeadroom = 8.f;
+
+template <int DIM, int TERMS>
+struct Shape {
+  static constexpr int kTile = DIM * kPage;      // bytes of a key or value page
+  static constexpr int kQ = TERMS * 128 * DIM;   // a tile's query terms
+  static constexpr int kV16 = 2 * kTile;
+  static constexpr int kStages = (226 * 1024 - 1024 - 1024 - 2 * kQ - 2 * kV16) / (2 * kTile) > 4
+                                     ? 4 : (226 * 1024 - 1024 - 1024 - 2 * kQ - 2 * kV16) / (2 * kTile);
+  static constexpr int kSmem = 1024 + kStages * 2 * kTile + 2 * kV16 + 2 * kQ + 1024;
+  static_assert(kStages >= 2, "two pages in flight");
+};
+
+// D[tmem] (+)= A[tmem, f16] . B[smem, f16]^T, K = 16
+__device__ __forceinline__ void mma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t"
+      ".reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t"
+      "}" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_32x32(uint32_t taddr, const uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31};"
+      ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+      "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]),
+      "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]),
+      "r"(r[31]), "r"(taddr)
+      : "memory");
+}
+
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile uint32_t* abort_flag) {
+  return __all_sync(0xffffffffu, mbar_wait<false>(bar, parity, abort_flag));
+}
+
+// e4m3 bytes to f16, a NaN to zero (`hits` tells that there was one).
+__device__ __forceinline__ void to_f16(uint32_t w, uint32_t& a, uint32_t& b, uint32_t& hits) {
+  const uint32_t hit = ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;  // 0x80 at every 0x7f
+  hits |= hit;
+  w &= ~((hit >> 7) * 255u);
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(a) : "h"(static_cast<uint16_t>(w)));
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(b) : "h"(static_cast<uint16_t>(w >> 16)));
+}
+
+template <typename T, int DIM>
+__global__ void __launch_bounds__(kThreads, 1)
+    tg_attention_many_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
+                                  const __grid_constant__ AttentionParams p, int token_tiles, int tile_tokens) {
+  constexpr int kTerms = std::is_same<T, __half>::value ? 3 : 2;
+  using Sh = Shape<DIM, kTerms>;
+  constexpr int kStages = Sh::kStages;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* v16_smem = smem + kStages * 2 * Sh::kTile;
+  uint8_t* q_smem = v16_smem + 2 * Sh::kV16;
+  uint8_t* misc = q_smem + 2 * Sh::kQ;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(misc);
+  volatile uint32_t* abort_flag = reinterpret_cast<volatile uint32_t*>(misc + 512);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(misc + 528);
+  uint32_t* nan_flag = reinterpret_cast<uint32_t*>(misc + 532);
+  const uint32_t bar0 = smem_u32(bars);
+  const uint32_t b_kfull = bar0, b_kempty = b_kfull + 8 * kStages, b_vfull = b_kempty + 8 * kStages, b_vempty = b_vfull + 8 * kStages,
+                 b_hfull = b_vempty + 8 * kStages, b_hempty = b_hfull + 16, b_sfull = b_hempty + 16, b_pready = b_sfull + 16,
+                 b_pvdone = b_pready + 16, b_qready = b_pvdone + 16;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  if (warp == 0) {
+    if (elect_one()) {
+      prefetch_tmap(&tmK);
+      prefetch_tmap(&tmV);
+    }
+    if (lane == 0) {
+      for (int i = 0; i < kStages; ++i) {
+        mbar_init(b_kfull + 8 * i, 1);
+        mbar_init(b_kempty + 8 * i, 1);
+        mbar_init(b_vfull + 8 * i, 1);
+        mbar_init(b_vempty + 8 * i, 2);
+      }
+      for (int i = 0; i < 2; ++i) {
+        mbar_init(b_hfull + 8 * i, 2);
+        mbar_init(b_hempty + 8 * i, 1);
+        mbar_init(b_sfull + 8 * i, 1);
+        mbar_init(b_pready + 8 * i, 4);
+        mbar_init(b_pvdone + 8 * i, 1);
+        mbar_init(b_qready + 8 * i, 4);
+      }
+      init_abort_flag(abort_flag, p.wait_limit_us);
+      *nan_flag = 0;
+      fence_mbar_init();
+    }
+  } else if (warp == 1) {
+    tmem_alloc(smem_u32(tmem_slot), 512);
+    tmem_relinquish();
+  }
+  griddep_wait();
+  griddep_launch_dependents();
+  // later tokens see more: their blocks come first
+  const int head = blockIdx.x % p.c.heads;
+  const int tile = token_tiles - 1 - blockIdx.x / p.c.heads;
+  int first;
+  const int b = find_sequence(p.c.cu, p.c.seqs, tile, 2 * tile_tokens, 1, first);
+  SeqView v = {};
+  if (tile >= first) v = view_sequence(p, b, (tile - first) * 2 * tile_tokens, 2 * tile_tokens);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  const int pages = v.n > 0 ? v.tiles : 0;
+  const int active = v.n > tile_tokens ? 2 : 1;  // tiles that have rows
+  bool ok = true;
+  int site = 0;
+
+  if (pages == 0) {
+    // no rows: a number of the ragged numbering that nobody has
+  } else if (warp == 0) {
+    // ------------------------------------------------------------------------------------------ copies
+    const int rows_k = p.c.pages * p.c.heads * kPage, rows_v = p.c.pages * p.c.heads * DIM;
+    int issued = 0;
+    for (int base = 0; base < pages && ok; base += 32) {
+      const int page = base + lane < pages ? v.page_of(base + lane) : p.c.max_pages;
+      int phys = page < p.c.max_pages ? p.c.table[b * p.c.table_pitch + page] : -1;
+      if (phys < 0 || phys >= p.c.pages) phys = -1;
+      for (int i = 0; i < min(32, pages - base); ++i, ++issued) {
+        const int stage = issued % kStages;
+        const uint32_t parity = ((issued / kStages) & 1) ^ 1;
+        const int ph = __shfl_sync(0xffffffffu, phys, i);
+        // a page that is not there: a box behind the end of the cache, which reads as zeros
+        const int yk = ph >= 0 ? (ph * p.c.heads + head) * kPage : rows_k, yv = ph >= 0 ? (ph * p.c.heads + head) * DIM : rows_v;
+        const uint32_t dst = smem_u32(smem + stage * 2 * Sh::kTile);
+        if (!warp_wait(b_kempty + 8 * stage, parity, abort_flag)) {
+          ok = false;
+          site = 1;
+          break;
+        }
+        if (elect_one()) {
+          mbar_arrive_expect_tx(b_kfull + 8 * stage, Sh::kTile);
+          tma_load_2d(dst, &tmK, b_kfull + 8 * stage, 0, yk);
+        }
+        __syncwarp();
+        if (!warp_wait(b_vempty + 8 * stage, parity, abort_flag)) {
+          ok = false;
+          site = 2;
+          break;
+        }
+        if (elect_one()) {
+          mbar_arrive_expect_tx(b_vfull + 8 * stage, Sh::kTile);
+          tma_load_2d(dst + Sh::kTile, &tmV, b_vfull + 8 * stage, 0, yv);
+        }
+        __syncwarp();
+      }
+    }
+    if (!ok) {
+      if (lane == 0) *p.status = kRoleProducer * 1000 + site;
+      // copies still in flight land before the block leaves (a bounded number of parked tries each; the page at which it
+      // stopped may have its keys under way)
+      for (int i = max(issued - kStages, 0); i <= issued; ++i) {
+        const uint32_t parity = (i / kStages) & 1;
+        if (i < issued || site == 2)
+          for (int tries = 0; tries < 1000 && !mbar_try_wait(b_kfull + 8 * (i % kStages), parity); ++tries) {
+          }
+        if (i < issued)
+          for (int tries = 0; tries < 1000 && !mbar_try_wait(b_vfull + 8 * (i % kStages), parity); ++tries) {
+          }
+      }
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------------------------------------ products
+    constexpr uint32_t idesc_s = make_idesc_e4m3_f32(128, kPage);
+    constexpr uint32_t idesc_o = make_idesc_e4m3_f32(128, DIM);  // the same fields: format 0 is f16 in kind::f16
+    const uint32_t q_addr = smem_u32(q_smem), v_addr = smem_u32(v16_smem);
+    auto scores = [&](int w, int j) {
+      const uint64_t bd = rows_desc<DIM>(smem_u32(smem + (j % kStages) * 2 * Sh::kTile));
+      if (elect_one()) {
+#pragma unroll
+        for (int term = 0; term < kTerms; ++term) {
+          const uint64_t ad = rows_desc<DIM>(q_addr + w * Sh::kQ + term * 128 * DIM);
+#pragma unroll
+          for (int k = 0; k < DIM / 32; ++k) mma_f8f6f4(tmem + w * 128, ad + 2 * k, bd + 2 * k, idesc_s, term + k > 0);
+        }
+        tc_commit(b_sfull + 8 * w);
+        if (w == active - 1) tc_commit(b_kempty + 8 * (j % kStages));
+      }
+      __syncwarp();
+    };
+    ok = warp_wait(b_kfull, 0, abort_flag);
+    for (int w = 0; w < active && ok; ++w) {
+      ok = warp_wait(b_qready + 8 * w, 0, abort_flag);
+      if (!ok) break;
+      tc_fence_after();
+      scores(w, 0);
+    }
+    if (!ok) site = 1;
+    for (int j = 0; j < pages && ok; ++j) {
+      for (int w = 0; w < active; ++w) {
+        if ((w == 0 && !warp_wait(b_hfull + 8 * (j & 1), (j >> 1) & 1, abort_flag)) || !warp_wait(b_pready + 8 * w, j & 1, abort_flag)) {
+          ok = false;
+          site = 2;
+          break;
+        }
+        tc_fence_after();
+        if (elect_one()) {
+#pragma unroll
+          for (int k = 0; k < kPage / 16; ++k) {
+            const uint64_t bd = make_kmajor_sw128_desc(v_addr + (j & 1) * Sh::kV16 + (k >> 2) * Sh::kTile) + 2 * (k & 3);
+            mma_f16_ts(tmem + 256 + w * 128, tmem + w * 128 + k * 8, bd, idesc_o, j + k > 0);
+          }
+          tc_commit(b_pvdone + 8 * w);
+          if (w == active - 1) tc_commit(b_hempty + 8 * (j & 1));
+        }
+        __syncwarp();
+        if (j + 1 < pages) {
+          // S takes the columns that P is read from: not before that product is done
+          if ((w == 0 && !warp_wait(b_kfull + 8 * ((j + 1) % kStages), ((j + 1) / kStages) & 1, abort_flag)) ||
+              !warp_wait(b_pvdone + 8 * w, j & 1, abort_flag)) {
+            ok = false;
+            site = 3;
+            break;
+          }
+          tc_fence_after();
+          scores(w, j + 1);
+        }
+      }
+    }
+    if (!ok && lane == 0) *p.status = kRoleMma * 1000 + site;
+  } else if (warp < 4) {
+    // ------------------------------------------------------------------------------------------ values to f16
+    const int t = (warp - 2) * 32 + lane;
+    bool nan = false;
+    for (int j = 0; j < pages; ++j) {
+      const int stage = j % kStages;
+      if (!warp_wait(b_vfull + 8 * stage, (j / kStages) & 1, abort_flag) || !warp_wait(b_hempty + 8 * (j & 1), ((j >> 1) & 1) ^ 1, abort_flag)) {
+        ok = false;
+        break;
+      }
+      const uint8_t* src = smem + stage * 2 * Sh::kTile + Sh::kTile;
+      uint8_t* dst = v16_smem + (j & 1) * Sh::kV16;
+#pragma unroll 4
+      for (int u = t; u < DIM * 8; u += 64) {
+        const int d = u % DIM, c = u / DIM;  // sixteen tokens of one element: 16 bytes in, 32 out
+        const uint4 w = *reinterpret_cast<const uint4*>(src + d * kPage + ((c ^ (d & 7)) << 4));
+        uint4 lo, hi;
+        uint32_t hits = 0;
+        to_f16(w.x, lo.x, lo.y, hits);
+        to_f16(w.y, lo.z, lo.w, hits);
+        to_f16(w.z, hi.x, hi.y, hits);
+        to_f16(w.w, hi.z, hi.w, hits);
+        if (hits != 0) {
+          // of interest only where some row sees the token
+          const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
+          const int at = v.page_of(j) * kPage + c * 16;
+#pragma unroll
+          for (int x = 0; x < 16; ++x)
+            if (((ww[x >> 2] >> (8 * (x & 3))) & 127u) == 127u && at + x < min(v.len, v.pos0 + v.n) &&
+                (p.window == 0 || at + x > static_cast<int64_t>(v.pos0) - p.window || at + x < p.sinks))
+              nan = true;
+        }
+        uint8_t* at = dst + (c >> 2) * Sh::kTile + d * 128;
+        const int c2 = (c & 3) * 2;
+        *reinterpret_cast<uint4*>(at + ((c2 ^ (d & 7)) << 4)) = lo;
+        *reinterpret_cast<uint4*>(at + (((c2 + 1) ^ (d & 7)) << 4)) = hi;
+      }
+      if (nan) *reinterpret_cast<volatile uint32_t*>(nan_flag) = 1u;
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(b_hfull + 8 * (j & 1));
+        mbar_arrive(b_vempty + 8 * stage);
+      }
+    }
+    if (!ok && lane == 0) *p.status = kRoleProducer * 1000 + 3;
+  } else if ((warp - 4) / 4 < active) {
+    // ------------------------------------------------------------------------------------------ softmax: thread = row
+    const int w = (warp - 4) / 4, quarter = warp & 3, row = quarter * 32 + lane;
+    const uint32_t lane_off = static_cast<uint32_t>(quarter * 32) << 16;
+    const uint32_t t_s = tmem + w * 128 + lane_off, t_o = tmem + 256 + w * 128 + lane_off;
+    const int i = w * tile_tokens + row / p.group, g = row % p.group;  // token of the block, head of the group
+    const bool live = row < tile_tokens * p.group && i < v.n;
+    const int pos = v.pos0 + i;
+    float mul;
+    {
+      const T* src = static_cast<const T*>(p.q) + static_cast<int64_t>(v.lo + i) * p.q_tok + (head * p.group + g) * p.q_head;
+      uint4 x[DIM / 8];
+      uint32_t top = 0;
+#pragma unroll
+      for (int e = 0; e < DIM / 8; ++e) x[e] = live ? *reinterpret_cast<const uint4*>(src + e * 8) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+      for (int e = 0; e < DIM / 8; ++e) {
+        const uint32_t ww[4] = {x[e].x, x[e].y, x[e].z, x[e].w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float2 u = unpack_pair<T>(ww[k]);
+          top = max(top, max(__float_as_uint(u.x) & 0x7fffffffu, __float_as_uint(u.y) & 0x7fffffffu));
+        }
+      }
+      const float sc = cache_scale(__uint_as_float(top)), inv = pow2_reciprocal(sc);
+      // a row that holds an infinity or NaN has no answer
+      mul = top >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : sc * p.scale * 1.4426950408889634f;
+#pragma unroll
+      for (int c = 0; c < DIM / 16; ++c) {
+        uint32_t out[kTerms][4];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const uint32_t ww[4] = {x[2 * c + h].x, x[2 * c + h].y, x[2 * c + h].z, x[2 * c + h].w};
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const float2 u = unpack_pair<T>(ww[k]);
+            uint32_t term[kTerms];
+            split_e4m3<kTerms>(u.x * inv, u.y * inv, 1.f, term);
+#pragma unroll
+            for (int y = 0; y < kTerms; ++y) out[y][h * 2 + (k >> 1)] = (k & 1) ? out[y][h * 2 + (k >> 1)] | (term[y] << 16) : term[y];
+          }
+        }
+#pragma unroll
+        for (int y = 0; y < kTerms; ++y)
+          *reinterpret_cast<uint4*>(q_smem + w * Sh::kQ + y * 128 * DIM + swizzled<DIM>(row, c * 16)) =
+              make_uint4(out[y][0], out[y][1], out[y][2], out[y][3]);
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(b_qready + 8 * w);
+    }
+    // what all rows of the tile see
+    const int tile_first = v.pos0 + w * tile_tokens, tile_last = v.pos0 + min(v.n, (w + 1) * tile_tokens) - 1;
+    const int all_hi = min(v.len, tile_first + 1);
+    const int all_lo = p.window > 0 ? static_cast<int>(max(static_cast<int64_t>(tile_last) - p.window + 1, int64_t(0))) : 0;
+    const int row_hi = min(v.len, pos + 1);
+    const int row_lo = p.window > 0 ? static_cast<int>(max(static_cast<int64_t>(pos) - p.window + 1, int64_t(0))) : 0;
+    // page and scales of the next pages, read ahead
+    auto page_number = [&](int j) {
+      const int page = j < pages ? v.page_of(j) : p.c.max_pages;
+      const int phys = page < p.c.max_pages ? p.c.table[b * p.c.table_pitch + page] : -1;
+      return phys >= 0 && phys < p.c.pages ? phys : -1;
+    };
+    auto scales = [&](int phys, float& ks, float& vs) {
+      ks = vs = 1.f;
+      if (phys >= 0) {
+        ks = p.c.ks[static_cast<int64_t>(phys) * p.c.heads + head];
+        vs = p.c.vs[static_cast<int64_t>(phys) * p.c.heads + head];
+      }
+    };
+    float ref = kUnset, l = 0.f, ks, vs, ks1, vs1;
+    int phys = page_number(0), phys1 = page_number(1);
+    scales(phys, ks, vs);
+    for (int j = 0; j < pages; ++j) {
+      scales(phys1, ks1, vs1);
+      const int phys2 = page_number(j + 2);
+      const int base = v.page_of(j) * kPage;
+      const bool whole = phys >= 0 && base + kPage <= all_hi && (base >= all_lo || base + kPage <= p.sinks);
+      const float lv = log2f(vs), f = mul * ks;
+      if (!warp_wait(b_sfull + 8 * w, j & 1, abort_flag)) {
+        ok = false;
+        site = 1;
+        break;
+      }
+      tc_fence_after();
+      uint32_t s[4][32];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) tmem_ld_32x32(t_s + c * 32, s[c]);
+      tmem_ld_wait();
+      if (!whole) {
+        const int hi = phys >= 0 ? row_hi - base : 0, lo = row_lo - base, sink = p.sinks - base;
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+          for (int k = 0; k < 32; ++k) {
+            const int t = c * 32 + k;
+            if (t >= hi || (t < lo && t >= sink)) s[c][k] = 0xff800000u;
+          }
+      }
+      float mx[4];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        mx[c] = __uint_as_float(s[c][0]);
+#pragma unroll
+        for (int k = 1; k < 32; ++k) mx[c] = fmaxf(mx[c], __uint_as_float(s[c][k]));
+      }
+      const float top = fmaf(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])), f, lv);
+      const bool move = top > ref + kHeadroom;
+      if (__any_sync(0xffffffffu, move)) {
+        const float now = move ? top : ref, shrink = exp2_approx(ref - now);
+        ref = now;
+        l *= shrink;
+        // the product of the page before is done: this page's S was issued behind it
+        if (j > 0) {
+#pragma unroll 1
+          for (int c = 0; c < DIM; c += 32) {
+            uint32_t o[32];
+            tmem_ld_32x32(t_o + c, o);
+            tmem_ld_wait();
+#pragma unroll
+            for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * shrink);
+            tmem_st_32x32(t_o + c, o);
+          }
+          tmem_st_wait();
+        }
+      }
+      const float shift = lv - ref;
+      float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        uint32_t pk[32];
+#pragma unroll
+        for (int k = 0; k < 32; ++k) {
+          const int c = h * 2 + (k >> 4), e = (k & 15) * 2;
+          const float p0 = exp2_approx(fmaf(__uint_as_float(s[c][e]), f, shift)), p1 = exp2_approx(fmaf(__uint_as_float(s[c][e + 1]), f, shift));
+          sum[k & 1] += p0;
+          sum[2 + (k & 1)] += p1;
+          pk[k] = pack_pair<__half>(p0, p1);
+        }
+        tmem_st_32x32(t_s + h * 32, pk);
+      }
+      // the sums take p as it is, in 32 bits
+      l = fmaf((sum[0] + sum[1]) + (sum[2] + sum[3]), 1.0f / vs, l);
+      tmem_st_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(b_pready + 8 * w);
+      phys = phys1;
+      ks = ks1;
+      vs = vs1;
+      phys1 = phys2;
+    }
+    if (ok && !warp_wait(b_pvdone + 8 * w, (pages - 1) & 1, abort_flag)) {
+      ok = false;
+      site = 2;
+    }
+    if (ok) {
+      tc_fence_after();
+      // a NaN among the values was kept from the products: it belongs to the rows that see its token
+      uint32_t bad[4] = {0, 0, 0, 0};
+      if (*reinterpret_cast<volatile uint32_t*>(nan_flag) != 0) {
+        for (int j = 0; j < pages; ++j) {
+          const int ph = page_number(j), base = v.page_of(j) * kPage;
+          if (ph < 0) continue;
+          const uint8_t* src = p.c.v + (static_cast<int64_t>(ph) * p.c.heads + head) * (kPage * DIM);
+          for (int u = 0; u < DIM * 8; ++u) {
+            const uint4 w = reinterpret_cast<const uint4*>(src)[u];
+            const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
+            const int d = u >> 3, t0 = base + (u & 7) * 16;
+#pragma unroll
+            for (int x = 0; x < 16; ++x)
+              if (((ww[x >> 2] >> (8 * (x & 3))) & 127u) == 127u && t0 + x < row_hi && (t0 + x >= row_lo || t0 + x < p.sinks)) {
+#pragma unroll
+                for (int y = 0; y < 4; ++y)
+                  if (y == (d >> 5)) bad[y] |= 1u << (d & 31);
+              }
+          }
+        }
+        __syncwarp();
+      }
+      const float inv = l == 0.f ? 0.f : 1.0f / l;
+      T* out = static_cast<T*>(p.o) + static_cast<int64_t>(v.lo + i) * p.o_tok + (head * p.group + g) * p.o_head;
+#pragma unroll
+      for (int c = 0; c < DIM; c += 32) {
+        uint32_t o[32];
+        tmem_ld_32x32(t_o + c, o);
+        tmem_ld_wait();
+        if (bad[c >> 5] != 0) {
+#pragma unroll
+          for (int k = 0; k < 32; ++k)
+            if ((bad[c >> 5] >> k) & 1u) o[k] = 0x7fc00000u;
+        }
+        if (live) {
+#pragma unroll
+          for (int k = 0; k < 32; k += 8) {
+            uint32_t r[4];
+#pragma unroll
+            for (int y = 0; y < 4; ++y)
+              r[y] = l == 0.f ? 0u : pack_pair<T>(__uint_as_float(o[k + 2 * y]) * inv, __uint_as_float(o[k + 2 * y + 1]) * inv);
+            *reinterpret_cast<uint4*>(out + c + k) = make_uint4(r[0], r[1], r[2], r[3]);
+          }
+        }
+      }
+      tc_fence_before();
+    }
+    if (!ok && lane == 0) *p.status = kRoleEpilogue * 1000 + site;
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+template <typename T, int DIM>
+cudaError_t launch(const CUtensorMap& tmK, const CUtensorMap& tmV, const AttentionParams& p, cudaStream_t stream) {
+  constexpr int kTerms = std::is_same<T, __half>::value ? 3 : 2;
+  using Sh = Shape<DIM, kTerms>;
+  auto kernel = tg_attention_many_rows_kernel<T, DIM>;
+  static bool set[64] = {};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (!set[dev & 63]) {
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Sh::kSmem);
+    if (e != cudaSuccess) return e;
+    set[dev & 63] = true;
+  }
+  const int tile_tokens = 128 / p.group;
+  const int64_t token_tiles = p.tokens / (2 * tile_tokens) + static_cast<int64_t>(p.c.seqs);
+  if (token_tiles * p.c.heads > 0x7fffffff) return cudaErrorInvalidValue;
+  return launch_pdl(kernel, dim3(static_cast<unsigned>(token_tiles * p.c.heads)), dim3(kThreads), Sh::kSmem, stream, tmK, tmV, p,
+                    static_cast<int>(token_tiles), tile_tokens);
+}
+
+}  // namespace
+
+cudaError_t launch_attention_many_rows(const CUtensorMap& tmK, const CUtensorMap& tmV, const AttentionParams& p, bool bf16,
+                                       cudaStream_t stream) {
+  if (bf16)
+    return p.c.dim == 128 ? launch<__nv_bfloat16, 128>(tmK, tmV, p, stream) : launch<__nv_bfloat16, 64>(tmK, tmV, p, stream);
+  return p.c.dim == 128 ? launch<__half, 128>(tmK, tmV, p, stream) : launch<__half, 64>(tmK, tmV, p, stream);
+}
+
+}  // namespace tg

@@ -28,6 +28,9 @@ int few_rows_blocks(int dim, int rows_padded, bool bf16, int num_sms);
 uint64_t few_rows_workspace(int dim, int rows_padded, int blocks);
 cudaError_t launch_attention_few_rows(const CUtensorMap& tmK, const CUtensorMap& tmV, const AttentionParams& p, int rows_padded,
                                       int blocks, bool bf16, cudaStream_t stream);
+// Many rows: the products are what counts.
+cudaError_t launch_attention_many_rows(const CUtensorMap& tmK, const CUtensorMap& tmV, const AttentionParams& p, bool bf16,
+                                       cudaStream_t stream);
 
 // ------------------------------------------------------------------------------------------ device side
 __device__ __forceinline__ float redux_max(float v) {
