@@ -410,8 +410,8 @@ TG_API int32_t tg_kv_cache_read(const TgTensorDesc* Ko, const TgTensorDesc* Vo, 
  * only j > i - window or j < sinks.  A token that sees nothing gets zeros.  max_q_len: no sequence has more new tokens than
  * this (rows beyond it are not computed).  workspace: at least tg_paged_attention_workspace_bytes() bytes, 16-byte
  * aligned, contents immaterial; calls that may overlap need one each. */
-TG_API uint64_t tg_paged_attention_workspace_bytes(int64_t tokens, int64_t q_heads, int64_t kv_heads, int64_t head_dim,
-                                                   int64_t seqs, int32_t max_q_len, int32_t num_sms);
+TG_API uint64_t tg_paged_attention_workspace_bytes(int64_t q_heads, int64_t kv_heads, int64_t head_dim, int32_t max_q_len,
+                                                   int32_t num_sms);
 TG_API int32_t tg_paged_attention(const TgTensorDesc* O, const TgTensorDesc* Q, const TgTensorDesc* Kc, const TgTensorDesc* Vc,
                                   const TgTensorDesc* Ks, const TgTensorDesc* Vs, const TgTensorDesc* block_table,
                                   const TgTensorDesc* seq_lens, const TgTensorDesc* cu_seqlens, int32_t max_q_len, float scale,

@@ -162,7 +162,7 @@ SIGNATURES = {
     ),
     "tg_kv_cache_read": (ctypes.c_int32, [_P] * 8 + [ctypes.c_int32, ctypes.c_uint64]),
     "tg_paged_attention_workspace_bytes": (
-        ctypes.c_uint64, [ctypes.c_int64] * 5 + [ctypes.c_int32, ctypes.c_int32],
+        ctypes.c_uint64, [ctypes.c_int64] * 3 + [ctypes.c_int32, ctypes.c_int32],
     ),
     "tg_paged_attention": (
         ctypes.c_int32,
@@ -196,29 +196,34 @@ def lib() -> ctypes.CDLL:
 
 
 # The descriptor is marshalled with one struct.pack call (about half the cost of filling a ctypes Structure
-# field by field); the packed bytes have exactly the layout of TensorDesc / TgTensorDesc.
-_DESC = struct.Struct("Qi4x5q5qi4x")
-assert _DESC.size == ctypes.sizeof(TensorDesc)
-_PAD = ((), (0,), (0, 0), (0, 0, 0), (0, 0, 0, 0), (0, 0, 0, 0, 0))
+# field by field); the packed bytes have exactly the layout of TensorDesc / TgTensorDesc.  One format per rank: the
+# unused extents and strides are pad bytes.
+_PACK = tuple(struct.Struct(f"Qi4x{n}q{8 * (5 - n)}x{n}q{8 * (5 - n)}xi4x").pack for n in range(6))
+assert len(_PACK[0](0, 0, 0)) == ctypes.sizeof(TensorDesc)
 
 
 def desc(t: Optional[torch.Tensor]) -> Optional[bytes]:
     """Descriptor of a tensor as the bytes of a TgTensorDesc (None passes through as a NULL pointer)."""
     if t is None:
         return None
-    nd = t.dim()
+    shape = t.shape
+    nd = len(shape)
     if nd > 5:
         raise ValueError("tensors of more than 5 dimensions are not supported")
     code = DTYPE_CODES.get(t.dtype)
     if code is None:
         raise TileGymB200Error(-2, f"dtype {t.dtype} has no code in the C ABI")
-    pad = _PAD[5 - nd]
-    return _DESC.pack(t.data_ptr(), nd, *t.shape, *pad, *t.stride(), *pad, code)
+    return _PACK[nd](t.data_ptr(), nd, *shape, *t.stride(), code)
 
 
 def desc2d(ptr: int, rows: int, cols: int, row_stride: int, dtype: torch.dtype) -> bytes:
     """Descriptor of a row-major 2-D view given by numbers (saves creating the view tensor)."""
-    return _DESC.pack(ptr, 2, rows, cols, 0, 0, 0, row_stride, 1, 0, 0, 0, DTYPE_CODES[dtype])
+    return _PACK[2](ptr, 2, rows, cols, row_stride, 1, DTYPE_CODES[dtype])
+
+
+def desc3d(ptr: int, n0: int, n1: int, n2: int, s0: int, s1: int, dtype: torch.dtype) -> bytes:
+    """Descriptor of a 3-D view with a dense last dimension, given by numbers."""
+    return _PACK[3](ptr, 3, n0, n1, n2, s0, s1, 1, DTYPE_CODES[dtype])
 
 
 def ref(d: Optional[bytes]):

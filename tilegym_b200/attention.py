@@ -11,6 +11,7 @@ is read back, so the calls can be captured into a CUDA graph whose tables change
 
 from __future__ import annotations
 
+import functools
 import math
 from typing import NamedTuple, Optional, Tuple
 
@@ -102,16 +103,26 @@ def rope_frequencies(
     return f.to(device), magnitude
 
 
-def _heads(x: torch.Tensor, name: str) -> torch.Tensor:
-    """[tokens, heads, dim] as the kernels read it (itself, or a copy where a pitch breaks the 16-byte alignment)."""
+def _heads(x: torch.Tensor, name: str) -> Tuple[torch.Tensor, bytes]:
+    """[tokens, heads, dim] as the kernels read it (itself, or a copy where a pitch breaks the 16-byte alignment), and its
+    descriptor.  The tensor has to be held until the launch: the allocator would hand a copy's memory to the next one."""
     if x.dim() != 3:
         raise _lib.TileGymB200Error(-6, f"{name} must be [tokens, heads, head_dim]")
     if x.dtype not in _16BIT:
         raise _lib.TileGymB200Error(-2, f"{name} must be bf16 or f16, got {x.dtype}")
+    n0, n1, n2 = x.shape
     s0, s1, s2 = x.stride()
     if s2 != 1 or s0 % 8 or s1 % 8 or x.data_ptr() % 16:
-        return x.clone(memory_format=torch.contiguous_format)
-    return x
+        x = x.clone(memory_format=torch.contiguous_format)
+        s0, s1 = n1 * n2, n2
+    return x, _lib.desc3d(x.data_ptr(), n0, n1, n2, s0, s1, x.dtype)
+
+
+def _new_heads(x: torch.Tensor) -> Tuple[torch.Tensor, bytes]:
+    """A dense new tensor of x's shape and type, and its descriptor."""
+    n0, n1, n2 = x.shape
+    out = torch.empty_like(x, memory_format=torch.contiguous_format)
+    return out, _lib.desc3d(out.data_ptr(), n0, n1, n2, n1 * n2, n2, x.dtype)
 
 
 def _frequencies(inv_freq: torch.Tensor) -> torch.Tensor:
@@ -149,23 +160,24 @@ def apply_rope(
     With inplace=True q and k are overwritten (their pitches must keep 16-byte alignment) and only the rotated elements
     are touched.
     """
-    dev = ops._need_cuda(q, k, positions, inv_freq)
+    dev = ops._cuda_index(q, k, positions, inv_freq)
     ops._no_grad_inputs(q, k)
-    q1, k1 = _heads(q, "q"), None if k is None else _heads(k, "k")
+    q1, q_desc = _heads(q, "q")
+    k1, k_desc = (None, None) if k is None else _heads(k, "k")
     if inplace:
         assert q1 is q and k1 is k, "in-place rotation needs dense heads on 16-byte boundaries"
-        qo, ko = q, k
+        qo, qo_desc, ko, ko_desc = q, q_desc, k, k_desc
     else:
-        qo = torch.empty(q.shape, dtype=q.dtype, device=dev)
-        ko = None if k is None else torch.empty(k.shape, dtype=k.dtype, device=dev)
+        qo, qo_desc = _new_heads(q)
+        ko, ko_desc = (None, None) if k is None else _new_heads(k)
     if positions.dtype not in (torch.int32, torch.int64):
         raise _lib.TileGymB200Error(-2, f"positions must be int32 or int64, got {positions.dtype}")
     if not positions.is_contiguous():
         positions = positions.contiguous()
     inv_freq = _frequencies(inv_freq)
     rc = _lib.lib().tg_apply_rope(
-        _lib.desc(qo), _lib.desc(ko), _lib.desc(q1), _lib.desc(k1), _lib.desc(positions), _lib.desc(inv_freq),
-        1 if interleaved else 0, float(magnitude), dev.index, ops._stream(dev),
+        qo_desc, ko_desc, q_desc, k_desc, _lib.desc(positions), _lib.desc(inv_freq), 1 if interleaved else 0, float(magnitude), dev,
+        torch._C._cuda_getCurrentRawStream(dev),
     )
     _lib.check_rc(rc)
     return qo, ko
@@ -197,24 +209,24 @@ def kv_cache_write(
     cu_seqlens, positions outside the table and pages outside the cache are left alone (their rows of q are unspecified).
     A page that is written must belong to one sequence.
     """
-    dev = ops._need_cuda(*cache, k, v, block_table, seq_lens, cu_seqlens, inv_freq, q)
+    dev = ops._cuda_index(*cache, k, v, block_table, seq_lens, cu_seqlens, inv_freq, q)
     ops._no_grad_inputs(k, v, q)
-    qo = None
+    qo = qo_desc = q_desc = None
     if q is not None:
         if inv_freq is None:
             raise _lib.TileGymB200Error(-6, "q is passed to be rotated: inv_freq is missing")
-        q = _heads(q, "q")
-        qo = torch.empty(q.shape, dtype=q.dtype, device=dev)
-    # every copy made here keeps its name until the launch: the allocator would hand its memory to the next one
-    k, v = _heads(k, "k"), _heads(v, "v")
+        q, q_desc = _heads(q, "q")
+        qo, qo_desc = _new_heads(q)
+    k, k_desc = _heads(k, "k")
+    v, v_desc = _heads(v, "v")
     block_table, seq_lens, cu_seqlens = _tables(block_table, seq_lens, cu_seqlens)
     if inv_freq is not None:
         inv_freq = _frequencies(inv_freq)
+    desc = _lib.desc
     rc = _lib.lib().tg_kv_cache_write(
-        _lib.desc(cache.k), _lib.desc(cache.v), _lib.desc(cache.k_scale), _lib.desc(cache.v_scale), _lib.desc(k),
-        _lib.desc(v), _lib.desc(block_table), _lib.desc(seq_lens), _lib.desc(cu_seqlens), _lib.desc(qo), _lib.desc(q),
-        _lib.desc(inv_freq), 1 if interleaved else 0, float(magnitude), dev.index,
-        ops._stream(dev),
+        desc(cache.k), desc(cache.v), desc(cache.k_scale), desc(cache.v_scale), k_desc, v_desc, desc(block_table), desc(seq_lens),
+        desc(cu_seqlens), qo_desc, q_desc, desc(inv_freq), 1 if interleaved else 0, float(magnitude), dev,
+        torch._C._cuda_getCurrentRawStream(dev),
     )
     _lib.check_rc(rc)
     return qo
@@ -268,36 +280,32 @@ def paged_attention(
     computed.  A token that sees nothing (a sequence of length 0 in a padded batch) gets zeros; rows outside cu_seqlens
     are not written.
     """
-    dev = ops._need_cuda(q, *cache, block_table, seq_lens, cu_seqlens, out)
+    dev = ops._cuda_index(q, *cache, block_table, seq_lens, cu_seqlens, out)
     ops._no_grad_inputs(q)
-    q = _heads(q, "q")
+    q, q_desc = _heads(q, "q")
     tokens, heads, dim = q.shape
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+        out, out_desc = _new_heads(q)
     else:
         assert out.shape == q.shape and out.dtype == q.dtype, "out must have q's shape and type"
+        out_desc = _lib.desc(out)
     if max_q_len is None:
         max_q_len = 1 if cu_seqlens is None else max(tokens, 1)
     block_table, seq_lens, cu_seqlens = _tables(block_table, seq_lens, cu_seqlens)
-    L = _lib.lib()
-    seqs = seq_lens.shape[0]
-    need = L.tg_paged_attention_workspace_bytes(tokens, heads, cache.k.shape[1], dim, seqs, int(max_q_len), _sms(dev))
+    need = _workspace_bytes(heads, cache.k.shape[1], dim, max_q_len, dev)
     # allocated per call: calls on other streams, and graphs that are replayed side by side, never share it
-    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-    rc = L.tg_paged_attention(
-        _lib.desc(out), _lib.desc(q), _lib.desc(cache.k), _lib.desc(cache.v), _lib.desc(cache.k_scale), _lib.desc(cache.v_scale),
-        _lib.desc(block_table), _lib.desc(seq_lens), _lib.desc(cu_seqlens), int(max_q_len), dim ** -0.5 if scale is None else float(scale), int(window),
-        int(sinks), ws.data_ptr() if ws is not None else 0, need, dev.index, ops._stream(dev),
+    ws = q.new_empty(need, dtype=torch.uint8) if need else None
+    desc = _lib.desc
+    rc = _lib.lib().tg_paged_attention(
+        out_desc, q_desc, desc(cache.k), desc(cache.v), desc(cache.k_scale), desc(cache.v_scale), desc(block_table), desc(seq_lens),
+        desc(cu_seqlens), int(max_q_len), dim ** -0.5 if scale is None else float(scale), int(window), int(sinks),
+        0 if ws is None else ws.data_ptr(), need, dev, torch._C._cuda_getCurrentRawStream(dev),
     )
     _lib.check_rc(rc)
     return out
 
 
-_sm_counts = {}
-
-
-def _sms(dev: torch.device) -> int:
-    n = _sm_counts.get(dev.index)
-    if n is None:
-        n = _sm_counts[dev.index] = torch.cuda.get_device_properties(dev).multi_processor_count
-    return n
+@functools.lru_cache(maxsize=256)
+def _workspace_bytes(heads: int, kv_heads: int, dim: int, max_q_len: int, dev: int) -> int:
+    sms = torch.cuda.get_device_properties(dev).multi_processor_count
+    return _lib.lib().tg_paged_attention_workspace_bytes(heads, kv_heads, dim, int(max_q_len), sms)

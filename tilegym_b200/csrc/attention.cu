@@ -17,7 +17,7 @@ static int few_rows_of(int64_t q_heads, int64_t kv_heads, int32_t max_q_len) {
   return rows <= kFewRowsMax ? few_rows_padded(static_cast<int>(rows)) : 0;
 }
 
-extern "C" TG_API uint64_t tg_paged_attention_workspace_bytes(int64_t, int64_t q_heads, int64_t kv_heads, int64_t head_dim, int64_t,
+extern "C" TG_API uint64_t tg_paged_attention_workspace_bytes(int64_t q_heads, int64_t kv_heads, int64_t head_dim,
                                                               int32_t max_q_len, int32_t num_sms) {
   const int rows = few_rows_of(q_heads, kv_heads, max_q_len);
   if (rows == 0) return 0;

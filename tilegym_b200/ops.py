@@ -46,6 +46,19 @@ def _need_cuda(*tensors: Optional[torch.Tensor]) -> torch.device:
     return dev
 
 
+def _cuda_index(*tensors: Optional[torch.Tensor]) -> int:
+    """`_need_cuda` for calls whose host time counts: the device's index."""
+    index = -1
+    for t in tensors:
+        if t is None:
+            continue
+        d = t.get_device()
+        if d < 0 or (d != index and index >= 0):
+            _need_cuda(*tensors)  # raises
+        index = d
+    return index
+
+
 def _stream(dev: torch.device) -> int:
     return torch._C._cuda_getCurrentRawStream(dev.index)
 
@@ -337,44 +350,50 @@ def rms_norm_quant(
     `fp8_block_scaled_mm` takes as A / As.  x, residual (..., hidden) bf16 or f16, hidden a multiple of 128 up to
     65536; weight (hidden,) in x's type or fp32.  With inplace=True h is written over `residual`.
     """
-    dev = _need_cuda(x, weight, residual)
+    dev = _cuda_index(x, weight, residual)
     _no_grad_inputs(x, residual)
     hidden = x.shape[-1]
-    if x.dtype not in (torch.bfloat16, torch.float16):
-        raise _lib.TileGymB200Error(-2, f"rms_norm_quant takes bf16 or f16, got {x.dtype}")
+    dtype = x.dtype
+    if dtype not in (torch.bfloat16, torch.float16):
+        raise _lib.TileGymB200Error(-2, f"rms_norm_quant takes bf16 or f16, got {dtype}")
     assert hidden % 128 == 0 and hidden > 0, "the hidden size must be a multiple of 128"
     assert weight.shape == (hidden,), "weight must hold one value per hidden element"
-    x2 = _rows16(x.reshape(-1, hidden))
-    T = x2.shape[0]
-    y = torch.empty(x.shape, dtype=_FP8, device=dev)
-    s = torch.empty(x.shape[:-1] + (hidden // 128,), dtype=torch.float32, device=dev)
-    r2 = h = None
+    shape = x.shape
+    x, x_desc, rows = _rows16(x, hidden)
+    y = torch.empty(shape, dtype=_FP8, device=x.device) if x.shape != shape or not x.is_contiguous() else torch.empty_like(x, dtype=_FP8)
+    s = x.new_empty(shape[:-1] + (hidden // 128,), dtype=torch.float32)
+    r_desc = h = None
     if residual is not None:
-        assert residual.shape == x.shape and residual.dtype == x.dtype, "residual must have x's shape and type"
+        assert residual.shape == shape and residual.dtype == dtype, "residual must have x's shape and type"
         if inplace:
             assert residual.is_contiguous() and residual.data_ptr() % 16 == 0, "an in-place residual must be contiguous and 16-byte aligned"
             h = residual
         else:
-            h = torch.empty(x.shape, dtype=x.dtype, device=dev)
-        r2 = _rows16(residual.reshape(-1, hidden))
+            h = torch.empty_like(y, dtype=dtype)
+        residual, r_desc, _ = _rows16(residual, hidden)
     else:
         assert not inplace, "inplace=True writes the sum over the residual: there is none"
     if not weight.is_contiguous() or weight.data_ptr() % 16:
         weight = weight.clone(memory_format=torch.contiguous_format)
     rc = _lib.lib().tg_rms_norm_quant(
-        _lib.desc2d(y.data_ptr(), T, hidden, hidden, _FP8), _lib.desc2d(s.data_ptr(), T, hidden // 128, hidden // 128, torch.float32),
-        _lib.desc2d(h.data_ptr(), T, hidden, hidden, h.dtype) if h is not None else None, _lib.desc(x2), _lib.desc(r2),
-        _lib.desc(weight), float(eps), float(weight_offset), dev.index, _stream(dev),
+        _lib.desc2d(y.data_ptr(), rows, hidden, hidden, _FP8), _lib.desc2d(s.data_ptr(), rows, hidden // 128, hidden // 128, torch.float32),
+        None if h is None else _lib.desc2d(h.data_ptr(), rows, hidden, hidden, dtype), x_desc, r_desc, _lib.desc(weight), float(eps),
+        float(weight_offset), dev, torch._C._cuda_getCurrentRawStream(dev),
     )
     _lib.check_rc(rc)
     return (y, s) if h is None else (y, s, h)
 
 
-def _rows16(x2: torch.Tensor) -> torch.Tensor:
-    """A 2-D tensor whose rows are dense and start on 16-byte boundaries (itself, or a copy)."""
-    if x2.stride(1) != 1 or x2.data_ptr() % 16 or x2.stride(0) * x2.element_size() % 16:
-        return x2.clone(memory_format=torch.contiguous_format)
-    return x2
+def _rows16(x: torch.Tensor, hidden: int) -> Tuple[torch.Tensor, bytes, int]:
+    """(x, descriptor, rows) of x (..., hidden) as a matrix whose rows are dense and start on 16-byte boundaries: x itself,
+    a view, or a copy."""
+    if x.is_contiguous() and x.data_ptr() % 16 == 0:  # rows are hidden * 2 bytes: a multiple of 16 with the 128-blocks
+        rows = x.numel() // hidden
+        return x, _lib.desc2d(x.data_ptr(), rows, hidden, hidden, x.dtype), rows
+    x = x.reshape(-1, hidden)
+    if x.stride(1) != 1 or x.data_ptr() % 16 or x.stride(0) * x.element_size() % 16:
+        x = x.clone(memory_format=torch.contiguous_format)
+    return x, _lib.desc(x), x.shape[0]
 
 
 def weight_dequant(
