@@ -205,6 +205,10 @@ __device__ __forceinline__ uint32_t pack_pair(float a, float b) {
   }
 }
 
+// One pair turned: written out so that every kernel rounds alike.
+__device__ __forceinline__ float turn_first(float x, float y, float2 cs) { return __fmaf_rn(x, cs.x, -__fmul_rn(y, cs.y)); }
+__device__ __forceinline__ float turn_second(float x, float y, float2 cs) { return __fmaf_rn(y, cs.x, __fmul_rn(x, cs.y)); }
+
 // Turns 8 pairs.  Half layout: a holds elements i .. i + 7 of the head, b their partners i + rotary / 2 ..; interleaved:
 // a and b hold 16 neighbouring elements and pairs sit side by side.  Both come back rounded to T.
 template <typename T>
@@ -215,16 +219,16 @@ __device__ __forceinline__ void rotate_unit(uint4& a, uint4& b, const float2 (&c
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const float2 x = unpack_pair<T>(wa[i]), y = unpack_pair<T>(wb[i]);
-      wa[i] = pack_pair<T>(x.x * cs[i].x - x.y * cs[i].y, x.y * cs[i].x + x.x * cs[i].y);
-      wb[i] = pack_pair<T>(y.x * cs[i + 4].x - y.y * cs[i + 4].y, y.y * cs[i + 4].x + y.x * cs[i + 4].y);
+      wa[i] = pack_pair<T>(turn_first(x.x, x.y, cs[i]), turn_second(x.x, x.y, cs[i]));
+      wb[i] = pack_pair<T>(turn_first(y.x, y.y, cs[i + 4]), turn_second(y.x, y.y, cs[i + 4]));
     }
   } else {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const float2 x = unpack_pair<T>(wa[i]), y = unpack_pair<T>(wb[i]);
       const float2 c0 = cs[2 * i], c1 = cs[2 * i + 1];
-      wa[i] = pack_pair<T>(x.x * c0.x - y.x * c0.y, x.y * c1.x - y.y * c1.y);
-      wb[i] = pack_pair<T>(y.x * c0.x + x.x * c0.y, y.y * c1.x + x.y * c1.y);
+      wa[i] = pack_pair<T>(turn_first(x.x, y.x, c0), turn_first(x.y, y.y, c1));
+      wb[i] = pack_pair<T>(turn_second(x.x, y.x, c0), turn_second(x.y, y.y, c1));
     }
   }
 }
