@@ -11,7 +11,7 @@
 //
 // Per page and tile the tensor core needs 512 + 512 clocks (dim 128) and the exponentials 1024 (16 a clock), so the two
 // tiles take turns: while one is in its softmax the tensor core does the other's products.  `ref` is a running maximum that
-// moves only when a p would exceed 2^8 (f16 has room for that), which is when O is rescaled in TMEM.  TMEM is full: S of
+// moves only when a p would exceed 2^14 (f16 has room for that), which is when O is rescaled in TMEM.  TMEM is full: S of
 // both tiles (P takes the place of the S it came from) and O of both.
 // Warp 0 copies pages, warp 1 issues products, warps 2-3 convert values, warps 4-7 and 8-11 are the tiles' softmax.
 #include <cstdio>
@@ -22,8 +22,9 @@ namespace tg {
 namespace {
 
 constexpr int kThreads = 384;
+constexpr int kRegsOther = 88, kRegsSoftmax = 208;
 constexpr float kUnset = -1e30f;  // the reference of a row that has not seen a token yet
-constexpr float kHeadroom = 8.f;
+constexpr float kHeadroom = 14.f;  // p may reach 2^14 before ref moves (f16 ends at 2^16)
 
 template <int DIM, int TERMS>
 struct Shape {
@@ -140,9 +141,14 @@ __global__ void __launch_bounds__(kThreads, 1)
   bool ok = true;
   int site = 0;
 
-  if (pages == 0) {
-    // no rows: a number of the ragged numbering that nobody has
-  } else if (warp == 0) {
+  // Registers: 168 per thread at launch; the four warps that copy, multiply and convert give 80 each, the eight softmax warps,
+  // which hold a row of S, take 40 each: (88 + 2 * 208) * 128 is within the launch's 168 * 384.
+  static_assert((kRegsOther + 2 * kRegsSoftmax) * 128 <= 168 * kThreads, "the pool of a block is what it was launched with");
+  if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsOther));
+    if (pages == 0) {
+      // no rows: a number of the ragged numbering that nobody has
+    } else if (warp == 0) {
     // ------------------------------------------------------------------------------------------ copies
     const int rows_k = p.c.pages * p.c.heads * kPage, rows_v = p.c.pages * p.c.heads * DIM;
     int issued = 0;
@@ -193,7 +199,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
       }
     }
-  } else if (warp == 1) {
+    } else if (warp == 1) {
     // ------------------------------------------------------------------------------------------ products
     constexpr uint32_t idesc_s = make_idesc_e4m3_f32(128, kPage);
     constexpr uint32_t idesc_o = make_idesc_e4m3_f32(128, DIM);  // the same fields: format 0 is f16 in kind::f16
@@ -252,7 +258,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     }
     if (!ok && lane == 0) *p.status = kRoleMma * 1000 + site;
-  } else if (warp < 4) {
+    } else {
     // ------------------------------------------------------------------------------------------ values to f16
     const int t = (warp - 2) * 32 + lane;
     bool nan = false;
@@ -298,7 +304,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     }
     if (!ok && lane == 0) *p.status = kRoleProducer * 1000 + 3;
-  } else if ((warp - 4) / 4 < active) {
+    }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax));
+    if (pages > 0 && (warp - 4) / 4 < active) {
     // ------------------------------------------------------------------------------------------ softmax: thread = row
     const int w = (warp - 4) / 4, quarter = warp & 3, row = quarter * 32 + lane;
     const uint32_t lane_off = static_cast<uint32_t>(quarter * 32) << 16;
@@ -355,25 +364,25 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int all_lo = p.window > 0 ? static_cast<int>(max(static_cast<int64_t>(tile_last) - p.window + 1, int64_t(0))) : 0;
     const int row_hi = min(v.len, pos + 1);
     const int row_lo = p.window > 0 ? static_cast<int>(max(static_cast<int64_t>(pos) - p.window + 1, int64_t(0))) : 0;
-    // page and scales of the next pages, read ahead
-    auto page_number = [&](int j) {
+    // page numbers two pages ahead, scales one: nothing here waits for a load that it has just issued
+    auto page_entry = [&](int j) {
       const int page = j < pages ? v.page_of(j) : p.c.max_pages;
-      const int phys = page < p.c.max_pages ? p.c.table[b * p.c.table_pitch + page] : -1;
-      return phys >= 0 && phys < p.c.pages ? phys : -1;
+      return page < p.c.max_pages ? p.c.table[b * p.c.table_pitch + page] : -1;
     };
     auto scales = [&](int phys, float& ks, float& vs) {
       ks = vs = 1.f;
-      if (phys >= 0) {
+      if (phys >= 0 && phys < p.c.pages) {
         ks = p.c.ks[static_cast<int64_t>(phys) * p.c.heads + head];
         vs = p.c.vs[static_cast<int64_t>(phys) * p.c.heads + head];
       }
     };
     float ref = kUnset, l = 0.f, ks, vs, ks1, vs1;
-    int phys = page_number(0), phys1 = page_number(1);
-    scales(phys, ks, vs);
+    int entry = page_entry(0), entry1 = page_entry(1);
+    scales(entry, ks, vs);
     for (int j = 0; j < pages; ++j) {
-      scales(phys1, ks1, vs1);
-      const int phys2 = page_number(j + 2);
+      scales(entry1, ks1, vs1);
+      const int entry2 = page_entry(j + 2);
+      const int phys = entry >= 0 && entry < p.c.pages ? entry : -1;
       const int base = v.page_of(j) * kPage;
       const bool whole = phys >= 0 && base + kPage <= all_hi && (base >= all_lo || base + kPage <= p.sinks);
       const float lv = log2f(vs), f = mul * ks;
@@ -445,10 +454,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(b_pready + 8 * w);
-      phys = phys1;
+      entry = entry1;
       ks = ks1;
       vs = vs1;
-      phys1 = phys2;
+      entry1 = entry2;
     }
     if (ok && !warp_wait(b_pvdone + 8 * w, (pages - 1) & 1, abort_flag)) {
       ok = false;
@@ -460,8 +469,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       uint32_t bad[4] = {0, 0, 0, 0};
       if (*reinterpret_cast<volatile uint32_t*>(nan_flag) != 0) {
         for (int j = 0; j < pages; ++j) {
-          const int ph = page_number(j), base = v.page_of(j) * kPage;
-          if (ph < 0) continue;
+          const int ph = page_entry(j), base = v.page_of(j) * kPage;
+          if (ph < 0 || ph >= p.c.pages) continue;
           const uint8_t* src = p.c.v + (static_cast<int64_t>(ph) * p.c.heads + head) * (kPage * DIM);
           for (int u = 0; u < DIM * 8; ++u) {
             const uint4 w = reinterpret_cast<const uint4*>(src)[u];
@@ -504,6 +513,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       tc_fence_before();
     }
     if (!ok && lane == 0) *p.status = kRoleEpilogue * 1000 + site;
+    }
   }
   tc_fence_before();
   __syncthreads();
