@@ -9,11 +9,13 @@
 //   O [128 rows, dim]       += P . V        kind::f16: P in f16 from TMEM, V converted e4m3 -> f16 (exact) by two warps once
 //                                           per page for both tiles
 //
-// Per page and tile the tensor core needs 512 + 512 clocks (dim 128) and the exponentials 1024 (16 a clock), so the two
-// tiles take turns: while one is in its softmax the tensor core does the other's products.  `ref` is a running maximum that
-// moves only when a p would exceed 2^14 (f16 has room for that), which is when O is rescaled in TMEM.  TMEM is full: S of
-// both tiles (P takes the place of the S it came from) and O of both.
-// Warp 0 copies pages, warp 1 issues products, warps 2-3 convert values, warps 4-7 and 8-11 are the tiles' softmax.
+// The work goes by half pages (64 tokens): TMEM holds O of both tiles (2 x 128 columns) and two S buffers of 64 columns for
+// each, P taking the place of the S it came from, so that the next scores are there when a softmax is done with the last
+// and the tensor core never waits for one tile alone.  `ref` is a running maximum that
+// moves only when a p would exceed 2^14 (f16 has room for that), which is when O is rescaled in TMEM.
+// Warp 0 copies pages, warps 1 and 2 issue the score and the value products (a warp that issues is held up until the tensor
+// core has nearly caught up and then needs a few hundred clocks to find its next barriers ready: one warp for both left
+// the tensor core idle 60 % of the time), warps 4-7 convert values, warps 8-11 and 12-15 are the tiles' softmax.
 #include <cstdio>
 
 #include "tg_attention.cuh"
@@ -21,8 +23,9 @@
 namespace tg {
 namespace {
 
-constexpr int kThreads = 384;
-constexpr int kRegsOther = 88, kRegsSoftmax = 208;
+constexpr int kThreads = 512;
+constexpr int kRegsLaunch = 128, kRegsOther = 72, kRegsSoftmax = 184;
+constexpr int kHalf = kPage / 2;  // tokens of a step
 constexpr float kUnset = -1e30f;  // the reference of a row that has not seen a token yet
 constexpr float kHeadroom = 14.f;  // p may reach 2^14 before ref moves (f16 ends at 2^16)
 
@@ -64,11 +67,9 @@ __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatil
   return __all_sync(0xffffffffu, mbar_wait<false>(bar, parity, abort_flag));
 }
 
-// e4m3 bytes to f16, a NaN to zero (`hits` tells that there was one).
-__device__ __forceinline__ void to_f16(uint32_t w, uint32_t& a, uint32_t& b, uint32_t& hits) {
-  const uint32_t hit = ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;  // 0x80 at every 0x7f
-  hits |= hit;
-  w &= ~((hit >> 7) * 255u);
+__device__ __forceinline__ uint32_t nan_bytes(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }  // 0x80 at every 0x7f
+
+__device__ __forceinline__ void to_f16(uint32_t w, uint32_t& a, uint32_t& b) {
   asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(a) : "h"(static_cast<uint16_t>(w)));
   asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(b) : "h"(static_cast<uint16_t>(w >> 16)));
 }
@@ -91,8 +92,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint32_t* nan_flag = reinterpret_cast<uint32_t*>(misc + 532);
   const uint32_t bar0 = smem_u32(bars);
   const uint32_t b_kfull = bar0, b_kempty = b_kfull + 8 * kStages, b_vfull = b_kempty + 8 * kStages, b_vempty = b_vfull + 8 * kStages,
-                 b_hfull = b_vempty + 8 * kStages, b_hempty = b_hfull + 16, b_sfull = b_hempty + 16, b_pready = b_sfull + 16,
-                 b_pvdone = b_pready + 16, b_qready = b_pvdone + 16;
+                 b_hfull = b_vempty + 8 * kStages, b_hempty = b_hfull + 16, b_qready = b_hempty + 16;
+  // by tile and buffer: + 16 * tile + 8 * buffer
+  const uint32_t b_sfull = b_qready + 16, b_pready = b_sfull + 32, b_pvdone = b_pready + 32;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   if (warp == 0) {
@@ -105,15 +107,17 @@ __global__ void __launch_bounds__(kThreads, 1)
         mbar_init(b_kfull + 8 * i, 1);
         mbar_init(b_kempty + 8 * i, 1);
         mbar_init(b_vfull + 8 * i, 1);
-        mbar_init(b_vempty + 8 * i, 2);
+        mbar_init(b_vempty + 8 * i, 4);
       }
       for (int i = 0; i < 2; ++i) {
-        mbar_init(b_hfull + 8 * i, 2);
+        mbar_init(b_hfull + 8 * i, 4);
         mbar_init(b_hempty + 8 * i, 1);
+        mbar_init(b_qready + 8 * i, 4);
+      }
+      for (int i = 0; i < 4; ++i) {
         mbar_init(b_sfull + 8 * i, 1);
         mbar_init(b_pready + 8 * i, 4);
         mbar_init(b_pvdone + 8 * i, 1);
-        mbar_init(b_qready + 8 * i, 4);
       }
       init_abort_flag(abort_flag, p.wait_limit_us);
       *nan_flag = 0;
@@ -137,16 +141,15 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   const int pages = v.n > 0 ? v.tiles : 0;
-  const int active = v.n > tile_tokens ? 2 : 1;  // tiles that have rows
+  const int tiles = v.n > tile_tokens ? 2 : 1;  // that have rows
   bool ok = true;
   int site = 0;
 
-  // Registers: 168 per thread at launch; the four warps that copy, multiply and convert give 80 each, the eight softmax warps,
-  // which hold a row of S, take 40 each: (88 + 2 * 208) * 128 is within the launch's 168 * 384.
-  static_assert((kRegsOther + 2 * kRegsSoftmax) * 128 <= 168 * kThreads, "the pool of a block is what it was launched with");
-  if (warp < 4) {
+  // Registers: the warps that copy, multiply and convert give up what the softmax warps, which hold half a row of S, take.
+  static_assert(2 * kRegsOther + 2 * kRegsSoftmax <= 4 * kRegsLaunch && kRegsLaunch * kThreads <= 65536, "within what the block was launched with");
+  if (warp < 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsOther));
-    if (pages == 0) {
+    if (pages == 0 || warp == 3) {
       // no rows: a number of the ragged numbering that nobody has
     } else if (warp == 0) {
     // ------------------------------------------------------------------------------------------ copies
@@ -199,68 +202,78 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
       }
     }
-    } else if (warp == 1) {
+    } else if (warp < 3) {
     // ------------------------------------------------------------------------------------------ products
-    constexpr uint32_t idesc_s = make_idesc_e4m3_f32(128, kPage);
+    constexpr uint32_t idesc_s = make_idesc_e4m3_f32(128, kHalf);
     constexpr uint32_t idesc_o = make_idesc_e4m3_f32(128, DIM);  // the same fields: format 0 is f16 in kind::f16
-    const uint32_t q_addr = smem_u32(q_smem), v_addr = smem_u32(v16_smem);
-    auto scores = [&](int w, int j) {
-      const uint64_t bd = rows_desc<DIM>(smem_u32(smem + (j % kStages) * 2 * Sh::kTile));
-      if (elect_one()) {
-#pragma unroll
-        for (int term = 0; term < kTerms; ++term) {
-          const uint64_t ad = rows_desc<DIM>(q_addr + w * Sh::kQ + term * 128 * DIM);
-#pragma unroll
-          for (int k = 0; k < DIM / 32; ++k) mma_f8f6f4(tmem + w * 128, ad + 2 * k, bd + 2 * k, idesc_s, term + k > 0);
-        }
-        tc_commit(b_sfull + 8 * w);
-        if (w == active - 1) tc_commit(b_kempty + 8 * (j % kStages));
+    // every number that an address is made of comes from lane 0, so that it can live in uniform registers
+    const uint32_t base = __shfl_sync(0xffffffffu, smem_u32(smem), 0), tm = __shfl_sync(0xffffffffu, tmem, 0);
+    const uint32_t v_addr = base + kStages * 2 * Sh::kTile, q_addr = v_addr + 2 * Sh::kV16;
+    const int halves = 2 * __shfl_sync(0xffffffffu, pages, 0), active = __shfl_sync(0xffffffffu, tiles, 0);
+    auto need = [&](uint32_t bar, uint32_t parity, int where) {
+      if (ok && !warp_wait(bar, parity, abort_flag)) {
+        ok = false;
+        site = where;
       }
-      __syncwarp();
     };
-    ok = warp_wait(b_kfull, 0, abort_flag);
-    for (int w = 0; w < active && ok; ++w) {
-      ok = warp_wait(b_qready + 8 * w, 0, abort_flag);
-      if (!ok) break;
-      tc_fence_after();
-      scores(w, 0);
-    }
-    if (!ok) site = 1;
-    for (int j = 0; j < pages && ok; ++j) {
-      for (int w = 0; w < active; ++w) {
-        if ((w == 0 && !warp_wait(b_hfull + 8 * (j & 1), (j >> 1) & 1, abort_flag)) || !warp_wait(b_pready + 8 * w, j & 1, abort_flag)) {
-          ok = false;
-          site = 2;
-          break;
-        }
-        tc_fence_after();
-        if (elect_one()) {
-#pragma unroll
-          for (int k = 0; k < kPage / 16; ++k) {
-            const uint64_t bd = make_kmajor_sw128_desc(v_addr + (j & 1) * Sh::kV16 + (k >> 2) * Sh::kTile) + 2 * (k & 3);
-            mma_f16_ts(tmem + 256 + w * 128, tmem + w * 128 + k * 8, bd, idesc_o, j + k > 0);
-          }
-          tc_commit(b_pvdone + 8 * w);
-          if (w == active - 1) tc_commit(b_hempty + 8 * (j & 1));
-        }
-        __syncwarp();
-        if (j + 1 < pages) {
-          // S takes the columns that P is read from: not before that product is done
-          if ((w == 0 && !warp_wait(b_kfull + 8 * ((j + 1) % kStages), ((j + 1) / kStages) & 1, abort_flag)) ||
-              !warp_wait(b_pvdone + 8 * w, j & 1, abort_flag)) {
-            ok = false;
-            site = 3;
-            break;
-          }
+    if (warp == 1) {
+      // scores of half page h of tile w, into buffer h & 1: behind the product that read P from there
+      int stage = 0;
+      uint32_t round = 0;
+      need(b_qready, 0, 1);
+      if (active == 2) need(b_qready + 8, 0, 1);
+#pragma unroll 1
+      for (int h = 0; h < halves && ok; ++h) {
+        const int buf = h & 1;
+        if (buf == 0) need(b_kfull + 8 * stage, round, 2);
+#pragma unroll 1
+        for (int w = 0; w < active; ++w) {
+          if (h >= 2) need(b_pvdone + 16 * w + 8 * buf, ((h >> 1) & 1) ^ 1, 3);
+          if (!ok) break;
           tc_fence_after();
-          scores(w, j + 1);
+          if (elect_one()) {
+            const uint64_t bd = rows_desc<DIM>(base + stage * 2 * Sh::kTile + buf * kHalf * DIM);
+#pragma unroll
+            for (int term = 0; term < kTerms; ++term) {
+              const uint64_t ad = rows_desc<DIM>(q_addr + w * Sh::kQ + term * 128 * DIM);
+#pragma unroll
+              for (int k = 0; k < DIM / 32; ++k) mma_f8f6f4(tm + w * 128 + buf * kHalf, ad + 2 * k, bd + 2 * k, idesc_s, term + k > 0);
+            }
+            tc_commit(b_sfull + 16 * w + 8 * buf);
+            if (w == active - 1 && buf == 1) tc_commit(b_kempty + 8 * stage);
+          }
+          __syncwarp();
+        }
+        if (buf == 1 && ++stage == kStages) {
+          stage = 0;
+          round ^= 1u;
+        }
+      }
+    } else {
+#pragma unroll 1
+      for (int h = 0; h < halves && ok; ++h) {
+        const int j = h >> 1, buf = h & 1;
+        if (buf == 0) need(b_hfull + 8 * (j & 1), (j >> 1) & 1, 4);
+#pragma unroll 1
+        for (int w = 0; w < active; ++w) {
+          need(b_pready + 16 * w + 8 * buf, j & 1, 5);
+          if (!ok) break;
+          tc_fence_after();
+          if (elect_one()) {
+            const uint64_t bd = make_kmajor_sw128_desc(v_addr + (j & 1) * Sh::kV16 + buf * Sh::kTile);
+#pragma unroll
+            for (int k = 0; k < kHalf / 16; ++k) mma_f16_ts(tm + 256 + w * 128, tm + w * 128 + buf * kHalf + k * 8, bd + 2 * k, idesc_o, h + k > 0);
+            tc_commit(b_pvdone + 16 * w + 8 * buf);
+            if (w == active - 1 && buf == 1) tc_commit(b_hempty + 8 * (j & 1));
+          }
+          __syncwarp();
         }
       }
     }
     if (!ok && lane == 0) *p.status = kRoleMma * 1000 + site;
     } else {
     // ------------------------------------------------------------------------------------------ values to f16
-    const int t = (warp - 2) * 32 + lane;
+    const int t = (warp - 4) * 32 + lane;
     bool nan = false;
     for (int j = 0; j < pages; ++j) {
       const int stage = j % kStages;
@@ -271,25 +284,26 @@ __global__ void __launch_bounds__(kThreads, 1)
       const uint8_t* src = smem + stage * 2 * Sh::kTile + Sh::kTile;
       uint8_t* dst = v16_smem + (j & 1) * Sh::kV16;
 #pragma unroll 4
-      for (int u = t; u < DIM * 8; u += 64) {
+      for (int u = t; u < DIM * 8; u += 128) {
         const int d = u % DIM, c = u / DIM;  // sixteen tokens of one element: 16 bytes in, 32 out
         const uint4 w = *reinterpret_cast<const uint4*>(src + d * kPage + ((c ^ (d & 7)) << 4));
-        uint4 lo, hi;
-        uint32_t hits = 0;
-        to_f16(w.x, lo.x, lo.y, hits);
-        to_f16(w.y, lo.z, lo.w, hits);
-        to_f16(w.z, hi.x, hi.y, hits);
-        to_f16(w.w, hi.z, hi.w, hits);
-        if (hits != 0) {
-          // of interest only where some row sees the token
-          const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
+        uint32_t ww[4] = {w.x, w.y, w.z, w.w};
+        if ((nan_bytes(w.x) | nan_bytes(w.y) | nan_bytes(w.z) | nan_bytes(w.w)) != 0) {
+          // a NaN becomes zero here, and is of interest only where some row sees the token
           const int at = v.page_of(j) * kPage + c * 16;
 #pragma unroll
           for (int x = 0; x < 16; ++x)
             if (((ww[x >> 2] >> (8 * (x & 3))) & 127u) == 127u && at + x < min(v.len, v.pos0 + v.n) &&
                 (p.window == 0 || at + x > static_cast<int64_t>(v.pos0) - p.window || at + x < p.sinks))
               nan = true;
+#pragma unroll
+          for (int x = 0; x < 4; ++x) ww[x] &= ~((nan_bytes(ww[x]) >> 7) * 255u);
         }
+        uint4 lo, hi;
+        to_f16(ww[0], lo.x, lo.y);
+        to_f16(ww[1], lo.z, lo.w);
+        to_f16(ww[2], hi.x, hi.y);
+        to_f16(ww[3], hi.z, hi.w);
         uint8_t* at = dst + (c >> 2) * Sh::kTile + d * 128;
         const int c2 = (c & 3) * 2;
         *reinterpret_cast<uint4*>(at + ((c2 ^ (d & 7)) << 4)) = lo;
@@ -307,11 +321,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax));
-    if (pages > 0 && (warp - 4) / 4 < active) {
+    if (pages > 0 && (warp - 8) / 4 < tiles) {
     // ------------------------------------------------------------------------------------------ softmax: thread = row
-    const int w = (warp - 4) / 4, quarter = warp & 3, row = quarter * 32 + lane;
+    const int w = (warp - 8) / 4, quarter = warp & 3, row = quarter * 32 + lane;
     const uint32_t lane_off = static_cast<uint32_t>(quarter * 32) << 16;
-    const uint32_t t_s = tmem + w * 128 + lane_off, t_o = tmem + 256 + w * 128 + lane_off;
+    const uint32_t t_s0 = tmem + w * 128 + lane_off, t_o = tmem + 256 + w * 128 + lane_off;
     const int i = w * tile_tokens + row / p.group, g = row % p.group;  // token of the block, head of the group
     const bool live = row < tile_tokens * p.group && i < v.n;
     const int pos = v.pos0 + i;
@@ -379,89 +393,103 @@ __global__ void __launch_bounds__(kThreads, 1)
     float ref = kUnset, l = 0.f, ks, vs, ks1, vs1;
     int entry = page_entry(0), entry1 = page_entry(1);
     scales(entry, ks, vs);
-    for (int j = 0; j < pages; ++j) {
+    for (int j = 0; j < pages && ok; ++j) {
       scales(entry1, ks1, vs1);
       const int entry2 = page_entry(j + 2);
-      const int phys = entry >= 0 && entry < p.c.pages ? entry : -1;
-      const int base = v.page_of(j) * kPage;
-      const bool whole = phys >= 0 && base + kPage <= all_hi && (base >= all_lo || base + kPage <= p.sinks);
-      const float lv = log2f(vs), f = mul * ks;
-      if (!warp_wait(b_sfull + 8 * w, j & 1, abort_flag)) {
-        ok = false;
-        site = 1;
-        break;
+      const bool here = entry >= 0 && entry < p.c.pages;
+      const float f = mul * ks;
+      // log2 and reciprocal of the page's scale: a power of two where the cache was written by this library
+      const uint32_t vb = __float_as_uint(vs);
+      float lv, inv_vs;
+      if ((vb & 0x807fffffu) == 0 && vb >= 0x00800000u && vb < 0x7e800000u) {
+        lv = static_cast<float>(static_cast<int>(vb >> 23) - 127);
+        inv_vs = pow2_reciprocal(vs);
+      } else {
+        lv = log2f(vs);
+        inv_vs = 1.0f / vs;
       }
-      tc_fence_after();
-      uint32_t s[4][32];
-#pragma unroll
-      for (int c = 0; c < 4; ++c) tmem_ld_32x32(t_s + c * 32, s[c]);
-      tmem_ld_wait();
-      if (!whole) {
-        const int hi = phys >= 0 ? row_hi - base : 0, lo = row_lo - base, sink = p.sinks - base;
-#pragma unroll
-        for (int c = 0; c < 4; ++c)
-#pragma unroll
-          for (int k = 0; k < 32; ++k) {
-            const int t = c * 32 + k;
-            if (t >= hi || (t < lo && t >= sink)) s[c][k] = 0xff800000u;
-          }
-      }
-      float mx[4];
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        mx[c] = __uint_as_float(s[c][0]);
-#pragma unroll
-        for (int k = 1; k < 32; ++k) mx[c] = fmaxf(mx[c], __uint_as_float(s[c][k]));
-      }
-      const float top = fmaf(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])), f, lv);
-      const bool move = top > ref + kHeadroom;
-      if (__any_sync(0xffffffffu, move)) {
-        const float now = move ? top : ref, shrink = exp2_approx(ref - now);
-        ref = now;
-        l *= shrink;
-        // the product of the page before is done: this page's S was issued behind it
-        if (j > 0) {
 #pragma unroll 1
-          for (int c = 0; c < DIM; c += 32) {
-            uint32_t o[32];
-            tmem_ld_32x32(t_o + c, o);
-            tmem_ld_wait();
-#pragma unroll
-            for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * shrink);
-            tmem_st_32x32(t_o + c, o);
-          }
-          tmem_st_wait();
+      for (int half = 0; half < 2; ++half) {
+        const int base = v.page_of(j) * kPage + half * kHalf;
+        const bool whole = here && base + kHalf <= all_hi && (base >= all_lo || base + kHalf <= p.sinks);
+        const uint32_t t_s = t_s0 + half * kHalf;
+        if (!warp_wait(b_sfull + 16 * w + 8 * half, j & 1, abort_flag)) {
+          ok = false;
+          site = 1;
+          break;
         }
-      }
-      const float shift = lv - ref;
-      float sum[4] = {0.f, 0.f, 0.f, 0.f};
+        tc_fence_after();
+        uint32_t s[2][32];
+        tmem_ld_32x32(t_s, s[0]);
+        tmem_ld_32x32(t_s + 32, s[1]);
+        tmem_ld_wait();
+        if (!whole) {
+          const int hi = here ? row_hi - base : 0, lo = row_lo - base, sink = p.sinks - base;
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
+          for (int t = 0; t < kHalf; ++t)
+            if (t >= hi || (t < lo && t >= sink)) s[t >> 5][t & 31] = 0xff800000u;
+        }
+        float mx[4];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          mx[c] = __uint_as_float(s[c >> 1][(c & 1) * 16]);
+#pragma unroll
+          for (int k = 1; k < 16; ++k) mx[c] = fmaxf(mx[c], __uint_as_float(s[c >> 1][(c & 1) * 16 + k]));
+        }
+        const float top = fmaf(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])), f, lv);
+        const bool move = top > ref + (ref == kUnset ? 0.f : kHeadroom);
+        if (__any_sync(0xffffffffu, move)) {
+          const float now = move ? top : ref, shrink = exp2_approx(ref - now);
+          ref = now;
+          l *= shrink;
+          if (j + half > 0) {
+            // not before the product of the half page in front is done
+            const int h = 2 * j + half - 1;
+            if (!warp_wait(b_pvdone + 16 * w + 8 * (h & 1), (h >> 1) & 1, abort_flag)) {
+              ok = false;
+              site = 2;
+              break;
+            }
+            tc_fence_after();
+#pragma unroll 1
+            for (int c = 0; c < DIM; c += 32) {
+              uint32_t o[32];
+              tmem_ld_32x32(t_o + c, o);
+              tmem_ld_wait();
+#pragma unroll
+              for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * shrink);
+              tmem_st_32x32(t_o + c, o);
+            }
+            tmem_st_wait();
+          }
+        }
+        const float shift = lv - ref;
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};
         uint32_t pk[32];
 #pragma unroll
         for (int k = 0; k < 32; ++k) {
-          const int c = h * 2 + (k >> 4), e = (k & 15) * 2;
+          const int c = k >> 4, e = (k & 15) * 2;
           const float p0 = exp2_approx(fmaf(__uint_as_float(s[c][e]), f, shift)), p1 = exp2_approx(fmaf(__uint_as_float(s[c][e + 1]), f, shift));
           sum[k & 1] += p0;
           sum[2 + (k & 1)] += p1;
           pk[k] = pack_pair<__half>(p0, p1);
         }
-        tmem_st_32x32(t_s + h * 32, pk);
+        tmem_st_32x32(t_s, pk);
+        // the sums take p as it is, in 32 bits
+        l = fmaf((sum[0] + sum[1]) + (sum[2] + sum[3]), inv_vs, l);
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(b_pready + 16 * w + 8 * half);
       }
-      // the sums take p as it is, in 32 bits
-      l = fmaf((sum[0] + sum[1]) + (sum[2] + sum[3]), 1.0f / vs, l);
-      tmem_st_wait();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(b_pready + 8 * w);
       entry = entry1;
       ks = ks1;
       vs = vs1;
       entry1 = entry2;
     }
-    if (ok && !warp_wait(b_pvdone + 8 * w, (pages - 1) & 1, abort_flag)) {
+    if (ok && !warp_wait(b_pvdone + 16 * w + 8, (pages - 1) & 1, abort_flag)) {
       ok = false;
-      site = 2;
+      site = 3;
     }
     if (ok) {
       tc_fence_after();
