@@ -13,9 +13,9 @@
 // each, P taking the place of the S it came from, so that the next scores are there when a softmax is done with the last
 // and the tensor core never waits for one tile alone.  `ref` is a running maximum that
 // moves only when a p would exceed 2^14 (f16 has room for that), which is when O is rescaled in TMEM.
-// Warp 0 copies pages, warps 1 and 2 issue the score and the value products (a warp that issues is held up until the tensor
-// core has nearly caught up and then needs a few hundred clocks to find its next barriers ready: one warp for both left
-// the tensor core idle 60 % of the time), warps 4-7 convert values, warps 8-11 and 12-15 are the tiles' softmax.
+// Warp 0 copies pages, warps 1 and 2 issue the tiles' score products and warp 3 the value products (a warp that issues is
+// held up until the tensor core has nearly caught up and then needs a few hundred clocks to find its next barriers ready:
+// with one warp for all the tensor core was idle 60 % of the time, with two 45 %), warps 4-7 convert values, warps 8-11 and 12-15 are the tiles' softmax.
 #include <cstdio>
 
 #include "tg_attention.cuh"
@@ -34,9 +34,9 @@ struct Shape {
   static constexpr int kTile = DIM * kPage;      // bytes of a key or value page
   static constexpr int kQ = TERMS * 128 * DIM;   // a tile's query terms
   static constexpr int kV16 = 2 * kTile;
-  static constexpr int kStages = (226 * 1024 - 1024 - 1024 - 2 * kQ - 2 * kV16) / (2 * kTile) > 4
-                                     ? 4 : (226 * 1024 - 1024 - 1024 - 2 * kQ - 2 * kV16) / (2 * kTile);
-  static constexpr int kSmem = 1024 + kStages * 2 * kTile + 2 * kV16 + 2 * kQ + 1024;
+  static constexpr int kStages = (227 * 1024 - 1024 - 2048 - 2 * kQ - 2 * kV16) / (2 * kTile) > 4
+                                     ? 4 : (227 * 1024 - 1024 - 2048 - 2 * kQ - 2 * kV16) / (2 * kTile);
+  static constexpr int kSmem = 1024 + kStages * 2 * kTile + 2 * kV16 + 2 * kQ + 2048;
   static_assert(kStages >= 2, "two pages in flight");
 };
 
@@ -90,6 +90,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   volatile uint32_t* abort_flag = reinterpret_cast<volatile uint32_t*>(misc + 512);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(misc + 528);
   uint32_t* nan_flag = reinterpret_cast<uint32_t*>(misc + 532);
+  float* rowmul = reinterpret_cast<float*>(misc + 1024);  // [2][128]
   const uint32_t bar0 = smem_u32(bars);
   const uint32_t b_kfull = bar0, b_kempty = b_kfull + 8 * kStages, b_vfull = b_kempty + 8 * kStages, b_vempty = b_vfull + 8 * kStages,
                  b_hfull = b_vempty + 8 * kStages, b_hempty = b_hfull + 16, b_qready = b_hempty + 16;
@@ -105,7 +106,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (lane == 0) {
       for (int i = 0; i < kStages; ++i) {
         mbar_init(b_kfull + 8 * i, 1);
-        mbar_init(b_kempty + 8 * i, 1);
+        mbar_init(b_kempty + 8 * i, 2);
         mbar_init(b_vfull + 8 * i, 1);
         mbar_init(b_vempty + 8 * i, 4);
       }
@@ -149,8 +150,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   static_assert(2 * kRegsOther + 2 * kRegsSoftmax <= 4 * kRegsLaunch && kRegsLaunch * kThreads <= 65536, "within what the block was launched with");
   if (warp < 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsOther));
-    if (pages == 0 || warp == 3) {
-      // no rows: a number of the ragged numbering that nobody has
+    if (pages == 0 || (warp == 2 && tiles == 1)) {
+      // no rows: a number of the ragged numbering that nobody has; or none in the second tile
     } else if (warp == 0) {
     // ------------------------------------------------------------------------------------------ copies
     const int rows_k = p.c.pages * p.c.heads * kPage, rows_v = p.c.pages * p.c.heads * DIM;
@@ -202,7 +203,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
       }
     }
-    } else if (warp < 3) {
+    } else if (warp < 4) {
     // ------------------------------------------------------------------------------------------ products
     constexpr uint32_t idesc_s = make_idesc_e4m3_f32(128, kHalf);
     constexpr uint32_t idesc_o = make_idesc_e4m3_f32(128, DIM);  // the same fields: format 0 is f16 in kind::f16
@@ -216,34 +217,35 @@ __global__ void __launch_bounds__(kThreads, 1)
         site = where;
       }
     };
-    if (warp == 1) {
-      // scores of half page h of tile w, into buffer h & 1: behind the product that read P from there
+    if (warp < 3) {
+      // scores of half page h of this warp's tile, into buffer h & 1: behind the product that read P from there
+      const int w = __shfl_sync(0xffffffffu, warp, 0) - 1;
       int stage = 0;
       uint32_t round = 0;
-      need(b_qready, 0, 1);
-      if (active == 2) need(b_qready + 8, 0, 1);
+      need(b_qready + 8 * w, 0, 1);
 #pragma unroll 1
       for (int h = 0; h < halves && ok; ++h) {
         const int buf = h & 1;
         if (buf == 0) need(b_kfull + 8 * stage, round, 2);
-#pragma unroll 1
-        for (int w = 0; w < active; ++w) {
-          if (h >= 2) need(b_pvdone + 16 * w + 8 * buf, ((h >> 1) & 1) ^ 1, 3);
-          if (!ok) break;
-          tc_fence_after();
-          if (elect_one()) {
-            const uint64_t bd = rows_desc<DIM>(base + stage * 2 * Sh::kTile + buf * kHalf * DIM);
+        if (h >= 2) need(b_pvdone + 16 * w + 8 * buf, ((h >> 1) & 1) ^ 1, 3);
+        if (!ok) break;
+        tc_fence_after();
+        if (elect_one()) {
+          const uint64_t bd = rows_desc<DIM>(base + stage * 2 * Sh::kTile + buf * kHalf * DIM);
 #pragma unroll
-            for (int term = 0; term < kTerms; ++term) {
-              const uint64_t ad = rows_desc<DIM>(q_addr + w * Sh::kQ + term * 128 * DIM);
+          for (int term = 0; term < kTerms; ++term) {
+            const uint64_t ad = rows_desc<DIM>(q_addr + w * Sh::kQ + term * 128 * DIM);
 #pragma unroll
-              for (int k = 0; k < DIM / 32; ++k) mma_f8f6f4(tm + w * 128 + buf * kHalf, ad + 2 * k, bd + 2 * k, idesc_s, term + k > 0);
-            }
-            tc_commit(b_sfull + 16 * w + 8 * buf);
-            if (w == active - 1 && buf == 1) tc_commit(b_kempty + 8 * stage);
+            for (int k = 0; k < DIM / 32; ++k) mma_f8f6f4(tm + w * 128 + buf * kHalf, ad + 2 * k, bd + 2 * k, idesc_s, term + k > 0);
           }
-          __syncwarp();
+          tc_commit(b_sfull + 16 * w + 8 * buf);
+          if (buf == 1) {
+            // the stage is free when both tiles have read it
+            tc_commit(b_kempty + 8 * stage);
+            if (active == 1) tc_commit(b_kempty + 8 * stage);
+          }
         }
+        __syncwarp();
         if (buf == 1 && ++stage == kStages) {
           stage = 0;
           round ^= 1u;
@@ -275,7 +277,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     // ------------------------------------------------------------------------------------------ values to f16
     const int t = (warp - 4) * 32 + lane;
     bool nan = false;
-    for (int j = 0; j < pages; ++j) {
+    // the queries pass through this space first
+    for (int w = 0; w < tiles && ok; ++w) ok = warp_wait(b_qready + 8 * w, 0, abort_flag);
+    for (int j = 0; j < pages && ok; ++j) {
       const int stage = j % kStages;
       if (!warp_wait(b_vfull + 8 * stage, (j / kStages) & 1, abort_flag) || !warp_wait(b_hempty + 8 * (j & 1), ((j >> 1) & 1) ^ 1, abort_flag)) {
         ok = false;
@@ -329,49 +333,58 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int i = w * tile_tokens + row / p.group, g = row % p.group;  // token of the block, head of the group
     const bool live = row < tile_tokens * p.group && i < v.n;
     const int pos = v.pos0 + i;
-    float mul;
+    // ---- queries: eight elements per thread, split into e4m3 terms under a power-of-two scale of their row (a short loop:
+    // straight-line code that a block runs once is paid for in instruction fetches)
     {
-      const T* src = static_cast<const T*>(p.q) + static_cast<int64_t>(v.lo + i) * p.q_tok + (head * p.group + g) * p.q_head;
-      uint4 x[DIM / 8];
-      uint32_t top = 0;
+      constexpr int kLanes = DIM / 8, kRows = 128 / kLanes;
+      const int st = quarter * 32 + lane, e = (st % kLanes) * 8;
+      // all copies first, into the space of the f16 values, which waits for the queries: one latency, no registers
+      uint8_t* raw = v16_smem + w * Sh::kV16 + e * 2;
+      const T* q0 = static_cast<const T*>(p.q) + static_cast<int64_t>(v.lo + w * tile_tokens) * p.q_tok + head * p.group * p.q_head + e;
+#pragma unroll 4
+      for (int r = st / kLanes; r < 128; r += kRows) {
+        const int ti = r / p.group;
+        if (ti < tile_tokens && w * tile_tokens + ti < v.n)
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(raw + r * (2 * DIM))), "l"(q0 + ti * p.q_tok + (r - ti * p.group) * p.q_head) : "memory");
+        else
+          *reinterpret_cast<uint4*>(raw + r * (2 * DIM)) = make_uint4(0, 0, 0, 0);
+      }
+      asm volatile("cp.async.wait_all;" ::: "memory");
+#pragma unroll 2
+      for (int r = st / kLanes; r < 128; r += kRows) {
+        const uint4 x = *reinterpret_cast<const uint4*>(raw + r * (2 * DIM));  // this thread's own copy
+        const uint32_t ww[4] = {x.x, x.y, x.z, x.w};
+        float f[8];
+        uint32_t top = 0;
 #pragma unroll
-      for (int e = 0; e < DIM / 8; ++e) x[e] = live ? *reinterpret_cast<const uint4*>(src + e * 8) : make_uint4(0, 0, 0, 0);
-#pragma unroll
-      for (int e = 0; e < DIM / 8; ++e) {
-        const uint32_t ww[4] = {x[e].x, x[e].y, x[e].z, x[e].w};
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const float2 u = unpack_pair<T>(ww[k]);
+        for (int j = 0; j < 4; ++j) {
+          const float2 u = unpack_pair<T>(ww[j]);
+          f[2 * j] = u.x;
+          f[2 * j + 1] = u.y;
           top = max(top, max(__float_as_uint(u.x) & 0x7fffffffu, __float_as_uint(u.y) & 0x7fffffffu));
         }
-      }
-      const float sc = cache_scale(__uint_as_float(top)), inv = pow2_reciprocal(sc);
-      // a row that holds an infinity or NaN has no answer
-      mul = top >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : sc * p.scale * 1.4426950408889634f;
 #pragma unroll
-      for (int c = 0; c < DIM / 16; ++c) {
-        uint32_t out[kTerms][4];
+        for (int o = kLanes / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+        const float sc = cache_scale(__uint_as_float(top)), inv = pow2_reciprocal(sc);
+        uint32_t out[kTerms][2];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const uint32_t ww[4] = {x[2 * c + h].x, x[2 * c + h].y, x[2 * c + h].z, x[2 * c + h].w};
+        for (int j = 0; j < 4; ++j) {
+          uint32_t term[kTerms];
+          split_e4m3<kTerms>(f[2 * j] * inv, f[2 * j + 1] * inv, 1.f, term);
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const float2 u = unpack_pair<T>(ww[k]);
-            uint32_t term[kTerms];
-            split_e4m3<kTerms>(u.x * inv, u.y * inv, 1.f, term);
-#pragma unroll
-            for (int y = 0; y < kTerms; ++y) out[y][h * 2 + (k >> 1)] = (k & 1) ? out[y][h * 2 + (k >> 1)] | (term[y] << 16) : term[y];
-          }
+          for (int y = 0; y < kTerms; ++y) out[y][j >> 1] = (j & 1) ? out[y][j >> 1] | (term[y] << 16) : term[y];
         }
 #pragma unroll
         for (int y = 0; y < kTerms; ++y)
-          *reinterpret_cast<uint4*>(q_smem + w * Sh::kQ + y * 128 * DIM + swizzled<DIM>(row, c * 16)) =
-              make_uint4(out[y][0], out[y][1], out[y][2], out[y][3]);
+          *reinterpret_cast<uint2*>(q_smem + w * Sh::kQ + y * 128 * DIM + swizzled<DIM>(r, e)) = make_uint2(out[y][0], out[y][1]);
+        // a row that holds an infinity or NaN has no answer
+        if (e == 0) rowmul[w * 128 + r] = top >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : sc * p.scale * 1.4426950408889634f;
       }
       fence_proxy_async_smem();
-      __syncwarp();
+      asm volatile("barrier.cta.sync %0, 128;" ::"r"(1 + w) : "memory");  // the tile's four warps, none of which can fail here
       if (lane == 0) mbar_arrive(b_qready + 8 * w);
     }
+    const float mul = rowmul[w * 128 + row];
     // what all rows of the tile see
     const int tile_first = v.pos0 + w * tile_tokens, tile_last = v.pos0 + min(v.n, (w + 1) * tile_tokens) - 1;
     const int all_hi = min(v.len, tile_first + 1);
@@ -517,15 +530,16 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       const float inv = l == 0.f ? 0.f : 1.0f / l;
       T* out = static_cast<T*>(p.o) + static_cast<int64_t>(v.lo + i) * p.o_tok + (head * p.group + g) * p.o_head;
-#pragma unroll
+#pragma unroll 1
       for (int c = 0; c < DIM; c += 32) {
         uint32_t o[32];
         tmem_ld_32x32(t_o + c, o);
         tmem_ld_wait();
-        if (bad[c >> 5] != 0) {
+        const uint32_t nan = c < 64 ? (c < 32 ? bad[0] : bad[1]) : (c < 96 ? bad[2] : bad[3]);
+        if (nan != 0) {
 #pragma unroll
           for (int k = 0; k < 32; ++k)
-            if ((bad[c >> 5] >> k) & 1u) o[k] = 0x7fc00000u;
+            if ((nan >> k) & 1u) o[k] = 0x7fc00000u;
         }
         if (live) {
 #pragma unroll
