@@ -17,7 +17,9 @@
 // Work: the pages that the units (sequence, cache head) see are numbered through, and every block takes an equal range of
 // them, wherever that begins and ends: no batch is too ragged.  A block that ends inside a unit leaves a partial result and
 // a record; the joining kernel adds the parts of such a unit in block order, so results do not depend on timing.
-// Warp 0 copies pages (TMA, a ring of page pairs), warp 1 issues the products, warps 2-5 do the softmax.
+// Warp 0 copies pages (TMA, a ring of page pairs), warp 1 issues the products, warps 2-5 do the softmax.  Where the shared
+// memory holds one block per SM only, four more warps share it: the two groups take pages in turn, each with references,
+// sums and an O^T of its own, which are joined when the unit ends (the softmax of 32 rows takes longer than copying the page).
 #include <cstdio>
 
 #include "tg_attention.cuh"
@@ -25,7 +27,6 @@
 namespace tg {
 namespace {
 
-constexpr int kThreads = 192;
 constexpr float kNominal = 3.f, kLimit = 8.f;  // p is kept times 2^3 and may reach 2^8 (e4m3 ends at 448) before ref moves
 constexpr float kUnset = -1e30f;  // the reference of a row that has not seen a token yet
 
@@ -39,12 +40,16 @@ struct Shape {
   static constexpr int kQ = TERMS * N * DIM;
   // two blocks share an SM where each still has a ring of three page pairs
   static constexpr int kBlocksPerSm = N == 16 && !(TERMS == 3 && DIM == 128) ? 2 : 1;
-  static constexpr int kMisc = 4096;
+  static constexpr int kGroups = kBlocksPerSm == 2 ? 1 : 2;  // of four softmax warps
+  static constexpr int kThreads = 64 + 128 * kGroups;
+  // barriers and notes; row factors; references; maxima and sums; rows that see a NaN
+  static constexpr int kRowmul = 1024, kRef = kRowmul + N * 4, kWmax = kRef + kGroups * 2 * N * 4, kNan = kWmax + kGroups * 2 * 4 * N * 4;
+  static constexpr int kMisc = kNan + (kGroups == 2 ? 2 * 128 * 8 : 0);
   // dim 64: the value operand is read as 128 rows, 64 of them whatever follows the page
   static constexpr int kBudget = (kBlocksPerSm == 2 ? 113 : 226) * 1024 - 1024 - 2 * kP - kQ - kMisc;
   static constexpr int kStages = kBudget / (2 * kTile) > 8 ? 8 : kBudget / (2 * kTile);
   static constexpr int kSmem = 1024 + kStages * 2 * kTile + 2 * kP + kQ + kMisc;
-  static constexpr int kTmemUsed = 2 * N + TERMS * N;  // S^T twice and the terms' O^T
+  static constexpr int kTmemUsed = 2 * N + kGroups * TERMS * N;  // S^T twice and each group's O^T by term
   static constexpr int kTmem = kTmemUsed <= 64 ? 64 : kTmemUsed <= 128 ? 128 : kTmemUsed <= 256 ? 256 : 512;
   static_assert(kStages >= 3, "the ring is too short to hide the latency of a page");
   static_assert(2 * kP + kQ >= 8192, "the value operand of dim 64 reads 8 KB behind its page");
@@ -67,18 +72,19 @@ __device__ __forceinline__ void load8(const float* src, float (&v)[8]) {
   v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
 }
 
-// The four softmax warps meet; true if any thread says so.  Nobody waits alone here: whatever a warp found, it comes.
-__device__ __forceinline__ bool softmax_vote(bool mine) {
+// Softmax warps meet at a hardware barrier (`count` threads); true if any thread says so.  Nobody waits alone here: whatever a
+// warp found, it comes.
+__device__ __forceinline__ bool softmax_vote(uint32_t barrier, uint32_t count, bool mine) {
   uint32_t any;
   asm volatile(
       "{\n\t"
       ".reg .pred p, q;\n\t"
       "setp.ne.u32 p, %1, 0;\n\t"
-      "barrier.cta.red.or.pred q, 1, 128, p;\n\t"
+      "barrier.cta.red.or.pred q, %2, %3, p;\n\t"
       "selp.u32 %0, 1, 0, q;\n\t"
       "}"
       : "=r"(any)
-      : "r"(static_cast<uint32_t>(mine))
+      : "r"(static_cast<uint32_t>(mine)), "r"(barrier), "r"(count)
       : "memory");
   return any != 0;
 }
@@ -147,11 +153,11 @@ __device__ __noinline__ void clean_values(const AttentionParams& p, const SeqVie
 }
 
 template <typename T, int DIM, int N>
-__global__ void __launch_bounds__(kThreads, (Shape<DIM, N, kTermsOf<T>>::kBlocksPerSm))
+__global__ void __launch_bounds__((Shape<DIM, N, kTermsOf<T>>::kThreads), (Shape<DIM, N, kTermsOf<T>>::kBlocksPerSm))
     tg_attention_few_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const __grid_constant__ AttentionParams p) {
   constexpr int kTerms = kTermsOf<T>;
   using Sh = Shape<DIM, N, kTerms>;
-  constexpr int kStages = Sh::kStages;
+  constexpr int kStages = Sh::kStages, kGroups = Sh::kGroups, kThreads = Sh::kThreads;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* p_smem = smem + kStages * 2 * Sh::kTile;
@@ -163,9 +169,7 @@ __global__ void __launch_bounds__(kThreads, (Shape<DIM, N, kTermsOf<T>>::kBlocks
   volatile uint32_t* abort_flag = reinterpret_cast<volatile uint32_t*>(misc + 512 + 8 * sizeof(TileInfo));
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(misc + 512 + 8 * sizeof(TileInfo) + 16);
   int64_t* sched = reinterpret_cast<int64_t*>(misc + 512 + 8 * sizeof(TileInfo) + 32);  // 0 tiles in front, 1 sequence, 2.. warp sums
-  float* rowmul = reinterpret_cast<float*>(misc + 1024);
-  float* ref = reinterpret_cast<float*>(misc + 1280);        // [2][N]
-  float* wmax = reinterpret_cast<float*>(misc + 2048);       // [2][4][N]: the four warps' maxima, or sums, by row
+  float* rowmul = reinterpret_cast<float*>(misc + Sh::kRowmul);
 
   const uint32_t bar0 = smem_u32(bars);
   const uint32_t b_full = bar0, b_empty = bar0 + 8 * kStages, b_sfull = b_empty + 8 * kStages, b_sempty = b_sfull + 16,
@@ -188,7 +192,7 @@ __global__ void __launch_bounds__(kThreads, (Shape<DIM, N, kTermsOf<T>>::kBlocks
         mbar_init(b_pready + 8 * i, 4);
         mbar_init(b_pvdone + 8 * i, 1);
       }
-      mbar_init(b_qready, 4);
+      mbar_init(b_qready, 4 * kGroups);
       init_abort_flag(abort_flag, p.wait_limit_us);
       fence_mbar_init();
     }
@@ -252,7 +256,6 @@ __global__ void __launch_bounds__(kThreads, (Shape<DIM, N, kTermsOf<T>>::kBlocks
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  const uint32_t t_o = tmem + 2 * N;
 
   Cursor cur;
   cur.b = static_cast<int>(sched[1]);
@@ -338,7 +341,8 @@ __global__ void __launch_bounds__(kThreads, (Shape<DIM, N, kTermsOf<T>>::kBlocks
         const uint64_t a = make_kmajor_sw128_desc(smem_u32(smem + stage * 2 * Sh::kTile + Sh::kTile));
         const uint64_t b = make_kmajor_sw128_desc(p_addr + buf * Sh::kP);
 #pragma unroll
-        for (int k = 0; k < kPage / 32; ++k) mma_f8f6f4(t_o, a + 2 * k, b + 2 * k, idesc_pv, !(first && k == 0));
+        for (int k = 0; k < kPage / 32; ++k)
+          mma_f8f6f4(tmem + 2 * N + (kGroups == 2 ? buf * kTerms * N : 0), a + 2 * k, b + 2 * k, idesc_pv, !(first && k == 0));
         tc_commit(b_empty + 8 * stage);
         tc_commit(b_pvdone + 8 * buf);
       }
@@ -374,14 +378,14 @@ __global__ void __launch_bounds__(kThreads, (Shape<DIM, N, kTermsOf<T>>::kBlocks
           tc_commit(b_sfull + 8 * buf);
         }
         __syncwarp();
-        if (t > t0 && !issue_pv(it - 1, t - 1 == t0)) {
+        if (t > t0 && !issue_pv(it - 1, t - 1 < t0 + kGroups)) {
           ok = false;
           site = 3;
           break;
         }
       }
       // the unit's last product does not wait for the next unit's queries
-      if (ok && !issue_pv(it - 1, t1 - 1 == t0)) {
+      if (ok && !issue_pv(it - 1, t1 - 1 < t0 + kGroups)) {
         ok = false;
         site = 4;
       }
@@ -391,9 +395,20 @@ __global__ void __launch_bounds__(kThreads, (Shape<DIM, N, kTermsOf<T>>::kBlocks
     if (!ok && lane == 0) *p.status = kRoleMma * 1000 + site;
   } else {
     // ------------------------------------------------------------------------------------------ softmax
-    // A wait that gives up is remembered, not acted on: the four warps leave together at their next vote.
-    const int quarter = warp & 3, token = quarter * 32 + lane, st = (warp - 2) * 32 + lane;
+    // A wait that gives up is remembered, not acted on: the warps leave together at their next vote, a group's own (which
+    // ends its pages) or the one of all.
+    const int quarter = warp & 3, token = quarter * 32 + lane, at = (warp - 2) * 32 + lane, group = kGroups == 2 ? at >> 7 : 0;
+    const int st = at & 127;
     const uint32_t lane_off = static_cast<uint32_t>(quarter * 32) << 16;
+    const uint32_t t_all = tmem + 2 * N + lane_off, t_o = t_all + group * kTerms * N;
+    float* refs = reinterpret_cast<float*>(misc + Sh::kRef);          // [group][copy][N]
+    float* ref = refs + group * 2 * N;
+    float* maxima = reinterpret_cast<float*>(misc + Sh::kWmax);       // [group][copy][4][N]: the warps' maxima, or sums, by row
+    float* wmax = maxima + group * 8 * N;
+    int2* side_notes = reinterpret_cast<int2*>(misc + 960);           // [group]: which copies hold its sums and references
+    uint64_t* nan_notes = reinterpret_cast<uint64_t*>(misc + Sh::kNan);  // [group][element of the head]
+    auto vote = [&](bool mine) { return softmax_vote(1 + group, 128, mine); };
+    auto vote_all = [&](bool mine) { return softmax_vote(kGroups == 2 ? 3 : 1, 128 * kGroups, mine); };
     int it = 0, turn = 0;
     int64_t tile_at = begin;
     float l[N];
@@ -411,21 +426,21 @@ __global__ void __launch_bounds__(kThreads, (Shape<DIM, N, kTermsOf<T>>::kBlocks
       const int rows = v.n * p.group;
       // ---- queries: eight elements per thread, split into e4m3 terms under a power-of-two scale of their row
       {
-        constexpr int kLanes = DIM / 8, kRows = 128 / kLanes, kPasses = N / kRows, kBatch = kPasses < 4 ? kPasses : 4;
-        const int e = (st % kLanes) * 8;
+        constexpr int kLanes = DIM / 8, kRows = 128 * kGroups / kLanes, kPasses = (N + kRows - 1) / kRows, kBatch = kPasses < 4 ? kPasses : 4;
+        const int e = (at % kLanes) * 8;
 #pragma unroll 1
         for (int r0 = 0; r0 < rows; r0 += kRows * kBatch) {
           uint4 w[kBatch];
 #pragma unroll
           for (int k = 0; k < kBatch; ++k) {
-            const int r = r0 + k * kRows + st / kLanes, i = r / p.group;
+            const int r = r0 + k * kRows + at / kLanes, i = r / p.group;
             w[k] = make_uint4(0, 0, 0, 0);
             if (r < rows)
               w[k] = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.q) + (v.lo + i) * p.q_tok + (cur.h * p.group + r - i * p.group) * p.q_head + e);
           }
 #pragma unroll
           for (int k = 0; k < kBatch; ++k) {
-            const int r = r0 + k * kRows + st / kLanes;
+            const int r = r0 + k * kRows + at / kLanes;
             const uint32_t ww[4] = {w[k].x, w[k].y, w[k].z, w[k].w};
             float f[8];
             uint32_t top = 0;
@@ -462,7 +477,7 @@ __global__ void __launch_bounds__(kThreads, (Shape<DIM, N, kTermsOf<T>>::kBlocks
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(b_qready);
-        if (softmax_vote(!ok)) break;
+        if (vote_all(!ok)) break;
       }
 #pragma unroll
       for (int r = 0; r < N; ++r) l[r] = 0.f;
@@ -470,9 +485,10 @@ __global__ void __launch_bounds__(kThreads, (Shape<DIM, N, kTermsOf<T>>::kBlocks
       // positions that every row sees: [all_lo, all_hi), and the first tokens
       const int all_hi = min(v.len, v.pos0 + 1);
       const int all_lo = p.window > 0 ? static_cast<int>(max(static_cast<int64_t>(v.pos0) + v.n - p.window, int64_t(0))) : 0;
-      bool gave_up = false;
+      int mine = 0;  // pages of this unit that this group has done
       for (int t = t0; t < t1; ++t, ++it) {
         const int stage = it % kStages, buf = it & 1;
+        if (kGroups == 2 && buf != group) continue;
         wait(b_full + 8 * stage, (it / kStages) & 1, 1);
         const TileInfo ti = info[stage];
         const bool whole = ti.base >= 0 && ti.base + kPage <= all_hi && (ti.base >= all_lo || ti.base + kPage <= p.sinks);
@@ -512,7 +528,7 @@ __global__ void __launch_bounds__(kThreads, (Shape<DIM, N, kTermsOf<T>>::kBlocks
               if (r < see_lo || r >= see_hi) z[r] = -INFINITY;
           }
         };
-        bool move = t == t0;
+        bool move = mine == 0;
         if (!move) {
           exponents(true);
           float over = -INFINITY;
@@ -521,7 +537,7 @@ __global__ void __launch_bounds__(kThreads, (Shape<DIM, N, kTermsOf<T>>::kBlocks
             if (g >= rows) break;
             over = fmaxf(over, fmaxf(fmaxf(fmaxf(z[g], z[g + 1]), fmaxf(z[g + 2], z[g + 3])), fmaxf(fmaxf(z[g + 4], z[g + 5]), fmaxf(z[g + 6], z[g + 7]))));
           }
-          move = softmax_vote(over > kLimit || !ok);
+          move = vote(over > kLimit || !ok);
         }
         if (move) {
           // ---- some row's exponent has outgrown its reference (or has none yet): every row's maximum, and a new reference
@@ -540,9 +556,10 @@ __global__ void __launch_bounds__(kThreads, (Shape<DIM, N, kTermsOf<T>>::kBlocks
               *reinterpret_cast<float4*>(wm + quarter * N + g + 4) = make_float4(m[4], m[5], m[6], m[7]);
             }
           }
-          if (t > t0) wait(b_pvdone + 8 * ((it - 1) & 1), ((it - 1) >> 1) & 1, 3);
-          if (softmax_vote(!ok)) {
-            gave_up = true;
+          const int last = it - kGroups;  // this group's page before
+          if (mine > 0) wait(b_pvdone + 8 * (last & 1), (last >> 1) & 1, 3);
+          if (vote(!ok)) {
+            ok = false;
             break;
           }
           tc_fence_after();
@@ -577,25 +594,26 @@ __global__ void __launch_bounds__(kThreads, (Shape<DIM, N, kTermsOf<T>>::kBlocks
               *reinterpret_cast<float4*>(now + g) = make_float4(top[0], top[1], top[2], top[3]);
               *reinterpret_cast<float4*>(now + g + 4) = make_float4(top[4], top[5], top[6], top[7]);
             }
-            if (t > t0 && any) {
+            if (mine > 0 && any) {
 #pragma unroll
               for (int x = 0; x < kTerms; ++x) {
                 uint32_t o[8];
-                tmem_ld_32x8(t_o + lane_off + x * N + g, o);
+                tmem_ld_32x8(t_o + x * N + g, o);
                 tmem_ld_wait();
 #pragma unroll
                 for (int j = 0; j < 8; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * f[j]);
-                tmem_st_32x8(t_o + lane_off + x * N + g, o);
+                tmem_st_32x8(t_o + x * N + g, o);
               }
             }
           }
-          if (t > t0) tmem_st_wait();
-          side ^= 1;  // read again behind the next vote, or this one's below
-          if (softmax_vote(!ok)) {
-            gave_up = true;
+          if (mine > 0) tmem_st_wait();
+          side ^= 1;
+          if (vote(!ok)) {
+            ok = false;
             break;
           }
         }
+        ++mine;
         // ---- P.  Its buffer is free: S^T of this page was issued behind the product before the last, which read it, and the
         // barrier that announced S^T counts every product issued before.
         const uint32_t pb = smem_u32(p_smem) + buf * Sh::kP + token;
@@ -627,8 +645,9 @@ __global__ void __launch_bounds__(kThreads, (Shape<DIM, N, kTermsOf<T>>::kBlocks
           mbar_arrive(b_pready + 8 * buf);
         }
       }
-      if (gave_up) break;
       // ---- the unit's (or this block's part of its) result: thread = element of the head
+      // the groups' copies: the other one has to know where to look
+      if (kGroups == 2 && st == 0) side_notes[group] = make_int2(turn & 1, side);
       float* sums = wmax + (turn & 1) * 4 * N;
       ++turn;
 #pragma unroll
@@ -654,34 +673,66 @@ __global__ void __launch_bounds__(kThreads, (Shape<DIM, N, kTermsOf<T>>::kBlocks
         c += __shfl_xor_sync(0xffffffffu, c, 16);
         if (lane < 8) sums[quarter * N + g + lane] = c;
       }
-      wait(b_pvdone + 8 * ((it - 1) & 1), ((it - 1) >> 1) & 1, 4);
-      if (softmax_vote(!ok)) break;
+      if (mine > 0) {
+        const int last = kGroups == 2 && ((it - 1) & 1) != group ? it - 2 : it - 1;
+        wait(b_pvdone + 8 * (last & 1), (last >> 1) & 1, 4);
+      }
+      if (kGroups == 2) nan_notes[group * 128 + token] = nan_rows;
+      if (vote_all(!ok)) break;
       tc_fence_after();
+      // a group that had no page of the unit (it was cut to one) has sums of zero, references unset and no O^T
+      bool has[kGroups];
+      int2 copy[kGroups];
+#pragma unroll
+      for (int x = 0; x < kGroups; ++x) copy[x] = kGroups == 2 ? side_notes[x] : make_int2((turn - 1) & 1, side);
+#pragma unroll
+      for (int x = 0; x < kGroups; ++x) has[x] = kGroups == 1 || t1 - t0 >= 2 || ((it - 1) & 1) == x;
+      if (kGroups == 2) nan_rows |= nan_notes[(group ^ 1) * 128 + token];
       const bool whole_unit = t0 == 0 && t1 == v.tiles;
       const int64_t slot = 2 * static_cast<int64_t>(blockIdx.x) + (t0 > 0 ? 0 : 1);
-      T* out = static_cast<T*>(p.o) + v.lo * p.o_tok + static_cast<int64_t>(cur.h) * p.group * p.o_head + token;
-      int in_group = 0;
 #pragma unroll
       for (int g = 0; g < N; g += 8) {
         if (g >= rows) break;
-        float o[8], sum[8];
-        uint32_t part[kTerms][8];
+        if (kGroups == 2 && ((g >> 3) & 1) != group) continue;  // the groups share the rows
+        float o[8], sum[8], base[8];
 #pragma unroll
-        for (int x = 0; x < kTerms; ++x) tmem_ld_32x8(t_o + lane_off + x * N + g, part[x]);
-        load8(sums + g, sum);
+        for (int x = 0; x < kGroups; ++x) {
+          uint32_t part[kTerms][8];
 #pragma unroll
-        for (int q = 1; q < 4; ++q) {
-          float w[8];
-          load8(sums + q * N + g, w);
+          for (int y = 0; y < kTerms; ++y) tmem_ld_32x8(t_all + (x * kTerms + y) * N + g, part[y]);
+          float lx[8], rx[8];
+          const float* sx = maxima + x * 8 * N + copy[x].x * 4 * N + g;
+          load8(sx, lx);
 #pragma unroll
-          for (int j = 0; j < 8; ++j) sum[j] += w[j];
-        }
-        tmem_ld_wait();
+          for (int q = 1; q < 4; ++q) {
+            float w[8];
+            load8(sx + q * N, w);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          o[j] = __uint_as_float(part[kTerms - 1][j]);
+            for (int j = 0; j < 8; ++j) lx[j] += w[j];
+          }
+          load8(refs + x * 2 * N + copy[x].y * N + g, rx);
+          tmem_ld_wait();
 #pragma unroll
-          for (int x = kTerms - 2; x >= 0; --x) o[j] = fmaf(o[j], 1.f / kTermStep, __uint_as_float(part[x][j]));
+          for (int j = 0; j < 8; ++j) {
+            float ox = __uint_as_float(part[kTerms - 1][j]);
+#pragma unroll
+            for (int y = kTerms - 2; y >= 0; --y) ox = fmaf(ox, 1.f / kTermStep, __uint_as_float(part[y][j]));
+            if (!has[x]) {
+              ox = 0.f;
+              lx[j] = 0.f;
+              rx[j] = kUnset;
+            }
+            if (x == 0) {
+              o[j] = ox;
+              sum[j] = lx[j];
+              base[j] = rx[j];
+            } else {
+              const float m = fmaxf(base[j], rx[j]), f0 = exp2_approx(base[j] - m), f1 = exp2_approx(rx[j] - m);
+              o[j] = fmaf(o[j], f0, ox * f1);
+              sum[j] = fmaf(sum[j], f0, lx[j] * f1);
+              base[j] = m;
+            }
+          }
         }
         if (nan_rows != 0) {
 #pragma unroll
@@ -692,6 +743,8 @@ __global__ void __launch_bounds__(kThreads, (Shape<DIM, N, kTermsOf<T>>::kBlocks
           T res[8];
 #pragma unroll
           for (int j = 0; j < 8; ++j) res[j] = static_cast<T>(sum[j] == 0.f ? 0.f : __fdividef(o[j], sum[j]));
+          int i = g / p.group, in_group = g - i * p.group;
+          T* out = static_cast<T*>(p.o) + (v.lo + i) * p.o_tok + (static_cast<int64_t>(cur.h) * p.group + in_group) * p.o_head + token;
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
             if (g + j < rows && token < DIM) *out = res[j];
@@ -708,12 +761,12 @@ __global__ void __launch_bounds__(kThreads, (Shape<DIM, N, kTermsOf<T>>::kBlocks
           }
           if (token == 0) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) p.part_ml[slot * N + g + j] = make_float2(ref[side * N + g + j], sum[j]);
+            for (int j = 0; j < 8; ++j) p.part_ml[slot * N + g + j] = make_float2(base[j], sum[j]);
           }
         }
       }
       tc_fence_before();
-      if (left == 0 && st == 0) {
+      if (left == 0 && at == 0) {
         // does the unit go on behind this block, and did it begin here?
         int4 rec = make_int4(-1, 0, 0, 0);
         if (t0 == 0 && t1 < v.tiles) {
@@ -727,7 +780,7 @@ __global__ void __launch_bounds__(kThreads, (Shape<DIM, N, kTermsOf<T>>::kBlocks
       if (left > 0 && !next_unit(p, cur)) break;
     }
     if (!ok && lane == 0) *p.status = kRoleEpilogue * 1000 + site;
-    if (abort_flag[0] && st == 0) p.record[blockIdx.x] = make_int4(-1, 0, 0, 0);
+    if (abort_flag[0] && at == 0) p.record[blockIdx.x] = make_int4(-1, 0, 0, 0);
   }
   tc_fence_before();
   __syncthreads();
@@ -779,7 +832,7 @@ cudaError_t launch_n(const CUtensorMap& tmK, const CUtensorMap& tmV, const Atten
     if (e != cudaSuccess) return e;
     set[dev & 63] = true;
   }
-  e = launch_pdl(kernel, dim3(blocks), dim3(kThreads), Sh::kSmem, stream, tmK, tmV, p);
+  e = launch_pdl(kernel, dim3(blocks), dim3(Sh::kThreads), Sh::kSmem, stream, tmK, tmV, p);
   if (e != cudaSuccess) return e;
   return launch_pdl(tg_attention_join_kernel<T, DIM>, dim3(blocks, (p.max_q_len * p.group + 3) / 4), dim3(4 * DIM), 0, stream, p, N);
 }
