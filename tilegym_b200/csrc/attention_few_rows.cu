@@ -8,16 +8,18 @@
 //   O^T [dim, R]        += V^T [dim, 128] . P           p = p1 + p2 (+ p3) in e4m3, the same way
 //
 // The two factors that are not in the cache are split into e4m3 terms, each holding what the one before left: two hold a
-// bf16 q exactly and p to 2^-8, three (f16) both to 2^-12.  The terms of q are summed by the accumulator; those of p are
-// kept 16 times larger each (which moves the end of e4m3's range out of reach) and have columns of their own in O^T, joined
-// at the end.  `ref` is a running maximum of the exponent that is only moved when a p would leave the format (2^5 of
+// bf16 q exactly and p to 2^-8, three (f16) both to 2^-12.  The terms are kept 16 times larger each (which moves the end of
+// e4m3's range out of reach) and stand side by side as rows of the operand, so a page is read once for all of them; their
+// columns of S^T and O^T are joined by the softmax and at the end.  (With 64 rows TMEM has no room for that: there the
+// accumulator sums q's terms, unscaled.)  `ref` is a running maximum of the exponent that is only moved when a p would leave the format (2^5 of
 // headroom), which rescales O^T in TMEM.  Keeping v_scale in the exponent keeps p at one magnitude whatever the pages'
 // scales are.
 //
-// Work: the pages that the units (sequence, cache head) see are numbered through, and every block takes an equal range of
-// them, wherever that begins and ends: no batch is too ragged.  A block that ends inside a unit leaves a partial result and
+// Work: the pages that the units (sequence, cache head) see are numbered through, each unit kUnitCost numbers in front of
+// them for what it costs to begin and end one, and every block takes an equal range of the numbers, wherever that begins
+// and ends: no batch is too ragged.  A block that ends inside a unit leaves a partial result and
 // a record; the joining kernel adds the parts of such a unit in block order, so results do not depend on timing.
-// Warp 0 copies pages (TMA, a ring of page pairs), warp 1 issues the products, warps 2-5 do the softmax.  Where the shared
+// Warp 0 copies pages (TMA, a ring of page pairs), warps 1 and 2 issue the two products, warps 3-6 do the softmax.  Where the shared
 // memory holds one block per SM only, four more warps share it: the two groups take pages in turn, each with references,
 // sums and an O^T of its own, which are joined when the unit ends (the softmax of 32 rows takes longer than copying the page).
 #include <cstdio>
@@ -41,7 +43,10 @@ struct Shape {
   // two blocks share an SM where each still has a ring of three page pairs
   static constexpr int kBlocksPerSm = N == 16 && !(TERMS == 3 && DIM == 128) ? 2 : 1;
   static constexpr int kGroups = kBlocksPerSm == 2 ? 1 : 2;  // of four softmax warps
-  static constexpr int kThreads = 64 + 128 * kGroups;
+  static constexpr int kThreads = 96 + 128 * kGroups;
+  // A unit's queries, first references and result take about 8000 clocks; a page 2000 (one group, two blocks to share the
+  // SM) or 1100.
+  static constexpr int kUnitCost = kGroups == 1 ? 4 : 6;
   // barriers and notes; row factors; references; maxima and sums; rows that see a NaN
   static constexpr int kRowmul = 1024, kRef = kRowmul + N * 4, kWmax = kRef + kGroups * 2 * N * 4, kNan = kWmax + kGroups * 2 * 4 * N * 4;
   static constexpr int kMisc = kNan + (kGroups == 2 ? 2 * 128 * 8 : 0);
@@ -49,7 +54,9 @@ struct Shape {
   static constexpr int kBudget = (kBlocksPerSm == 2 ? 113 : 226) * 1024 - 1024 - 2 * kP - kQ - kMisc;
   static constexpr int kStages = kBudget / (2 * kTile) > 8 ? 8 : kBudget / (2 * kTile);
   static constexpr int kSmem = 1024 + kStages * 2 * kTile + 2 * kP + kQ + kMisc;
-  static constexpr int kTmemUsed = 2 * N + kGroups * TERMS * N;  // S^T twice and each group's O^T by term
+  static constexpr bool kStack = N <= 32;  // q's terms have columns of their own in S^T
+  static constexpr int kSCols = kStack ? TERMS * N : N;
+  static constexpr int kTmemUsed = 2 * kSCols + kGroups * TERMS * N;  // S^T twice and each group's O^T by term
   static constexpr int kTmem = kTmemUsed <= 64 ? 64 : kTmemUsed <= 128 ? 128 : kTmemUsed <= 256 ? 256 : 512;
   static_assert(kStages >= 3, "the ring is too short to hide the latency of a page");
   static_assert(2 * kP + kQ >= 8192, "the value operand of dim 64 reads 8 KB behind its page");
@@ -205,10 +212,11 @@ __global__ void __launch_bounds__((Shape<DIM, N, kTermsOf<T>>::kThreads), (Shape
 
   // ---- this block's range of pages
   int64_t total, begin = 0, end = 0, blocks;
+  auto numbers = [](const SeqView& v) { return v.tiles > 0 ? v.tiles + Sh::kUnitCost : 0; };
   {
-    const int mine = static_cast<int>(threadIdx.x) < p.c.seqs ? view_sequence(p, threadIdx.x, 0, p.max_q_len).tiles : 0;
+    const int mine = static_cast<int>(threadIdx.x) < p.c.seqs ? numbers(view_sequence(p, threadIdx.x, 0, p.max_q_len)) : 0;
     int64_t sum = mine;
-    for (int b = threadIdx.x + kThreads; b < p.c.seqs; b += kThreads) sum += view_sequence(p, b, 0, p.max_q_len).tiles;
+    for (int b = threadIdx.x + kThreads; b < p.c.seqs; b += kThreads) sum += numbers(view_sequence(p, b, 0, p.max_q_len));
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     if (lane == 0) sched[2 + warp] = sum;
@@ -228,7 +236,7 @@ __global__ void __launch_bounds__((Shape<DIM, N, kTermsOf<T>>::kThreads), (Shape
     int64_t before = 0;
     for (int base = 0; base < p.c.seqs && begin < end; base += kThreads) {
       const int b = base + threadIdx.x;
-      const int n = base == 0 ? mine : b < p.c.seqs ? view_sequence(p, b, 0, p.max_q_len).tiles : 0;
+      const int n = base == 0 ? mine : b < p.c.seqs ? numbers(view_sequence(p, b, 0, p.max_q_len)) : 0;
       int64_t incl = n;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -259,17 +267,27 @@ __global__ void __launch_bounds__((Shape<DIM, N, kTermsOf<T>>::kThreads), (Shape
 
   Cursor cur;
   cur.b = static_cast<int>(sched[1]);
-  int t0 = 0;
+  int from = 0;  // number within the unit at which this block's part begins
   const bool work = begin < end && cur.b >= 0;
   if (work) {
     cur.v = view_sequence(p, cur.b, 0, p.max_q_len);
     const int64_t rem = begin - sched[0] * p.c.heads;
-    cur.h = static_cast<int>(rem / cur.v.tiles);
-    t0 = static_cast<int>(rem - static_cast<int64_t>(cur.h) * cur.v.tiles);
+    cur.h = static_cast<int>(rem / numbers(cur.v));
+    from = static_cast<int>(rem - static_cast<int64_t>(cur.h) * numbers(cur.v));
   } else if (threadIdx.x == 0) {
     p.record[blockIdx.x] = make_int4(-1, 0, 0, 0);
   }
+  // this block's pages [t0, t1) of the current unit; false: the range ended in front of the unit's first page
+  int t0 = 0, t1 = 0;
   int64_t left = work ? end - begin : 0;
+  auto take = [&]() {
+    const int to = static_cast<int>(min(static_cast<int64_t>(numbers(cur.v)), from + left));
+    left -= to - from;
+    t0 = max(from - Sh::kUnitCost, 0);
+    t1 = max(to - Sh::kUnitCost, 0);
+    from = 0;
+    return t1 > t0;
+  };
   bool ok = true;
   int site = 0;
 
@@ -279,8 +297,7 @@ __global__ void __launch_bounds__((Shape<DIM, N, kTermsOf<T>>::kThreads), (Shape
     const int rows_k = p.c.pages * p.c.heads * kPage, rows_v = p.c.pages * p.c.heads * DIM;
     int it = 0;
     while (left > 0 && ok) {
-      const int t1 = static_cast<int>(min(static_cast<int64_t>(cur.v.tiles), t0 + left));
-      left -= t1 - t0;
+      if (!take()) break;
       for (int base = t0; base < t1 && ok; base += 32) {
         // 32 pages at a time: numbers first, so that copies start before the scales are here
         const int t = base + lane;
@@ -318,7 +335,6 @@ __global__ void __launch_bounds__((Shape<DIM, N, kTermsOf<T>>::kThreads), (Shape
           __syncwarp();
         }
       }
-      t0 = 0;
       if (left > 0 && !next_unit(p, cur)) break;
     }
     if (!ok) {
@@ -329,29 +345,12 @@ __global__ void __launch_bounds__((Shape<DIM, N, kTermsOf<T>>::kThreads), (Shape
         }
     }
   } else if (warp == 1) {
-    // ------------------------------------------------------------------------------------------ products
-    constexpr uint32_t idesc = make_idesc_e4m3_f32(128, N), idesc_pv = make_idesc_e4m3_f32(128, kTerms * N);
-    const uint32_t q_addr = smem_u32(q_smem), p_addr = smem_u32(p_smem);
+    // ------------------------------------------------------------------------------------------ scores
+    constexpr uint32_t idesc = make_idesc_e4m3_f32(128, Sh::kSCols);
+    const uint32_t q_addr = smem_u32(q_smem);
     int it = 0, unit = 0;
-    auto issue_pv = [&](int i, bool first) {
-      const int stage = i % kStages, buf = i & 1;
-      if (!warp_wait(b_pready + 8 * buf, (i >> 1) & 1, abort_flag)) return false;
-      tc_fence_after();
-      if (elect_one()) {
-        const uint64_t a = make_kmajor_sw128_desc(smem_u32(smem + stage * 2 * Sh::kTile + Sh::kTile));
-        const uint64_t b = make_kmajor_sw128_desc(p_addr + buf * Sh::kP);
-#pragma unroll
-        for (int k = 0; k < kPage / 32; ++k)
-          mma_f8f6f4(tmem + 2 * N + (kGroups == 2 ? buf * kTerms * N : 0), a + 2 * k, b + 2 * k, idesc_pv, !(first && k == 0));
-        tc_commit(b_empty + 8 * stage);
-        tc_commit(b_pvdone + 8 * buf);
-      }
-      __syncwarp();
-      return true;
-    };
     while (left > 0 && ok) {
-      const int t1 = static_cast<int>(min(static_cast<int64_t>(cur.v.tiles), t0 + left));
-      left -= t1 - t0;
+      if (!take()) break;
       if (!warp_wait(b_qready, unit & 1, abort_flag)) {
         ok = false;
         site = 1;
@@ -370,26 +369,46 @@ __global__ void __launch_bounds__((Shape<DIM, N, kTermsOf<T>>::kThreads), (Shape
         if (elect_one()) {
           const uint64_t a = rows_desc<DIM>(smem_u32(smem + stage * 2 * Sh::kTile));
 #pragma unroll
-          for (int term = 0; term < kTerms; ++term) {
+          for (int term = 0; term < (Sh::kStack ? 1 : kTerms); ++term) {
             const uint64_t b = rows_desc<DIM>(q_addr + term * N * DIM);
 #pragma unroll
-            for (int k = 0; k < DIM / 32; ++k) mma_f8f6f4(tmem + buf * N, a + 2 * k, b + 2 * k, idesc, term + k > 0);
+            for (int k = 0; k < DIM / 32; ++k) mma_f8f6f4(tmem + buf * Sh::kSCols, a + 2 * k, b + 2 * k, idesc, term + k > 0);
           }
           tc_commit(b_sfull + 8 * buf);
         }
         __syncwarp();
-        if (t > t0 && !issue_pv(it - 1, t - 1 < t0 + kGroups)) {
+      }
+      if (left > 0 && !next_unit(p, cur)) break;
+    }
+    if (!ok && lane == 0) *p.status = kRoleMma * 1000 + site;
+  } else if (warp == 2) {
+    // ------------------------------------------------------------------------------------------ values
+    constexpr uint32_t idesc = make_idesc_e4m3_f32(128, kTerms * N);
+    const uint32_t p_addr = smem_u32(p_smem);
+    int it = 0;
+    while (left > 0 && ok) {
+      if (!take()) break;
+      for (int t = t0; t < t1; ++t, ++it) {
+        const int stage = it % kStages, buf = it & 1;
+        if (!warp_wait(b_pready + 8 * buf, (it >> 1) & 1, abort_flag)) {
           ok = false;
           site = 3;
           break;
         }
+        tc_fence_after();
+        if (elect_one()) {
+          const uint64_t a = make_kmajor_sw128_desc(smem_u32(smem + stage * 2 * Sh::kTile + Sh::kTile));
+          const uint64_t b = make_kmajor_sw128_desc(p_addr + buf * Sh::kP);
+          const bool more = t - t0 >= kGroups;  // the group has an O^T of this unit already
+#pragma unroll
+          for (int k = 0; k < kPage / 32; ++k)
+            mma_f8f6f4(tmem + 2 * Sh::kSCols + (kGroups == 2 ? buf * kTerms * N : 0), a + 2 * k, b + 2 * k, idesc, more || k > 0);
+          // the softmax has had S^T, so both of the stage's pages are done with
+          tc_commit(b_empty + 8 * stage);
+          tc_commit(b_pvdone + 8 * buf);
+        }
+        __syncwarp();
       }
-      // the unit's last product does not wait for the next unit's queries
-      if (ok && !issue_pv(it - 1, t1 - 1 < t0 + kGroups)) {
-        ok = false;
-        site = 4;
-      }
-      t0 = 0;
       if (left > 0 && !next_unit(p, cur)) break;
     }
     if (!ok && lane == 0) *p.status = kRoleMma * 1000 + site;
@@ -397,10 +416,10 @@ __global__ void __launch_bounds__((Shape<DIM, N, kTermsOf<T>>::kThreads), (Shape
     // ------------------------------------------------------------------------------------------ softmax
     // A wait that gives up is remembered, not acted on: the warps leave together at their next vote, a group's own (which
     // ends its pages) or the one of all.
-    const int quarter = warp & 3, token = quarter * 32 + lane, at = (warp - 2) * 32 + lane, group = kGroups == 2 ? at >> 7 : 0;
+    const int quarter = warp & 3, token = quarter * 32 + lane, at = (warp - 3) * 32 + lane, group = kGroups == 2 ? at >> 7 : 0;
     const int st = at & 127;
     const uint32_t lane_off = static_cast<uint32_t>(quarter * 32) << 16;
-    const uint32_t t_all = tmem + 2 * N + lane_off, t_o = t_all + group * kTerms * N;
+    const uint32_t t_all = tmem + 2 * Sh::kSCols + lane_off, t_o = t_all + group * kTerms * N;
     float* refs = reinterpret_cast<float*>(misc + Sh::kRef);          // [group][copy][N]
     float* ref = refs + group * 2 * N;
     float* maxima = reinterpret_cast<float*>(misc + Sh::kWmax);       // [group][copy][4][N]: the warps' maxima, or sums, by row
@@ -410,7 +429,8 @@ __global__ void __launch_bounds__((Shape<DIM, N, kTermsOf<T>>::kThreads), (Shape
     auto vote = [&](bool mine) { return softmax_vote(1 + group, 128, mine); };
     auto vote_all = [&](bool mine) { return softmax_vote(kGroups == 2 ? 3 : 1, 128 * kGroups, mine); };
     int it = 0, turn = 0;
-    int64_t tile_at = begin;
+    int64_t number_at = begin - from;  // of the current unit
+    int4 rec = make_int4(-1, 0, 0, 0);
     float l[N];
     int side = 0;  // which of the two copies of the references holds
     auto wait = [&](uint32_t bar, uint32_t parity, int where) {
@@ -420,8 +440,7 @@ __global__ void __launch_bounds__((Shape<DIM, N, kTermsOf<T>>::kThreads), (Shape
       }
     };
     while (left > 0) {
-      const int t1 = static_cast<int>(min(static_cast<int64_t>(cur.v.tiles), t0 + left));
-      left -= t1 - t0;
+      if (!take()) break;
       const SeqView v = cur.v;
       const int rows = v.n * p.group;
       // ---- queries: eight elements per thread, split into e4m3 terms under a power-of-two scale of their row
@@ -458,7 +477,7 @@ __global__ void __launch_bounds__((Shape<DIM, N, kTermsOf<T>>::kThreads), (Shape
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
               uint32_t term[kTerms];
-              split_e4m3<kTerms>(f[2 * j] * inv, f[2 * j + 1] * inv, 1.f, term);
+              split_e4m3<kTerms>(f[2 * j] * inv, f[2 * j + 1] * inv, Sh::kStack ? kTermStep : 1.f, term);
 #pragma unroll
               for (int x = 0; x < kTerms; ++x) out[x][j >> 1] = (j & 1) ? out[x][j >> 1] | (term[x] << 16) : term[x];
             }
@@ -501,7 +520,7 @@ __global__ void __launch_bounds__((Shape<DIM, N, kTermsOf<T>>::kThreads), (Shape
         }
         wait(b_sfull + 8 * buf, (it >> 1) & 1, 2);
         tc_fence_after();
-        const uint32_t t_s = tmem + buf * N + lane_off;
+        const uint32_t t_s = tmem + buf * Sh::kSCols + lane_off;
         // ---- exponents: z = S * (row's factor * page's scale) + log2 v_scale - ref + kNominal, eight rows at a time
         float z[N];
         const float shift = ti.lv + kNominal;
@@ -509,9 +528,18 @@ __global__ void __launch_bounds__((Shape<DIM, N, kTermsOf<T>>::kThreads), (Shape
 #pragma unroll
           for (int c = 0; c < N; c += 16) {
             if (c >= rows) break;
-            uint32_t s[16];
-            tmem_ld_32x16(t_s + c, s);
+            constexpr int kParts = Sh::kStack ? kTerms : 1;
+            uint32_t part[kParts][16];
+#pragma unroll
+            for (int x = 0; x < kParts; ++x) tmem_ld_32x16(t_s + x * N + c, part[x]);
             tmem_ld_wait();
+            float s[16];
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+              s[j] = __uint_as_float(part[kParts - 1][j]);
+#pragma unroll
+              for (int x = kParts - 2; x >= 0; --x) s[j] = fmaf(s[j], 1.f / kTermStep, __uint_as_float(part[x][j]));
+            }
 #pragma unroll
             for (int g = 0; g < 16; g += 8) {
               if (c + g >= rows) break;
@@ -519,7 +547,7 @@ __global__ void __launch_bounds__((Shape<DIM, N, kTermsOf<T>>::kThreads), (Shape
               load8(rowmul + c + g, m);
               load8(ref + side * N + c + g, r);
 #pragma unroll
-              for (int j = 0; j < 8; ++j) z[c + g + j] = fmaf(__uint_as_float(s[g + j]), m[j] * ti.ks, with_ref ? shift - r[j] : shift);
+              for (int j = 0; j < 8; ++j) z[c + g + j] = fmaf(s[g + j], m[j] * ti.ks, with_ref ? shift - r[j] : shift);
             }
           }
           if (!whole) {
@@ -595,14 +623,15 @@ __global__ void __launch_bounds__((Shape<DIM, N, kTermsOf<T>>::kThreads), (Shape
               *reinterpret_cast<float4*>(now + g + 4) = make_float4(top[4], top[5], top[6], top[7]);
             }
             if (mine > 0 && any) {
+              uint32_t o[kTerms][8];
+#pragma unroll
+              for (int x = 0; x < kTerms; ++x) tmem_ld_32x8(t_o + x * N + g, o[x]);
+              tmem_ld_wait();
 #pragma unroll
               for (int x = 0; x < kTerms; ++x) {
-                uint32_t o[8];
-                tmem_ld_32x8(t_o + x * N + g, o);
-                tmem_ld_wait();
 #pragma unroll
-                for (int j = 0; j < 8; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * f[j]);
-                tmem_st_32x8(t_o + x * N + g, o);
+                for (int j = 0; j < 8; ++j) o[x][j] = __float_as_uint(__uint_as_float(o[x][j]) * f[j]);
+                tmem_st_32x8(t_o + x * N + g, o[x]);
               }
             }
           }
@@ -614,8 +643,8 @@ __global__ void __launch_bounds__((Shape<DIM, N, kTermsOf<T>>::kThreads), (Shape
           }
         }
         ++mine;
-        // ---- P.  Its buffer is free: S^T of this page was issued behind the product before the last, which read it, and the
-        // barrier that announced S^T counts every product issued before.
+        // ---- P; its buffer is free once the product before the last has read it
+        wait(b_pvdone + 8 * buf, ((it >> 1) & 1) ^ 1, 5);
         const uint32_t pb = smem_u32(p_smem) + buf * Sh::kP + token;
 #pragma unroll
         for (int g = 0; g < N; g += 8) {
@@ -766,21 +795,16 @@ __global__ void __launch_bounds__((Shape<DIM, N, kTermsOf<T>>::kThreads), (Shape
         }
       }
       tc_fence_before();
-      if (left == 0 && at == 0) {
-        // does the unit go on behind this block, and did it begin here?
-        int4 rec = make_int4(-1, 0, 0, 0);
-        if (t0 == 0 && t1 < v.tiles) {
-          const int64_t unit_end = tile_at + v.tiles;
-          rec = make_int4(v.lo, cur.h, v.n, static_cast<int>((unit_end * blocks - 1) / total));
-        }
-        p.record[blockIdx.x] = rec;
+      if (t0 == 0 && t1 < v.tiles) {
+        // the unit begins here and goes on behind this block
+        const int64_t unit_end = number_at + numbers(v);
+        rec = make_int4(v.lo, cur.h, v.n, static_cast<int>((unit_end * blocks - 1) / total));
       }
-      tile_at += t1 - t0;
-      t0 = 0;
+      number_at += numbers(v);
       if (left > 0 && !next_unit(p, cur)) break;
     }
     if (!ok && lane == 0) *p.status = kRoleEpilogue * 1000 + site;
-    if (abort_flag[0] && at == 0) p.record[blockIdx.x] = make_int4(-1, 0, 0, 0);
+    if (work && at == 0) p.record[blockIdx.x] = abort_flag[0] ? make_int4(-1, 0, 0, 0) : rec;
   }
   tc_fence_before();
   __syncthreads();
