@@ -348,6 +348,46 @@ def moe_decode_sweep(dev, hbm_peak_gbs: float):
     return {"shape": f"hidden={H} intermediate={I} experts={E} top_k={topk}", "rows": rows}
 
 
+def decoder_layer_sweep(dev, hbm_peak_gbs: float):
+    """A whole FP8 decoder layer of the Llama-3.1-8B sizes over its 8-bit cache: decode steps (one token per sequence, 2048
+    in the cache) as CUDA-graph replays over as many layers as make the weights exceed L2, and one 4096-token prompt."""
+    import tilegym_b200 as tg
+
+    hidden, heads, kv, dim, inter, ctx = 4096, 32, 8, 128, 14336, 2048
+    f, m = tg.rope_frequencies(dim, 500000.0, device=dev)
+
+    def weights():
+        def w(n, k):
+            return torch.randn(n, k, device=dev, dtype=torch.bfloat16).mul_(0.02)
+
+        one = torch.ones(hidden, device=dev, dtype=torch.bfloat16)
+        return {"norm1": one, "norm2": one, "qkv": w((heads + 2 * kv) * dim, hidden), "o": w(hidden, heads * dim),
+                "gate_up": w(2 * inter, hidden), "down": w(hidden, inter)}
+
+    layers = [tg.FP8DecoderLayer(weights(), heads, kv, dim, f, m) for _ in range(3)]  # 218 MB each
+    layer_bytes = (heads + 2 * kv) * dim * hidden + hidden * heads * dim + 3 * inter * hidden
+    rows = []
+    for seqs in (1, 16, 64):
+        per = ctx // 128 + 1
+        caches = [tg.FP8KVCache.empty(seqs * per, kv, dim, dev) for _ in layers]
+        table = torch.randperm(seqs * per, device=dev).to(torch.int32).view(seqs, per)
+        lens = torch.full((seqs,), ctx, dtype=torch.int32, device=dev)
+        x = torch.randn(seqs, hidden, device=dev, dtype=torch.bfloat16)
+        us = graph_time_us(lambda i: layers[i % 3](x, x, caches[i % 3], table, lens), 9)
+        gbs = (layer_bytes + 2 * seqs * ctx * kv * dim) / us / 1e3
+        rows.append({"sequences": seqs, "context": ctx, "us": round(us, 1), "gbs": round(gbs, 1), "frac_hbm": round(gbs / hbm_peak_gbs, 3)})
+    tokens = 4096
+    cache = tg.FP8KVCache.empty(tokens // 128, kv, dim, dev)
+    table = torch.arange(tokens // 128, device=dev, dtype=torch.int32)[None]
+    lens = torch.tensor([tokens], dtype=torch.int32, device=dev)
+    cu = torch.tensor([0, tokens], dtype=torch.int32, device=dev)
+    x = torch.randn(tokens, hidden, device=dev, dtype=torch.bfloat16)
+    us = graph_time_us(lambda i: layers[i % 3](x, x, cache, table, lens, cu), 6)
+    flops = 2 * tokens * layer_bytes + 2 * tokens * tokens * heads * dim
+    rows.append({"prompt": tokens, "us": round(us, 1), "tflops": round(flops / us / 1e6, 1)})
+    return rows
+
+
 def run_configs(dev, peaks):
     """Bounded sweeps of the benchmark configurations the headline number does not cover."""
     hbm = float(peaks["hbm_gbs"])
@@ -379,4 +419,5 @@ def run(dev, peaks):
         "swiglu_gate_up": swiglu_sweep(dev),
         "llama8b_mlp_block": mlp_block_sweep(dev),
         "fp8linear_decode": linear_decode_sweep(dev),
+        "decoder_layer": decoder_layer_sweep(dev, hbm),
     }

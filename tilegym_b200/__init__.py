@@ -6,7 +6,7 @@ Public surface (same names and signatures as the reference operators):
     matmul, bmm                                        (tilegym.ops)
 plus the per-tensor pieces the reference lacks (fp8_scaled_mm, fp8_block_scaled_mm, quant_per_tensor,
 weight_quant_block, FP8Linear), the decoder operators around the GEMMs (rms_norm_quant, apply_rope, kv_cache_write,
-kv_cache_read, paged_attention on an FP8KVCache) and apply_tilegym_kernel_to_llama / _deepseek_v2.
+kv_cache_read, paged_attention on an FP8KVCache), the FP8DecoderLayer that runs them together and apply_tilegym_kernel_to_llama / _deepseek_v2.
 """
 
 from .ops import (  # noqa: F401
@@ -38,6 +38,7 @@ from .attention import (  # noqa: E402,F401
     paged_attention,
     rope_frequencies,
 )
+from .decoder import FP8DecoderLayer  # noqa: E402,F401
 from .moe import FP8MoE, fused_experts_impl, fused_moe, moe_align_block_size  # noqa: E402,F401
 
 __version__ = "0.1.0"
