@@ -499,6 +499,32 @@ def test_attention_is_deterministic_on_any_stream_and_in_graphs(dev, new):
     check_attention(dev, q, ref, table, shorter, new, got=results[0])
 
 
+def test_caches_beyond_four_gigabytes(dev):
+    """Offsets that pass 32 bits: the same tokens in the last pages of a 4.9 GB cache (each of keys and values) and in a small one."""
+    pages, heads, dim = 37500, 8, 128
+    big = tg.FP8KVCache(torch.empty(pages, heads, 128, dim, dtype=torch.uint8, device=dev).view(F8),
+                        torch.empty(pages, heads, dim, 128, dtype=torch.uint8, device=dev).view(F8),
+                        torch.empty(pages, heads, device=dev), torch.empty(pages, heads, device=dev))
+    small = tg.FP8KVCache.empty(6, heads, dim, dev)
+    assert big.k.numel() > 2**32
+    t1 = i32([[0, 3, 1], [2, 4, 5]])
+    t2 = torch.where(t1 % 2 == 0, t1, pages - 6 + t1).to(torch.int32)  # page 0, 2, 4 and the last ones
+    lens, new = i32([300, 200]), [300, 200]
+    g = gen(31)
+    k, v = (torch.randn(500, heads, dim, generator=g).to(BF).to(dev) for _ in "kv")
+    q = torch.randn(500, 16, dim, generator=g).to(BF).to(dev)
+    got = []
+    for cache, t in ((small, t1), (big, t2)):
+        args = t.to(dev), lens.to(dev)
+        tg.kv_cache_write(cache, k, v, *args, cumulative(new).to(dev))
+        one = tg.paged_attention(q[:2], cache, *args)
+        many = tg.paged_attention(q, cache, *args, cumulative(new).to(dev), max_q_len=300)
+        got.append((one, many, *tg.kv_cache_read(cache, *args, 300)))
+    for a, b in zip(*got):
+        assert torch.equal(a, b)
+    assert torch.equal(big.k_scale[t2[0, 1]], small.k_scale[t1[0, 1]])
+
+
 # ------------------------------------------------------------------ refusals on the device
 def test_refuses_gradients(dev):
     x = torch.randn(2, 128, dtype=BF, device=dev, requires_grad=True)

@@ -399,6 +399,7 @@ int32_t api_make_page_map(CUtensorMap* map, uint64_t ptr, int64_t rows, int cols
   if (r != CUDA_SUCCESS) return fail(TG_ERR_ARGS, "cuTensorMapEncodeTiled (cache) failed with CUresult %d", static_cast<int>(r));
   return TG_OK;
 }
+bool api_pdl() { return knob(kKnobPdl, 1) != 0; }
 uint32_t api_wait_limit_us() { return g_wait_limit_us; }
 int32_t api_init_device(int dev, int* num_sms, int32_t** status) {
   int32_t rc = init_device(dev);

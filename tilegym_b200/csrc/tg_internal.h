@@ -115,6 +115,7 @@ int32_t api_make_map(CUtensorMap* map, uint64_t ptr, int64_t rows, int64_t K, in
 // dense rows of 64 or 128 bytes (64- or 128-byte swizzle), boxes of whole rows; for the pages of an 8-bit cache
 int32_t api_make_page_map(CUtensorMap* map, uint64_t ptr, int64_t rows, int cols, int box_rows);
 int32_t api_init_device(int dev, int* num_sms, int32_t** status);  // call with `dev` current
+bool api_pdl();  // programmatic dependent launch is on (TILEGYM_B200_PDL)
 uint32_t api_wait_limit_us();  // tg_set_wait_limit_us() value (0 = default), for GemmParams::wait_limit_us
 
 cudaError_t launch_act_quant(void* y, float* s, const void* x, int x_dtype, int64_t n_blocks, cudaStream_t stream);

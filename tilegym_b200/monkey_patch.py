@@ -2,8 +2,9 @@
 
 `apply_tilegym_kernel_to_<model>(rope, rms_norm, swiglu, attn, model, use_cutile)` is the signature of
 src/tilegym/transformers/monkey_patch.py:24-31 (llama), :64-72 (deepseek_v2) and the other model types; this
-package covers only the FP8 Linear path, so those flags are accepted for drop-in compatibility and do nothing
-here (the kernels they select are outside this library), and one opt-in keyword is added: `fp8_linear`.
+package patches only the Linear layers, so those flags are accepted for drop-in compatibility and do nothing here
+(norms, rotary positions and attention run on this package's kernels in `FP8DecoderLayer`, which replaces a whole
+layer), and one opt-in keyword is added: `fp8_linear`.
 With `fp8_linear=True` the nn.Linear layers of the decoder are replaced by `FP8Linear`:
   * `model` given  -> its Linear modules are converted in place (weights must be on a CUDA device);
   * `model` None   -> (the reference's "call before model initialisation" form) models of that type built
@@ -101,7 +102,7 @@ def _make(model_type: str, flags=("rope", "rms_norm", "swiglu", "attn"), default
         a = bound.arguments
         for flag in flags:
             if a[flag] and not (flag == fuse_flag and a["fp8_linear"]):
-                logger.debug("tilegym_b200: %s=True accepted; that kernel is not part of this library", flag)
+                logger.debug("tilegym_b200: %s=True accepted; nothing is patched for it", flag)
         _apply(model_type, a.get("model"), a["fp8_linear"], a["fp8_mode"],
                fuse_swiglu=bool(a[fuse_flag]) if fuse_flag else False)
 
