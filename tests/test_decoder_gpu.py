@@ -525,6 +525,45 @@ def test_caches_beyond_four_gigabytes(dev):
     assert torch.equal(big.k_scale[t2[0, 1]], small.k_scale[t1[0, 1]])
 
 
+def test_the_extension_and_ctypes_make_the_same_calls(dev, monkeypatch):
+    """The ordinary calls go through the C++ extension, the others and those without it through ctypes: same bits, same errors."""
+    assert _lib.fast is not None, "tilegym_b200/_bind.so is missing: run `python -m tilegym_b200.build`"
+    g = gen(41)
+    x, w, r = (torch.randn(*s, generator=g).to(BF).to(dev) for s in ((6, 256), (256,), (6, 256)))
+    table, ref = make_kv([300, 100], 2, 64, g)
+    qkv = torch.randn(4, 8, 64, generator=g).to(BF).to(dev)
+    f, _ = tg.rope_frequencies(64, device=dev)
+    td, ld, cu = table.to(dev), i32([300, 100]).to(dev), i32([0, 3, 4]).to(dev)
+    out = torch.empty(4, 4, 64, dtype=BF, device=dev)
+
+    def calls():
+        cache = on(dev, ref)
+        q = tg.kv_cache_write(cache, qkv[:, 4:6], qkv[:, 6:], td, ld, cu, inv_freq=f, q=qkv[:, :4])
+        res = [*tg.rms_norm_quant(x, w, 1e-5), *tg.rms_norm_quant(x, w, 1e-5, residual=r, weight_offset=0.5),
+               *tg.apply_rope(qkv[:, :4], qkv[:, 4:6], torch.arange(4, device=dev), f, True, 1.1), tg.apply_rope(qkv[:, :4], None, torch.arange(4, device=dev), f)[0],
+               q, *cache, tg.paged_attention(q, cache, td, ld, cu, max_q_len=3), tg.paged_attention(q, cache, td, ld, cu, window=50, sinks=2, scale=0.2)]
+        assert tg.paged_attention(q, cache, td, ld, cu, max_q_len=3, out=out) is out
+        assert tg.kv_cache_write(cache, qkv[:, 4:6], qkv[:, 6:], td, ld, cu) is None
+        rr = r.clone()
+        assert tg.rms_norm_quant(x, w, 1e-5, residual=rr, inplace=True)[2] is rr
+        with pytest.raises(_lib.TileGymB200Error):
+            tg.paged_attention(q, cache, td, ld, cu, sinks=2)
+        with pytest.raises(_lib.TileGymB200Error):
+            tg.paged_attention(q.float(), cache, td, ld, cu)
+        with pytest.raises(_lib.TileGymB200Error):
+            tg.kv_cache_write(cache, qkv[:, 4:6], qkv[:, 6:], td.long(), ld, cu)
+        with pytest.raises(AssertionError):
+            tg.paged_attention(q, cache, td, ld, cu, out=out[:3])
+        with pytest.raises(RuntimeError, match="no backward"):
+            tg.apply_rope(qkv.clone().requires_grad_(), None, torch.arange(4, device=dev), f)
+        return [*res, out.clone(), rr]
+
+    fast = calls()
+    monkeypatch.setattr(_lib, "fast", None)
+    for a, b in zip(fast, calls()):
+        assert torch.equal(a.view(torch.uint8) if a.dtype == F8 else a, b.view(torch.uint8) if b.dtype == F8 else b)
+
+
 # ------------------------------------------------------------------ refusals on the device
 def test_refuses_gradients(dev):
     x = torch.randn(2, 128, dtype=BF, device=dev, requires_grad=True)

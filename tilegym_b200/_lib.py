@@ -64,6 +64,13 @@ class TileGymB200Error(RuntimeError):
 
 _lib: Optional[ctypes.CDLL] = None
 
+# The extension that makes the ordinary calls of the decode-sized operators (csrc/torch_bind.cpp).  It calls the same library;
+# without it the same calls go through ctypes.
+try:
+    from . import _bind as fast
+except ImportError:
+    fast = None
+
 # name -> (restype, argtypes); the list the symbol-export test walks.
 _P = ctypes.c_char_p  # const TgTensorDesc*, passed as the packed bytes of desc()
 SIGNATURES = {

@@ -160,6 +160,10 @@ def apply_rope(
     With inplace=True q and k are overwritten (their pitches must keep 16-byte alignment) and only the rotated elements
     are touched.
     """
+    if _lib.fast is not None:
+        result = _lib.fast.apply_rope(q, k, positions, inv_freq, interleaved, magnitude, inplace)
+        if result is not None:
+            return result
     dev = ops._cuda_index(q, k, positions, inv_freq)
     ops._no_grad_inputs(q, k)
     q1, q_desc = _heads(q, "q")
@@ -209,6 +213,10 @@ def kv_cache_write(
     cu_seqlens, positions outside the table and pages outside the cache are left alone (their rows of q are unspecified).
     A page that is written must belong to one sequence.
     """
+    if _lib.fast is not None:
+        result = _lib.fast.kv_cache_write(*cache, k, v, block_table, seq_lens, cu_seqlens, inv_freq, q, interleaved, magnitude)
+        if result is not None:
+            return result[0]
     dev = ops._cuda_index(*cache, k, v, block_table, seq_lens, cu_seqlens, inv_freq, q)
     ops._no_grad_inputs(k, v, q)
     qo = qo_desc = q_desc = None
@@ -281,24 +289,30 @@ def paged_attention(
     are not written.
     """
     dev = ops._cuda_index(q, *cache, block_table, seq_lens, cu_seqlens, out)
+    if q.dim() != 3:
+        raise _lib.TileGymB200Error(-6, "q must be [tokens, heads, head_dim]")
+    tokens, heads, dim = q.shape
+    max_q_len = int(max_q_len) if max_q_len is not None else 1 if cu_seqlens is None else max(tokens, 1)
+    need = _workspace_bytes(heads, cache.k.shape[1], dim, max_q_len, dev)
+    scale = dim ** -0.5 if scale is None else float(scale)
+    if _lib.fast is not None:
+        result = _lib.fast.paged_attention(q, *cache, block_table, seq_lens, cu_seqlens, max_q_len, scale, int(window), int(sinks), out, need)
+        if result is not None:
+            return result if out is None else out
     ops._no_grad_inputs(q)
     q, q_desc = _heads(q, "q")
-    tokens, heads, dim = q.shape
     if out is None:
         out, out_desc = _new_heads(q)
     else:
         assert out.shape == q.shape and out.dtype == q.dtype, "out must have q's shape and type"
         out_desc = _lib.desc(out)
-    if max_q_len is None:
-        max_q_len = 1 if cu_seqlens is None else max(tokens, 1)
     block_table, seq_lens, cu_seqlens = _tables(block_table, seq_lens, cu_seqlens)
-    need = _workspace_bytes(heads, cache.k.shape[1], dim, max_q_len, dev)
     # allocated per call: calls on other streams, and graphs that are replayed side by side, never share it
     ws = q.new_empty(need, dtype=torch.uint8) if need else None
     desc = _lib.desc
     rc = _lib.lib().tg_paged_attention(
         out_desc, q_desc, desc(cache.k), desc(cache.v), desc(cache.k_scale), desc(cache.v_scale), desc(block_table), desc(seq_lens),
-        desc(cu_seqlens), int(max_q_len), dim ** -0.5 if scale is None else float(scale), int(window), int(sinks),
+        desc(cu_seqlens), max_q_len, scale, int(window), int(sinks),
         0 if ws is None else ws.data_ptr(), need, dev, torch._C._cuda_getCurrentRawStream(dev),
     )
     _lib.check_rc(rc)

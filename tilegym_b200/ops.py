@@ -350,6 +350,10 @@ def rms_norm_quant(
     `fp8_block_scaled_mm` takes as A / As.  x, residual (..., hidden) bf16 or f16, hidden a multiple of 128 up to
     65536; weight (hidden,) in x's type or fp32.  With inplace=True h is written over `residual`.
     """
+    if _lib.fast is not None:
+        result = _lib.fast.rms_norm_quant(x, weight, eps, residual, weight_offset, inplace)
+        if result is not None:
+            return result
     dev = _cuda_index(x, weight, residual)
     _no_grad_inputs(x, residual)
     hidden = x.shape[-1]
