@@ -211,9 +211,46 @@ __global__ void __launch_bounds__((Shape<DIM, N, kTermsOf<T>>::kThreads), (Shape
   griddep_launch_dependents();
 
   // ---- this block's range of pages
-  int64_t total, begin = 0, end = 0, blocks;
+  int64_t total, begin = 0, end = 0, blocks, front = 0;
+  Cursor cur;
+  cur.b = -1;
+  cur.v = SeqView{};
   auto numbers = [](const SeqView& v) { return v.tiles > 0 ? v.tiles + Sh::kUnitCost : 0; };
-  {
+  auto divide = [&]() {
+    total *= p.c.heads;
+    blocks = min(static_cast<int64_t>(gridDim.x), total);  // the others have nothing to do
+    if (blockIdx.x < blocks) {
+      begin = total * blockIdx.x / blocks;
+      end = total * (blockIdx.x + 1) / blocks;
+    }
+  };
+  if (p.c.seqs <= 32) {
+    // a lane per sequence, every warp for itself: no barrier in the way of a small batch
+    SeqView v = {};
+    if (lane < p.c.seqs) v = view_sequence(p, lane, 0, p.max_q_len);
+    const int n = numbers(v);
+    int64_t incl = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t up = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += up;
+    }
+    total = __shfl_sync(0xffffffffu, incl, 31);
+    divide();
+    if (begin < end) {
+      const int64_t target = begin / p.c.heads;
+      const uint32_t hit = __ballot_sync(0xffffffffu, n > 0 && incl - n <= target && target < incl);
+      cur.b = __ffs(hit) - 1;
+      front = __shfl_sync(0xffffffffu, incl - n, cur.b);
+      cur.v.lo = __shfl_sync(0xffffffffu, v.lo, cur.b);
+      cur.v.n = __shfl_sync(0xffffffffu, v.n, cur.b);
+      cur.v.len = __shfl_sync(0xffffffffu, v.len, cur.b);
+      cur.v.pos0 = __shfl_sync(0xffffffffu, v.pos0, cur.b);
+      cur.v.tiles = __shfl_sync(0xffffffffu, v.tiles, cur.b);
+      cur.v.sink_tiles = __shfl_sync(0xffffffffu, v.sink_tiles, cur.b);
+      cur.v.first_page = __shfl_sync(0xffffffffu, v.first_page, cur.b);
+    }
+  } else {
     const int mine = static_cast<int>(threadIdx.x) < p.c.seqs ? numbers(view_sequence(p, threadIdx.x, 0, p.max_q_len)) : 0;
     int64_t sum = mine;
     for (int b = threadIdx.x + kThreads; b < p.c.seqs; b += kThreads) sum += numbers(view_sequence(p, b, 0, p.max_q_len));
@@ -225,12 +262,7 @@ __global__ void __launch_bounds__((Shape<DIM, N, kTermsOf<T>>::kThreads), (Shape
     total = 0;
 #pragma unroll
     for (int w = 0; w < kThreads / 32; ++w) total += sched[2 + w];
-    total *= p.c.heads;
-    blocks = min(static_cast<int64_t>(gridDim.x), total);  // the others have nothing to do
-    if (blockIdx.x < blocks) {
-      begin = total * blockIdx.x / blocks;
-      end = total * (blockIdx.x + 1) / blocks;
-    }
+    divide();
     // the sequence in which it begins: prefix sums, as far as needed
     const int64_t target = begin / p.c.heads;
     int64_t before = 0;
@@ -259,21 +291,25 @@ __global__ void __launch_bounds__((Shape<DIM, N, kTermsOf<T>>::kThreads), (Shape
       before = all;
       if (before > target) break;  // the same for every thread
     }
+    __syncthreads();
+    cur.b = begin < end ? static_cast<int>(sched[1]) : -1;
+    if (cur.b >= 0) {
+      front = sched[0];
+      cur.v = view_sequence(p, cur.b, 0, p.max_q_len);
+    }
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
 
-  Cursor cur;
-  cur.b = static_cast<int>(sched[1]);
   int from = 0;  // number within the unit at which this block's part begins
   const bool work = begin < end && cur.b >= 0;
   if (work) {
-    cur.v = view_sequence(p, cur.b, 0, p.max_q_len);
-    const int64_t rem = begin - sched[0] * p.c.heads;
-    cur.h = static_cast<int>(rem / numbers(cur.v));
-    from = static_cast<int>(rem - static_cast<int64_t>(cur.h) * numbers(cur.v));
+    const int64_t rem = begin - front * p.c.heads;
+    const int each = numbers(cur.v);
+    cur.h = rem <= 0xffffffffll ? static_cast<int>(static_cast<uint32_t>(rem) / static_cast<uint32_t>(each)) : static_cast<int>(rem / each);
+    from = static_cast<int>(rem - static_cast<int64_t>(cur.h) * each);
   } else if (threadIdx.x == 0) {
     p.record[blockIdx.x] = make_int4(-1, 0, 0, 0);
   }
@@ -825,18 +861,35 @@ __global__ void __launch_bounds__(4 * DIM) tg_attention_join_kernel(const Attent
   if (rec.x < 0 || r >= rec.z * p.group) return;
   const int first = blockIdx.x, last = min(rec.w, static_cast<int>(gridDim.x) - 1);
   const int64_t head = (2 * static_cast<int64_t>(first) + 1) * rows_padded + r;  // the first part: slot 1 of its block
-  float m = p.part_ml[head].x;
-#pragma unroll 8
-  for (int i = first + 1; i <= last; ++i) m = fmaxf(m, p.part_ml[2 * static_cast<int64_t>(i) * rows_padded + r].x);
-  const float base = m == -INFINITY ? 0.f : m;
-  float l = 0.f, o = 0.f;
-#pragma unroll 8
-  for (int i = first; i <= last; ++i) {
-    const int64_t at = i == first ? head : 2 * static_cast<int64_t>(i) * rows_padded + r;
-    const float2 ml = p.part_ml[at];
-    const float f = exp2f(ml.x - base);
-    l = fmaf(ml.y, f, l);
-    o = fmaf(p.part_o[at * DIM + d], f, o);
+  // eight parts at a time, their loads in flight together
+  float m = -1e30f, l = 0.f, o = 0.f;
+  for (int i0 = first; i0 <= last; i0 += 8) {
+    float2 ml[8];
+    float x[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const int i = min(i0 + k, last);
+      const int64_t at = i == first ? head : 2 * static_cast<int64_t>(i) * rows_padded + r;
+      ml[k] = p.part_ml[at];
+      x[k] = p.part_o[at * DIM + d];
+      if (i0 + k > last) {
+        ml[k] = make_float2(-1e30f, 0.f);
+        x[k] = 0.f;
+      }
+    }
+    float top = m;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) top = fmaxf(top, ml[k].x);
+    const float shrink = exp2f(m - top);
+    l *= shrink;
+    o *= shrink;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const float f = exp2f(ml[k].x - top);
+      l = fmaf(ml[k].y, f, l);
+      o = fmaf(x[k], f, o);
+    }
+    m = top;
   }
   const int i = r / p.group;
   static_cast<T*>(p.o)[(rec.x + i) * p.o_tok + (rec.y * p.group + r - i * p.group) * p.o_head + d] = static_cast<T>(l == 0.f ? 0.f : o / l);
