@@ -367,16 +367,25 @@ __global__ void __launch_bounds__(kThreads, 1)
       // all copies first, into the space of the f16 values, which waits for the queries: one latency, no registers
       uint8_t* raw = v16_smem + w * Sh::kV16 + e * 2;
       const T* q0 = static_cast<const T*>(p.q) + static_cast<int64_t>(v.lo + w * tile_tokens) * p.q_tok + head * p.group * p.q_head + e;
+      // (token, head of the group) of the row, stepped along with it
+      int ti = (st / kLanes) / p.group, hg = st / kLanes - ti * p.group;
+      const int step_t = kRows / p.group, step_h = kRows - step_t * p.group;
+      const int tokens = min(tile_tokens, v.n - w * tile_tokens);
 #pragma unroll 4
       for (int r = st / kLanes; r < 128; r += kRows) {
-        const int ti = r / p.group;
-        if (ti < tile_tokens && w * tile_tokens + ti < v.n)
-          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(raw + r * (2 * DIM))), "l"(q0 + ti * p.q_tok + (r - ti * p.group) * p.q_head) : "memory");
+        if (ti < tokens)
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(raw + r * (2 * DIM))), "l"(q0 + ti * p.q_tok + hg * p.q_head) : "memory");
         else
           *reinterpret_cast<uint4*>(raw + r * (2 * DIM)) = make_uint4(0, 0, 0, 0);
+        ti += step_t;
+        hg += step_h;
+        if (hg >= p.group) {
+          hg -= p.group;
+          ++ti;
+        }
       }
       asm volatile("cp.async.wait_all;" ::: "memory");
-#pragma unroll 2
+#pragma unroll 4
       for (int r = st / kLanes; r < 128; r += kRows) {
         const uint4 x = *reinterpret_cast<const uint4*>(raw + r * (2 * DIM));  // this thread's own copy
         const uint32_t ww[4] = {x.x, x.y, x.z, x.w};
