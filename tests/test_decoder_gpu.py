@@ -433,6 +433,58 @@ def test_attention_nan_stays_with_those_who_see_it(dev):
         assert bool(((got.cpu().double() - o).abs() <= allowed(BF, o, *rest))[rows].all())
 
 
+@pytest.mark.parametrize("n", [1, 70])
+def test_attention_nan_keys_at_every_place_of_a_page(dev, n):
+    """One NaN in the key of one token: every row that sees the token has no answer, whichever path its exponential takes."""
+    g = gen(25)
+    table, ref = make_kv([256], 1, 64, g)
+    q = torch.randn(n, 2, 64, generator=g).to(BF).to(dev)
+    cache = on(dev, ref)
+    for t in range(0, 128):
+        k = cache.k.clone()
+        k.view(torch.uint8)[int(table[0, 0]), 0, t, t % 64] = 127
+        got = tg.paged_attention(q, cache._replace(k=k), table.to(dev), i32([256]).to(dev), i32([0, n]).to(dev), max_q_len=n)
+        assert bool(got.isnan().all()), t
+
+
+@pytest.mark.parametrize("n", [6, 150])
+def test_attention_factors_that_are_no_numbers(dev, n):
+    """A row of q with a NaN, a page whose scale is one or infinite: only rows that see something of it lose their answer."""
+    g = gen(26)
+    table, ref = make_kv([200], 1, 64, g)
+    q = torch.randn(n, 2, 64, generator=g).to(BF).to(dev)
+
+    def run(q, k_scale=ref[2], length=200):
+        cache = on(dev, [ref[0], ref[1], k_scale, ref[3]])
+        return tg.paged_attention(q, cache, table.to(dev), i32([length]).to(dev), i32([0, n]).to(dev), max_q_len=n)
+
+    good = run(q)
+    row = n // 2
+    for value in (math.nan, math.inf):
+        bad_q = q.clone()
+        bad_q[row, 1, 3] = value
+        bad = run(bad_q)
+        assert bool(bad[row, 1].isnan().all())
+        bad[row, 1] = good[row, 1]
+        assert torch.equal(bad, good)
+        scale = ref[2].clone()
+        scale[table[0, 1], 0] = value
+        bad = run(q, scale)
+        see = (torch.arange(200 - n, 200) >= 128).to(dev)  # positions that see the second page
+        assert bool(bad[see].isnan().all()) and torch.equal(bad[~see], good[~see])
+        # a length that leaves the row nothing to see
+        assert bool((run(bad_q, length=n - row - 1)[: row + 1] == 0).all())
+
+
+@pytest.mark.parametrize("heads,group,new,past", [(1, 64, [3, 1], [200, 0]), (3, 5, [40, 13], [128, 300]), (2, 33, [2, 2], [127, 5]), (1, 1, [513], [1])])
+def test_attention_group_sizes(dev, heads, group, new, past):
+    g = gen(group)
+    lens = [n + p for n, p in zip(new, past)]
+    table, ref = make_kv(lens, heads, 64, g)
+    q = torch.randn(sum(new), heads * group, 64, generator=g).to(BF)
+    check_attention(dev, q, ref, table, lens, new)
+
+
 def test_attention_padding_bad_pages_strides_and_out(dev):
     g = gen(23)
     lens, new = [300, 0, 200], [2, 1, 3]

@@ -75,15 +75,16 @@ __device__ __forceinline__ void to_f16(uint32_t w, uint32_t& a, uint32_t& b) {
   asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(b) : "h"(static_cast<uint16_t>(w >> 16)));
 }
 
+// maxima that a NaN gets through: the polynomial below would swallow one
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float d;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
 }
 
 // 2^x of a pair without the special-function unit: x = n + f with |f| <= 1/2, 2^f by a polynomial of degree 4 (fitted to the
 // relative error over that range, 2.6e-6 at most), n added to the exponent.  x <= 100; below -126 the result is 2^-126 or so,
-// which f16 rounds to zero (its share of the 32-bit sum is as small).
+// which f16 rounds to zero (its share of the 32-bit sum is as small).  A NaN is taken for -126: the row's maximum has seen to it.
 __device__ __forceinline__ float2 exp2_pair(float2 x) {
   const float2 magic = make_float2(12582912.f, 12582912.f), minus = make_float2(-12582912.f, -12582912.f);
   x.x = fmaxf(x.x, -126.f);
@@ -445,7 +446,12 @@ __global__ void __launch_bounds__(kThreads, 1)
       scales(entry1, ks1, vs1);
       const int entry2 = page_entry(j + 2);
       const bool here = entry >= 0 && entry < p.c.pages;
-      const float f = mul * ks;
+      float f = mul * ks;
+      // a factor that is no positive number (a row of q or a scale with an infinity or NaN) belongs to the tokens that the row
+      // sees, but -inf * f of the hidden ones has to stay -inf
+      if (f == 0.f) f = 1e-38f;
+      const bool odd = !(f > 0.f && f < INFINITY);
+      if (odd) f = 1.f;
       // log2 and reciprocal of the page's scale: a power of two where the cache was written by this library
       const uint32_t vb = __float_as_uint(vs);
       float lv, inv_vs;
@@ -484,9 +490,14 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
           for (int k = 1; k < 15; k += 2)
             mx[c] = max3(mx[c], __uint_as_float(s[c >> 1][(c & 1) * 16 + k]), __uint_as_float(s[c >> 1][(c & 1) * 16 + k + 1]));
-          mx[c] = fmaxf(mx[c], __uint_as_float(s[c >> 1][(c & 1) * 16 + 15]));
         }
-        const float top = fmaf(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])), f, lv);
+        auto last = [&](int c) { return __uint_as_float(s[c >> 1][(c & 1) * 16 + 15]); };
+        mx[0] = max3(mx[0], last(0), last(1));
+        mx[1] = max3(mx[1], last(2), last(3));
+        mx[2] = max3(mx[2], mx[3], mx[0]);
+        const float most = max3(mx[1], mx[2], mx[2]), top = fmaf(most, f, lv);
+        // the row sees a NaN (the sum keeps it)
+        if (most != -INFINITY && (odd || !(top < INFINITY))) l = __uint_as_float(0x7fc00000u);
         const bool move = top > ref + (ref == kUnset ? 0.f : kHeadroom);
         if (__any_sync(0xffffffffu, move)) {
           const float now = move ? top : ref, shrink = exp2_approx(ref - now);
