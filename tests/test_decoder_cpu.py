@@ -127,6 +127,8 @@ def test_rope_refusals():
     bad = torch.zeros(4, 2, 68, dtype=BF)[..., :64]
     assert call(Q=bad) == -8
     assert call(Q=q[:0], Qo=q[:0], P=pos[:0]) == 0
+    assert call(K=q, Ko=q) == -6  # one tensor as q and k, in place
+    assert call(Qo=torch.zeros(1, 2, 64, dtype=BF).expand(4, 2, 64)) == -6 and call(Qo=torch.zeros(4, 1, 64, dtype=BF).expand(4, 2, 64)) == -6
     with pytest.raises(RuntimeError, match="CUDA tensors only"):
         tg.apply_rope(q, None, pos, f)
 
@@ -172,6 +174,8 @@ def test_cache_and_attention_refusals():
     assert attend(Q=wide, O=wide) == -6  # 65 query heads on a cache head
     assert attend(n=0) == -6 and attend(window=-1) == -6 and attend(sinks=-1, window=4) == -6 and attend(sinks=2) == -6
     assert attend(scale=0.0) == -6 and attend(scale=float("nan")) == -6 and attend(scale=float("inf")) == -6
+    assert attend(O=q[:1].expand(2, 8, 64)) == -6 and attend(O=q[:, :1].expand(2, 8, 64)) == -6
+    assert attend(O=torch.zeros(5, 8, 64, dtype=BF).as_strided((2, 8, 64), (256, 64, 1))) == -6  # rows that reach into the next
     assert attend(Q=q[:1], O=q[:1]) == -6 and attend(Q=q[:0], O=q[:0], C=cu) == 0
     assert read(K=torch.zeros(2, 5, 2, 64)) == -2 and read(V=torch.zeros(2, 4, 2, 64, dtype=BF)) == -6
     with pytest.raises(RuntimeError, match="CUDA tensors only"):
@@ -187,3 +191,26 @@ def test_operators_have_no_backward():
     with torch.no_grad():
         ops._no_grad_inputs(x)
     ops._no_grad_inputs(x.detach(), None)
+
+
+def test_layer_refusals():
+    """What a layer has beside the projections that FP8DecoderLayer knows is refused before anything is quantised."""
+    nn = torch.nn
+
+    def layer(**change):
+        m = nn.Module()
+        m.self_attn, m.mlp = nn.Module(), nn.Module()
+        m.mlp.act_fn = nn.SiLU()
+        m.self_attn.scaling = 64**-0.5
+        for name, value in change.items():
+            owner, name = (m.self_attn, name[4:]) if name.startswith("att_") else (m.mlp, name[4:]) if name.startswith("mlp_") else (m, name)
+            setattr(owner, name, value)
+        return m
+
+    f = torch.ones(32, dtype=torch.float64)
+    for change in ({"att_q_norm": nn.LayerNorm(64)}, {"att_scaling": 0.2}, {"att_sinks": nn.Parameter(torch.zeros(8))}, {"mlp_act_fn": nn.GELU()},
+                   {"pre_feedforward_layernorm": nn.LayerNorm(64)}, {"att_attn_logit_softcapping": 50.0}):
+        with pytest.raises(NotImplementedError):
+            tg.FP8DecoderLayer.from_layer(layer(**change), 64, f)
+    with pytest.raises(AttributeError):  # an ordinary one gets as far as its projections
+        tg.FP8DecoderLayer.from_layer(layer(), 64, f)

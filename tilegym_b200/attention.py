@@ -21,13 +21,14 @@ from . import _lib, ops
 
 PAGE_TOKENS = 128  # tokens of a cache page, and of a scale
 
+_INT_MAX = 2**31 - 1
 _FP8 = torch.float8_e4m3fn
 _16BIT = (torch.bfloat16, torch.float16)
 
 
 class FP8KVCache(NamedTuple):
     """k [pages, kv_heads, 128, head_dim] and v [pages, kv_heads, head_dim, 128] (values lie [dim][token]) in
-    float8_e4m3fn, k_scale / v_scale [pages, kv_heads] fp32.  A value is its byte times its block's scale."""
+    float8_e4m3fn, k_scale / v_scale [pages, kv_heads] fp32, positive.  A value is its byte times its block's scale."""
 
     k: torch.Tensor
     v: torch.Tensor
@@ -292,11 +293,13 @@ def paged_attention(
     if q.dim() != 3:
         raise _lib.TileGymB200Error(-6, "q must be [tokens, heads, head_dim]")
     tokens, heads, dim = q.shape
-    max_q_len = int(max_q_len) if max_q_len is not None else 1 if cu_seqlens is None else max(tokens, 1)
+    bound = 1 if cu_seqlens is None else max(tokens, 1)
+    max_q_len = bound if max_q_len is None else min(int(max_q_len), bound)
+    window, sinks = min(int(window), _INT_MAX), min(int(sinks), _INT_MAX)  # beyond any position they mean the same
     need = _workspace_bytes(heads, cache.k.shape[1], dim, max_q_len, dev)
     scale = dim ** -0.5 if scale is None else float(scale)
     if _lib.fast is not None:
-        result = _lib.fast.paged_attention(q, *cache, block_table, seq_lens, cu_seqlens, max_q_len, scale, int(window), int(sinks), out, need)
+        result = _lib.fast.paged_attention(q, *cache, block_table, seq_lens, cu_seqlens, max_q_len, scale, window, sinks, out, need)
         if result is not None:
             return result if out is None else out
     ops._no_grad_inputs(q)
@@ -312,7 +315,7 @@ def paged_attention(
     desc = _lib.desc
     rc = _lib.lib().tg_paged_attention(
         out_desc, q_desc, desc(cache.k), desc(cache.v), desc(cache.k_scale), desc(cache.v_scale), desc(block_table), desc(seq_lens),
-        desc(cu_seqlens), max_q_len, scale, int(window), int(sinks),
+        desc(cu_seqlens), max_q_len, scale, window, sinks,
         0 if ws is None else ws.data_ptr(), need, dev, torch._C._cuda_getCurrentRawStream(dev),
     )
     _lib.check_rc(rc)

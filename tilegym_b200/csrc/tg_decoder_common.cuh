@@ -54,6 +54,24 @@ inline int32_t check_heads(const TgTensorDesc* t, const char* what, int64_t rows
   return TG_OK;
 }
 
+// The same for a tensor that is written: no element of it lies on another one.
+inline int32_t check_heads_out(const TgTensorDesc* t, const char* what, int64_t rows, int64_t heads, int64_t dim, int32_t dtype) {
+  const int32_t rc = check_heads(t, what, rows, heads, dim, dtype);
+  if (rc != TG_OK || rows < 1 || heads < 1) return rc;
+  int64_t n[2] = {rows, heads}, pitch[2] = {t->strides[0], t->strides[1]};
+  if (n[0] == 1 || (n[1] > 1 && pitch[0] > pitch[1])) {  // the smaller pitch, or the dimension of one, last
+    n[0] = heads, n[1] = rows;
+    pitch[0] = t->strides[1], pitch[1] = t->strides[0];
+  }
+  int64_t extent = dim;
+  for (int i = 0; i < 2; ++i) {
+    if (n[i] == 1) continue;
+    if (pitch[i] < extent) return api_fail(TG_ERR_ARGS, "a tensor that is written must not overlap itself");
+    extent += (n[i] - 1) * pitch[i];
+  }
+  return TG_OK;
+}
+
 inline int32_t check_dense_nd(const TgTensorDesc* t, const char* what, int32_t dtype, int nd, const int64_t* shape, unsigned align) {
   if (t == nullptr) return api_fail(TG_ERR_NULL, what);
   if (t->dtype != dtype) return api_fail(TG_ERR_DTYPE, what);

@@ -29,6 +29,23 @@ from .attention import FP8KVCache, kv_cache_write, paged_attention
 _FP8 = torch.float8_e4m3fn
 
 
+def _refuse_other_layers(layer: nn.Module, head_dim: int) -> None:
+    """Layers that compute something else with the same projections would come out wrong without a word."""
+    att, mlp = layer.self_attn, layer.mlp
+    for owner, names in ((att, ("q_norm", "k_norm", "sinks", "attn_logit_softcapping")),
+                         (layer, ("pre_feedforward_layernorm", "post_feedforward_layernorm"))):
+        for name in names:
+            if getattr(owner, name, None) is not None:
+                raise NotImplementedError(f"FP8DecoderLayer does not implement {name}")
+    scaling = getattr(att, "scaling", None)
+    if scaling is not None and abs(scaling * head_dim**0.5 - 1.0) > 1e-6:
+        raise NotImplementedError(f"FP8DecoderLayer scales scores by head_dim^-0.5, not by {scaling}")
+    act = getattr(mlp, "act_fn", None)
+    probe = torch.linspace(-4.0, 4.0, 9)
+    if act is not None and not torch.allclose(act(probe), nn.functional.silu(probe), atol=1e-6):
+        raise NotImplementedError("FP8DecoderLayer takes an MLP with silu")
+
+
 class FP8DecoderLayer(nn.Module):
     """Built by `from_layer` from a layer with `input_layernorm`, `self_attn.{q,k,v,o}_proj`, `post_attention_layernorm` and
     `mlp.{gate,up,down}_proj` (Llama, Mistral, Qwen2, ...).  Hidden and intermediate sizes must be multiples of 128,
@@ -71,6 +88,7 @@ class FP8DecoderLayer(nn.Module):
                    **kwargs) -> "FP8DecoderLayer":
         """Quantises a layer whose weights are on a CUDA device.  kwargs go to the constructor (window, sinks, ...)."""
         att, mlp = layer.self_attn, layer.mlp
+        _refuse_other_layers(layer, head_dim)
         parts = [att.q_proj, att.k_proj, att.v_proj]
         weights = {
             "norm1": layer.input_layernorm.weight, "norm2": layer.post_attention_layernorm.weight,
