@@ -408,10 +408,10 @@ TG_API int32_t tg_kv_cache_read(const TgTensorDesc* Ko, const TgTensorDesc* Vo, 
 /* Causal attention of the new tokens over the cache (which already holds them): Q, O [T, q_heads, D] bf16 / f16, q_heads a
  * multiple of the cache's heads (at most 64 times).  A token at position i sees j <= i, and under a window (> 0) of those
  * only j > i - window or j < sinks.  A token that sees nothing gets zeros.  max_q_len: no sequence has more new tokens than
- * this (rows beyond it are not computed).  workspace: at least tg_paged_attention_workspace_bytes() bytes, 16-byte
- * aligned, contents immaterial; calls that may overlap need one each. */
+ * this (rows beyond it are not computed).  workspace: at least tg_paged_attention_workspace_bytes() bytes (tokens: T, pages_per_seq: columns
+ * of block_table; may be 0), 16-byte aligned, contents immaterial; calls that may overlap need one each. */
 TG_API uint64_t tg_paged_attention_workspace_bytes(int64_t q_heads, int64_t kv_heads, int64_t head_dim, int32_t max_q_len,
-                                                   int32_t num_sms);
+                                                   int64_t tokens, int64_t seqs, int64_t pages_per_seq, int32_t num_sms);
 TG_API int32_t tg_paged_attention(const TgTensorDesc* O, const TgTensorDesc* Q, const TgTensorDesc* Kc, const TgTensorDesc* Vc,
                                   const TgTensorDesc* Ks, const TgTensorDesc* Vs, const TgTensorDesc* block_table,
                                   const TgTensorDesc* seq_lens, const TgTensorDesc* cu_seqlens, int32_t max_q_len, float scale,

@@ -193,6 +193,20 @@ def test_operators_have_no_backward():
     ops._no_grad_inputs(x.detach(), None)
 
 
+def test_attention_workspace():
+    def size(heads, kv, dim, n, tokens, seqs, pages, sms=148):
+        return _lib.lib().tg_paged_attention_workspace_bytes(heads, kv, dim, n, tokens, seqs, pages, sms)
+
+    assert size(32, 8, 128, 1, 0, 0, 0) > 0 and size(32, 8, 128, 1, 5, 5, 9) == size(32, 8, 128, 1, 0, 0, 0)
+    assert size(32, 8, 128, 4096, 4096, 1, 4096) == 0  # blocks enough
+    # 100 tokens: two pairs of tiles and heads of 8, 16 blocks, nine to a block's pages; no more parts than pages in fours
+    assert size(32, 8, 128, 100, 100, 1, 400) == 16 * 9 * 256 * (128 * 4 + 8)
+    assert size(32, 8, 128, 100, 100, 1, 11) == 16 * 2 * 256 * (128 * 4 + 8)
+    assert size(32, 8, 128, 100, 100, 1, 7) == 0
+    assert size(1, 1, 64, 65, 65, 1, 1 << 20) == 32 * 256 * (64 * 4 + 8)
+    assert size(33, 8, 128, 1, 1, 1, 1) == 0 and size(0, 8, 128, 1, 1, 1, 1) == 0 and size(8, 0, 128, 1, 1, 1, 1) == 0
+
+
 def test_layer_refusals():
     """What a layer has beside the projections that FP8DecoderLayer knows is refused before anything is quantised."""
     nn = torch.nn

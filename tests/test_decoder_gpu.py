@@ -447,6 +447,46 @@ def test_attention_nan_keys_at_every_place_of_a_page(dev, n):
         assert bool(got.isnan().all()), t
 
 
+@pytest.mark.parametrize("heads,group,dim,dtype", [(1, 1, 64, BF), (2, 8, 128, BF), (3, 4, 128, HF), (1, 3, 64, HF)])
+@pytest.mark.parametrize("new,past", [([150], [4000]), ([130, 1, 0, 90], [1500, 600, 0, 5]), ([300], [0]), ([129], [385])])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (900, 5)])
+def test_attention_chunks_on_a_long_cache(dev, heads, group, dim, dtype, new, past, window, sinks):
+    """Few blocks for the device: several share the pages of their rows, and parts are joined."""
+    g = gen(27)
+    lens = [n + p for n, p in zip(new, past)]
+    table, ref = make_kv(lens, heads, dim, g)
+    q = torch.randn(sum(new), heads * group, dim, generator=g).to(dtype)
+    got = check_attention(dev, q, ref, table, lens, new, window=window, sinks=sinks)
+    # the same bits whenever it runs
+    again = check_attention(dev, q, ref, table, lens, new, window=window, sinks=sinks)
+    assert torch.equal(got, again)
+
+
+def test_attention_nan_reaches_over_parts(dev):
+    """A NaN in one part of the pages: of a key for the rows that see it, of a value for its element."""
+    g = gen(28)
+    n, length = 100, 2000
+    table, ref = make_kv([length], 1, 64, g)
+    q = torch.randn(n, 2, 64, generator=g).to(BF).to(dev)
+    cache = on(dev, ref)
+
+    def run(**change):
+        return tg.paged_attention(q, cache._replace(**change), table.to(dev), i32([length]).to(dev), i32([0, n]).to(dev), max_q_len=n)
+
+    good = run()
+    for at in (0, 700, 1500, 1950):
+        see = (torch.arange(length - n, length) >= at).to(dev)
+        k, v = cache.k.clone(), cache.v.clone()
+        k.view(torch.uint8)[int(table[0, at // 128]), 0, at % 128, 5] = 127
+        v.view(torch.uint8)[int(table[0, at // 128]), 0, 9, at % 128] = 255
+        bad = run(k=k)
+        assert bool(bad[see].isnan().all()) and torch.equal(bad[~see], good[~see])
+        bad = run(v=v)
+        assert bool(bad[see][:, :, 9].isnan().all())
+        bad[..., 9] = good[..., 9]
+        assert torch.equal(bad, good)
+
+
 @pytest.mark.parametrize("n", [6, 150])
 def test_attention_factors_that_are_no_numbers(dev, n):
     """A row of q with a NaN, a page whose scale is one or infinite: only rows that see something of it lose their answer."""

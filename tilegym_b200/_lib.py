@@ -169,7 +169,7 @@ SIGNATURES = {
     ),
     "tg_kv_cache_read": (ctypes.c_int32, [_P] * 8 + [ctypes.c_int32, ctypes.c_uint64]),
     "tg_paged_attention_workspace_bytes": (
-        ctypes.c_uint64, [ctypes.c_int64] * 3 + [ctypes.c_int32, ctypes.c_int32],
+        ctypes.c_uint64, [ctypes.c_int64] * 3 + [ctypes.c_int32] + [ctypes.c_int64] * 3 + [ctypes.c_int32],
     ),
     "tg_paged_attention": (
         ctypes.c_int32,

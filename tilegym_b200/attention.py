@@ -296,7 +296,12 @@ def paged_attention(
     bound = 1 if cu_seqlens is None else max(tokens, 1)
     max_q_len = bound if max_q_len is None else min(int(max_q_len), bound)
     window, sinks = min(int(window), _INT_MAX), min(int(sinks), _INT_MAX)  # beyond any position they mean the same
-    need = _workspace_bytes(heads, cache.k.shape[1], dim, max_q_len, dev)
+    kv_heads = cache.k.shape[1]
+    if max_q_len * heads <= 64 * kv_heads:  # few rows: no more counts
+        need = _workspace_bytes(heads, kv_heads, dim, max_q_len, 0, 0, 0, dev)
+    else:
+        seqs = seq_lens.numel()
+        need = _workspace_bytes(heads, kv_heads, dim, max_q_len, tokens, seqs, block_table.numel() // max(seqs, 1), dev)
     scale = dim ** -0.5 if scale is None else float(scale)
     if _lib.fast is not None:
         result = _lib.fast.paged_attention(q, *cache, block_table, seq_lens, cu_seqlens, max_q_len, scale, window, sinks, out, need)
@@ -322,7 +327,7 @@ def paged_attention(
     return out
 
 
-@functools.lru_cache(maxsize=256)
-def _workspace_bytes(heads: int, kv_heads: int, dim: int, max_q_len: int, dev: int) -> int:
+@functools.lru_cache(maxsize=1024)
+def _workspace_bytes(heads: int, kv_heads: int, dim: int, max_q_len: int, tokens: int, seqs: int, pages_per_seq: int, dev: int) -> int:
     sms = torch.cuda.get_device_properties(dev).multi_processor_count
-    return _lib.lib().tg_paged_attention_workspace_bytes(heads, kv_heads, dim, int(max_q_len), sms)
+    return _lib.lib().tg_paged_attention_workspace_bytes(heads, kv_heads, dim, max_q_len, tokens, seqs, pages_per_seq, sms)

@@ -18,10 +18,16 @@ static int few_rows_of(int64_t q_heads, int64_t kv_heads, int32_t max_q_len) {
 }
 
 extern "C" TG_API uint64_t tg_paged_attention_workspace_bytes(int64_t q_heads, int64_t kv_heads, int64_t head_dim,
-                                                              int32_t max_q_len, int32_t num_sms) {
+                                                              int32_t max_q_len, int64_t tokens, int64_t seqs, int64_t pages_per_seq,
+                                                              int32_t num_sms) {
+  if (q_heads < 1 || kv_heads < 1 || q_heads % kv_heads != 0 || q_heads / kv_heads > 64 || max_q_len < 1) return 0;
   const int rows = few_rows_of(q_heads, kv_heads, max_q_len);
-  if (rows == 0) return 0;
   const int dim = head_dim == 64 ? 64 : 128;
+  if (rows == 0) {
+    if (tokens < 1 || seqs < 1 || tokens > (1 << 28) || seqs > (1 << 20)) return 0;
+    const int group = static_cast<int>(q_heads / kv_heads);
+    return many_rows_workspace(dim, many_rows_tiles(tokens, seqs, group) * kv_heads, many_rows_splits(tokens, seqs, kv_heads, group, pages_per_seq, num_sms));
+  }
   // the larger of the two types' block counts
   return few_rows_workspace(dim, rows, few_rows_blocks(dim, rows, true, num_sms));
 }
@@ -92,6 +98,15 @@ extern "C" TG_API int32_t tg_paged_attention(const TgTensorDesc* O, const TgTens
     char msg[160];
     snprintf(msg, sizeof(msg), "paged_attention launch failed: %s", cudaGetErrorString(e));
     return api_fail(TG_ERR_LAUNCH, msg);
+  }
+  p.splits = many_rows_splits(T, p.c.seqs, p.c.heads, p.group, p.c.max_pages, num_sms);
+  if (p.splits > 1) {
+    const int64_t blocks = many_rows_tiles(T, p.c.seqs, p.group) * p.c.heads;
+    if (workspace == 0) return api_fail(TG_ERR_NULL, "the workspace is null");
+    if (workspace & 15u) return api_fail(TG_ERR_ALIGN, "the workspace must be 16-byte aligned");
+    if (workspace_bytes < many_rows_workspace(p.c.dim, blocks, p.splits)) return api_fail(TG_ERR_ARGS, "the workspace is too small");
+    p.part_o = reinterpret_cast<float*>(workspace);
+    p.part_ml = reinterpret_cast<float2*>(workspace + 256ull * blocks * p.splits * p.c.dim * 4);
   }
   const cudaError_t e = launch_attention_many_rows(tmK, tmV, p, Q->dtype == TG_BF16, st);
   if (e != cudaSuccess) {

@@ -13,6 +13,8 @@
 // each, P taking the place of the S it came from, so that the next scores are there when a softmax is done with the last
 // and the tensor core never waits for one tile alone.  `ref` is a running maximum that
 // moves only when a p would exceed 2^14 (f16 has room for that), which is when O is rescaled in TMEM.
+// Few blocks (a chunk of a prompt on a long cache, few heads) leave most SMs idle: there `splits` blocks share a block's pages,
+// each at least kMinPages, and a joining kernel adds their parts in order.
 // Warp 0 copies pages, warps 1 and 2 issue the tiles' score products and warp 3 the value products (a warp that issues is
 // held up until the tensor core has nearly caught up and then needs a few hundred clocks to find its next barriers ready:
 // with one warp for all the tensor core was idle 60 % of the time, with two 45 %), warps 4-7 convert values, warps 8-11 and 12-15 are the tiles' softmax.
@@ -27,6 +29,7 @@ constexpr int kThreads = 512;
 constexpr int kRegsLaunch = 128, kRegsOther = 72, kRegsSoftmax = 184;
 constexpr int kHalf = kPage / 2;  // tokens of a step
 constexpr int kPoly = 5;
+constexpr int kMinPages = 4;  // of a part: joining takes as long as three or four pages
 constexpr float kUnset = -1e30f;  // the reference of a row that has not seen a token yet
 constexpr float kHeadroom = 14.f;  // p may reach 2^14 before ref moves (f16 ends at 2^16)
 
@@ -101,7 +104,10 @@ __device__ __forceinline__ float2 exp2_pair(float2 x) {
   return r;
 }
 
-template <typename T, int DIM>
+// Parts that the pages of 256 rows are divided into.
+__device__ __forceinline__ int parts_of(const AttentionParams& p, const SeqView& v) { return max(min(p.splits, v.tiles / kMinPages), 1); }
+
+template <typename T, int DIM, bool kSplit>
 __global__ void __launch_bounds__(kThreads, 1)
     tg_attention_many_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                                   const __grid_constant__ AttentionParams p, int token_tiles, int tile_tokens) {
@@ -158,8 +164,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   griddep_wait();
   griddep_launch_dependents();
   // later tokens see more: their blocks come first
-  const int head = blockIdx.x % p.c.heads;
-  const int tile = token_tiles - 1 - blockIdx.x / p.c.heads;
+  const int whole_block = kSplit ? blockIdx.x / p.splits : blockIdx.x, split = kSplit ? blockIdx.x - whole_block * p.splits : 0;
+  const int head = whole_block % p.c.heads;
+  const int tile = token_tiles - 1 - whole_block / p.c.heads;
   int first;
   const int b = find_sequence(p.c.cu, p.c.seqs, tile, 2 * tile_tokens, 1, first);
   SeqView v = {};
@@ -168,7 +175,10 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  const int pages = v.n > 0 ? v.tiles : 0;
+  // this block's part of the pages, from number t0 on
+  const int parts = kSplit ? parts_of(p, v) : 1;
+  const int t0 = kSplit && split < parts ? static_cast<int>(static_cast<int64_t>(v.tiles) * split / parts) : 0;
+  const int pages = v.n <= 0 || split >= parts ? 0 : kSplit ? static_cast<int>(static_cast<int64_t>(v.tiles) * (split + 1) / parts) - t0 : v.tiles;
   const int tiles = v.n > tile_tokens ? 2 : 1;  // that have rows
   bool ok = true;
   int site = 0;
@@ -184,7 +194,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int rows_k = p.c.pages * p.c.heads * kPage, rows_v = p.c.pages * p.c.heads * DIM;
     int issued = 0;
     for (int base = 0; base < pages && ok; base += 32) {
-      const int page = base + lane < pages ? v.page_of(base + lane) : p.c.max_pages;
+      const int page = base + lane < pages ? v.page_of(t0 + base + lane) : p.c.max_pages;
       int phys = page < p.c.max_pages ? p.c.table[b * p.c.table_pitch + page] : -1;
       if (phys < 0 || phys >= p.c.pages) phys = -1;
       for (int i = 0; i < min(32, pages - base); ++i, ++issued) {
@@ -321,7 +331,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         uint32_t ww[4] = {w.x, w.y, w.z, w.w};
         if ((nan_bytes(w.x) | nan_bytes(w.y) | nan_bytes(w.z) | nan_bytes(w.w)) != 0) {
           // a NaN becomes zero here, and is of interest only where some row sees the token
-          const int at = v.page_of(j) * kPage + c * 16;
+          const int at = v.page_of(t0 + j) * kPage + c * 16;
 #pragma unroll
           for (int x = 0; x < 16; ++x)
             if (((ww[x >> 2] >> (8 * (x & 3))) & 127u) == 127u && at + x < min(v.len, v.pos0 + v.n) &&
@@ -429,7 +439,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int row_lo = p.window > 0 ? static_cast<int>(max(static_cast<int64_t>(pos) - p.window + 1, int64_t(0))) : 0;
     // page numbers two pages ahead, scales one: nothing here waits for a load that it has just issued
     auto page_entry = [&](int j) {
-      const int page = j < pages ? v.page_of(j) : p.c.max_pages;
+      const int page = j < pages ? v.page_of(t0 + j) : p.c.max_pages;
       return page < p.c.max_pages ? p.c.table[b * p.c.table_pitch + page] : -1;
     };
     auto scales = [&](int phys, float& ks, float& vs) {
@@ -464,7 +474,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
 #pragma unroll 1
       for (int half = 0; half < 2; ++half) {
-        const int base = v.page_of(j) * kPage + half * kHalf;
+        const int base = v.page_of(t0 + j) * kPage + half * kHalf;
         const bool whole = here && base + kHalf <= all_hi && (base >= all_lo || base + kHalf <= p.sinks);
         const uint32_t t_s = t_s0 + half * kHalf;
         if (!warp_wait(b_sfull + 16 * w + 8 * half, j & 1, abort_flag)) {
@@ -560,7 +570,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       uint32_t bad[4] = {0, 0, 0, 0};
       if (*reinterpret_cast<volatile uint32_t*>(nan_flag) != 0) {
         for (int j = 0; j < pages; ++j) {
-          const int ph = page_entry(j), base = v.page_of(j) * kPage;
+          const int ph = page_entry(j), base = v.page_of(t0 + j) * kPage;
           if (ph < 0 || ph >= p.c.pages) continue;
           const uint8_t* src = p.c.v + (static_cast<int64_t>(ph) * p.c.heads + head) * (kPage * DIM);
           for (int u = 0; u < DIM * 8; ++u) {
@@ -579,6 +589,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         __syncwarp();
       }
       const float inv = l == 0.f ? 0.f : 1.0f / l;
+      const int64_t slot = static_cast<int64_t>(blockIdx.x) * 256 + w * 128 + row;
+      if (kSplit && parts > 1) p.part_ml[slot] = make_float2(ref, l);
       T* out = static_cast<T*>(p.o) + static_cast<int64_t>(v.lo + i) * p.o_tok + (head * p.group + g) * p.o_head;
 #pragma unroll 1
       for (int c = 0; c < DIM; c += 32) {
@@ -591,7 +603,12 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int k = 0; k < 32; ++k)
             if ((nan >> k) & 1u) o[k] = 0x7fc00000u;
         }
-        if (live) {
+        if (kSplit && parts > 1) {
+          float4* part = reinterpret_cast<float4*>(p.part_o + slot * DIM + c);
+#pragma unroll
+          for (int k = 0; k < 32; k += 4)
+            part[k / 4] = make_float4(__uint_as_float(o[k]), __uint_as_float(o[k + 1]), __uint_as_float(o[k + 2]), __uint_as_float(o[k + 3]));
+        } else if (live) {
 #pragma unroll
           for (int k = 0; k < 32; k += 8) {
             uint32_t r[4];
@@ -615,11 +632,54 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
+// Adds the parts of a block in order: a warp per row, a lane DIM / 32 elements.
 template <typename T, int DIM>
-cudaError_t launch(const CUtensorMap& tmK, const CUtensorMap& tmV, const AttentionParams& p, cudaStream_t stream) {
+__global__ void __launch_bounds__(256) tg_attention_join_parts_kernel(const __grid_constant__ AttentionParams p, int token_tiles, int tile_tokens) {
+  griddep_wait();
+  griddep_launch_dependents();
+  constexpr int E = DIM / 32;
+  const int lane = threadIdx.x & 31, row = blockIdx.y * 8 + (threadIdx.x >> 5);  // of 256
+  const int head = blockIdx.x % p.c.heads, tile = token_tiles - 1 - blockIdx.x / p.c.heads;
+  int first;
+  const int b = find_sequence(p.c.cu, p.c.seqs, tile, 2 * tile_tokens, 1, first);
+  if (tile < first) return;
+  const SeqView v = view_sequence(p, b, (tile - first) * 2 * tile_tokens, 2 * tile_tokens);
+  const int parts = parts_of(p, v), r = row & 127;
+  const int i = (row >> 7) * tile_tokens + r / p.group, g = r % p.group;
+  if (parts == 1 || r >= tile_tokens * p.group || i >= v.n) return;
+  const int64_t slot0 = static_cast<int64_t>(blockIdx.x) * p.splits * 256 + row;
+  const float2 ml = lane < parts ? p.part_ml[slot0 + lane * 256] : make_float2(kUnset, 0.f);
+  const float f = exp2f(ml.x - redux_max(ml.x));
+  float l = ml.y * f;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+  float sum[E] = {};
+#pragma unroll 4
+  for (int k = 0; k < parts; ++k) {
+    const float fk = __shfl_sync(0xffffffffu, f, k);
+    const float* part = p.part_o + (slot0 + k * 256) * DIM + lane * E;
+    float x[E];
+    if constexpr (E == 4) {
+      const float4 y = *reinterpret_cast<const float4*>(part);
+      x[0] = y.x; x[1] = y.y; x[2] = y.z; x[3] = y.w;
+    } else {
+      const float2 y = *reinterpret_cast<const float2*>(part);
+      x[0] = y.x; x[1] = y.y;
+    }
+#pragma unroll
+    for (int e = 0; e < E; ++e) sum[e] = fmaf(x[e], fk, sum[e]);
+  }
+  T* out = static_cast<T*>(p.o) + static_cast<int64_t>(v.lo + i) * p.o_tok + (head * p.group + g) * p.o_head + lane * E;
+  const float inv = 1.0f / l;
+#pragma unroll
+  for (int e = 0; e < E; e += 2) *reinterpret_cast<uint32_t*>(out + e) = l == 0.f ? 0u : pack_pair<T>(sum[e] * inv, sum[e + 1] * inv);
+}
+
+template <typename T, int DIM, bool kSplit>
+cudaError_t launch_split(const CUtensorMap& tmK, const CUtensorMap& tmV, const AttentionParams& p, cudaStream_t stream) {
   constexpr int kTerms = std::is_same<T, __half>::value ? 3 : 2;
   using Sh = Shape<DIM, kTerms>;
-  auto kernel = tg_attention_many_rows_kernel<T, DIM>;
+  auto kernel = tg_attention_many_rows_kernel<T, DIM, kSplit>;
   static bool set[64] = {};
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
@@ -629,14 +689,32 @@ cudaError_t launch(const CUtensorMap& tmK, const CUtensorMap& tmV, const Attenti
     if (e != cudaSuccess) return e;
     set[dev & 63] = true;
   }
-  const int tile_tokens = 128 / p.group;
-  const int64_t token_tiles = p.tokens / (2 * tile_tokens) + static_cast<int64_t>(p.c.seqs);
-  if (token_tiles * p.c.heads > 0x7fffffff) return cudaErrorInvalidValue;
-  return launch_pdl(kernel, dim3(static_cast<unsigned>(token_tiles * p.c.heads)), dim3(kThreads), Sh::kSmem, stream, tmK, tmV, p,
-                    static_cast<int>(token_tiles), tile_tokens);
+  const int tile_tokens = 128 / p.group, token_tiles = static_cast<int>(many_rows_tiles(p.tokens, p.c.seqs, p.group));
+  const int64_t blocks = static_cast<int64_t>(token_tiles) * p.c.heads;
+  if (blocks * p.splits > 0x7fffffff) return cudaErrorInvalidValue;
+  e = launch_pdl(kernel, dim3(static_cast<unsigned>(blocks * p.splits)), dim3(kThreads), Sh::kSmem, stream, tmK, tmV, p, token_tiles, tile_tokens);
+  if (e != cudaSuccess || !kSplit) return e;
+  return launch_pdl(tg_attention_join_parts_kernel<T, DIM>, dim3(static_cast<unsigned>(blocks), 256 / 8), dim3(256), 0, stream, p, token_tiles, tile_tokens);
+}
+
+template <typename T, int DIM>
+cudaError_t launch(const CUtensorMap& tmK, const CUtensorMap& tmV, const AttentionParams& p, cudaStream_t stream) {
+  return p.splits > 1 ? launch_split<T, DIM, true>(tmK, tmV, p, stream) : launch_split<T, DIM, false>(tmK, tmV, p, stream);
 }
 
 }  // namespace
+
+int64_t many_rows_tiles(int64_t tokens, int64_t seqs, int group) { return tokens / (2 * (128 / group)) + seqs; }
+
+// As many parts as there are SMs for.  100 tokens on 32000, 32 heads on 8: 86 us, undivided 542; 500 tokens on 4000, 8 heads
+// on 2: 33 and 88; 1000 tokens on 4000, 32 heads on 8, are 136 blocks and stay whole (99 us).
+int many_rows_splits(int64_t tokens, int64_t seqs, int64_t heads, int group, int64_t max_pages, int num_sms) {
+  const int64_t blocks = many_rows_tiles(tokens, seqs, group) * heads;
+  const int64_t most = max_pages / kMinPages < 32 ? max_pages / kMinPages : 32, fit = blocks > 0 ? num_sms / blocks : 1;
+  return static_cast<int>(fit < 2 || most < 2 ? 1 : fit < most ? fit : most);
+}
+
+uint64_t many_rows_workspace(int dim, int64_t blocks, int splits) { return splits == 1 ? 0 : 256ull * blocks * splits * (dim * 4 + 8); }
 
 cudaError_t launch_attention_many_rows(const CUtensorMap& tmK, const CUtensorMap& tmV, const AttentionParams& p, bool bf16,
                                        cudaStream_t stream) {

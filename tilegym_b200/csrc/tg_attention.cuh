@@ -13,9 +13,10 @@ struct AttentionParams {
   float scale;
   int32_t window, sinks;
   int32_t max_q_len;
-  // workspace of the kernel for few rows: partial results of tile ranges that begin or end inside a unit
-  float* part_o;    // [2 * blocks][rows][dim]
-  float2* part_ml;  // [2 * blocks][rows]: reference exponent, sum
+  int32_t splits;  // many rows: blocks that share the pages of 256 rows
+  // workspace: partial results; for few rows of ranges that begin or end inside a unit
+  float* part_o;    // few rows: [2 * blocks][rows][dim], many: [blocks][splits][256][dim]
+  float2* part_ml;  // the same without dim: reference exponent, sum
   int4* record;     // [blocks]: unit that a block leaves unfinished
   int32_t* status;
   uint32_t wait_limit_us;
@@ -29,6 +30,9 @@ uint64_t few_rows_workspace(int dim, int rows_padded, int blocks);
 cudaError_t launch_attention_few_rows(const CUtensorMap& tmK, const CUtensorMap& tmV, const AttentionParams& p, int rows_padded,
                                       int blocks, bool bf16, cudaStream_t stream);
 // Many rows: the products are what counts.
+int64_t many_rows_tiles(int64_t tokens, int64_t seqs, int group);  // pairs of tiles, at most, of all sequences
+int many_rows_splits(int64_t tokens, int64_t seqs, int64_t heads, int group, int64_t max_pages, int num_sms);
+uint64_t many_rows_workspace(int dim, int64_t blocks, int splits);
 cudaError_t launch_attention_many_rows(const CUtensorMap& tmK, const CUtensorMap& tmV, const AttentionParams& p, bool bf16,
                                        cudaStream_t stream);
 
