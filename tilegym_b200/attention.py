@@ -22,6 +22,7 @@ from . import _lib, ops
 PAGE_TOKENS = 128  # tokens of a cache page, and of a scale
 
 _INT_MAX = 2**31 - 1
+_FEW_ROWS = 32  # (new tokens, heads of a group) that the kernel for few rows takes
 _FP8 = torch.float8_e4m3fn
 _16BIT = (torch.bfloat16, torch.float16)
 
@@ -297,7 +298,7 @@ def paged_attention(
     max_q_len = bound if max_q_len is None else min(int(max_q_len), bound)
     window, sinks = min(int(window), _INT_MAX), min(int(sinks), _INT_MAX)  # beyond any position they mean the same
     kv_heads = cache.k.shape[1]
-    if max_q_len * heads <= 64 * kv_heads:  # few rows: no more counts
+    if max_q_len * heads <= _FEW_ROWS * kv_heads:  # nothing more counts
         need = _workspace_bytes(heads, kv_heads, dim, max_q_len, 0, 0, 0, dev)
     else:
         seqs = seq_lens.numel()

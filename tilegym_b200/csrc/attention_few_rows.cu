@@ -1,4 +1,4 @@
-// Attention over the paged e4m3 cache for few rows: R = (new tokens of a sequence) * (query heads of a cache head) <= 64.
+// Attention over the paged e4m3 cache for few rows: R = (new tokens of a sequence) * (query heads of a cache head) <= 32.
 //
 // The cache's bytes are read once and are nearly all of the work, so the kernel is built to keep copies in flight, and the
 // cached bytes ARE the tensor core's operands: no conversion, no transposition.
@@ -10,8 +10,7 @@
 // The two factors that are not in the cache are split into e4m3 terms, each holding what the one before left: two hold a
 // bf16 q exactly and p to 2^-8, three (f16) both to 2^-12.  The terms are kept 16 times larger each (which moves the end of
 // e4m3's range out of reach) and stand side by side as rows of the operand, so a page is read once for all of them; their
-// columns of S^T and O^T are joined by the softmax and at the end.  (With 64 rows TMEM has no room for that: there the
-// accumulator sums q's terms, unscaled.)  `ref` is a running maximum of the exponent that is only moved when a p would leave the format (2^5 of
+// columns of S^T and O^T are joined by the softmax and at the end.  `ref` is a running maximum of the exponent that is only moved when a p would leave the format (2^5 of
 // headroom), which rescales O^T in TMEM.  Keeping v_scale in the exponent keeps p at one magnitude whatever the pages'
 // scales are.
 //
@@ -49,15 +48,14 @@ struct Shape {
   static constexpr int kUnitCost = kGroups == 1 ? 4 : 6;
   // barriers and notes; row factors; references; maxima and sums; rows that see a NaN
   static constexpr int kRowmul = 1024, kRef = kRowmul + N * 4, kWmax = kRef + kGroups * 2 * N * 4, kNan = kWmax + kGroups * 2 * 4 * N * 4;
-  static constexpr int kMisc = kNan + (kGroups == 2 ? 2 * 128 * 8 : 0);
+  static constexpr int kMisc = kNan + (kGroups == 2 ? 2 * 128 * 4 : 0);
   // dim 64: the value operand is read as 128 rows, 64 of them whatever follows the page
   static constexpr int kBudget = (kBlocksPerSm == 2 ? 113 : 226) * 1024 - 1024 - 2 * kP - kQ - kMisc;
   static constexpr int kStages = kBudget / (2 * kTile) > 8 ? 8 : kBudget / (2 * kTile);
   static constexpr int kSmem = 1024 + kStages * 2 * kTile + 2 * kP + kQ + kMisc;
-  static constexpr bool kStack = N <= 32;  // q's terms have columns of their own in S^T
-  static constexpr int kSCols = kStack ? TERMS * N : N;
+  static constexpr int kSCols = TERMS * N;  // q's terms have columns of their own in S^T
   static constexpr int kTmemUsed = 2 * kSCols + kGroups * TERMS * N;  // S^T twice and each group's O^T by term
-  static constexpr int kTmem = kTmemUsed <= 64 ? 64 : kTmemUsed <= 128 ? 128 : kTmemUsed <= 256 ? 256 : 512;
+  static constexpr int kTmem = kTmemUsed <= 128 ? 128 : kTmemUsed <= 256 ? 256 : 512;
   static_assert(kStages >= 3, "the ring is too short to hide the latency of a page");
   static_assert(2 * kP + kQ >= 8192, "the value operand of dim 64 reads 8 KB behind its page");
 };
@@ -114,7 +112,7 @@ __device__ __forceinline__ bool next_unit(const AttentionParams& p, Cursor& c) {
 // One element's row of a value page (128 tokens) of which not every row sees every token.  Values that nobody sees are
 // whatever memory held, NaN among it, and 0 * NaN is NaN: they become zeros.  A NaN that some rows see is kept from the
 // product, which would give it to all, and noted for those rows.
-__device__ __noinline__ void clean_values(const AttentionParams& p, const SeqView& v, int base, uint8_t* row, int d, uint64_t& nan_rows) {
+__device__ __noinline__ void clean_values(const AttentionParams& p, const SeqView& v, int base, uint8_t* row, int d, uint32_t& nan_rows) {
   // tokens of the page that some row sees: t < hi and (t >= lo or t < sink)
   const int hi = base >= 0 ? min(max(min(v.len, v.pos0 + v.n) - base, 0), kPage) : 0;
   const int lo = p.window > 0 ? static_cast<int>(min(max(static_cast<int64_t>(v.pos0) - p.window + 1 - base, int64_t(0)), int64_t(kPage))) : 0;
@@ -147,7 +145,7 @@ __device__ __noinline__ void clean_values(const AttentionParams& p, const SeqVie
         rows_that_see(p, v, base + t + x, true, a, z);
         a *= p.group;
         z *= p.group;
-        if (a < z) nan_rows |= (z >= 64 ? ~uint64_t(0) : (uint64_t(1) << z) - 1) & ~((uint64_t(1) << a) - 1);
+        if (a < z) nan_rows |= (z >= 32 ? ~0u : (1u << z) - 1) & ~((1u << a) - 1);
         const uint32_t keep = ~(255u << (8 * (x & 3)));
         if (x < 4) ww[0] &= keep;
         else if (x < 8) ww[1] &= keep;
@@ -404,12 +402,9 @@ __global__ void __launch_bounds__((Shape<DIM, N, kTermsOf<T>>::kThreads), (Shape
         tc_fence_after();
         if (elect_one()) {
           const uint64_t a = rows_desc<DIM>(smem_u32(smem + stage * 2 * Sh::kTile));
+          const uint64_t b = rows_desc<DIM>(q_addr);
 #pragma unroll
-          for (int term = 0; term < (Sh::kStack ? 1 : kTerms); ++term) {
-            const uint64_t b = rows_desc<DIM>(q_addr + term * N * DIM);
-#pragma unroll
-            for (int k = 0; k < DIM / 32; ++k) mma_f8f6f4(tmem + buf * Sh::kSCols, a + 2 * k, b + 2 * k, idesc, term + k > 0);
-          }
+          for (int k = 0; k < DIM / 32; ++k) mma_f8f6f4(tmem + buf * Sh::kSCols, a + 2 * k, b + 2 * k, idesc, k > 0);
           tc_commit(b_sfull + 8 * buf);
         }
         __syncwarp();
@@ -461,7 +456,7 @@ __global__ void __launch_bounds__((Shape<DIM, N, kTermsOf<T>>::kThreads), (Shape
     float* maxima = reinterpret_cast<float*>(misc + Sh::kWmax);       // [group][copy][4][N]: the warps' maxima, or sums, by row
     float* wmax = maxima + group * 8 * N;
     int2* side_notes = reinterpret_cast<int2*>(misc + 960);           // [group]: which copies hold its sums and references
-    uint64_t* nan_notes = reinterpret_cast<uint64_t*>(misc + Sh::kNan);  // [group][element of the head]
+    uint32_t* nan_notes = reinterpret_cast<uint32_t*>(misc + Sh::kNan);  // [group][element of the head]
     auto vote = [&](bool mine) { return softmax_vote(1 + group, 128, mine); };
     auto vote_all = [&](bool mine) { return softmax_vote(kGroups == 2 ? 3 : 1, 128 * kGroups, mine); };
     int it = 0, turn = 0;
@@ -513,7 +508,7 @@ __global__ void __launch_bounds__((Shape<DIM, N, kTermsOf<T>>::kThreads), (Shape
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
               uint32_t term[kTerms];
-              split_e4m3<kTerms>(f[2 * j] * inv, f[2 * j + 1] * inv, Sh::kStack ? kTermStep : 1.f, term);
+              split_e4m3<kTerms>(f[2 * j] * inv, f[2 * j + 1] * inv, kTermStep, term);
 #pragma unroll
               for (int x = 0; x < kTerms; ++x) out[x][j >> 1] = (j & 1) ? out[x][j >> 1] | (term[x] << 16) : term[x];
             }
@@ -536,7 +531,7 @@ __global__ void __launch_bounds__((Shape<DIM, N, kTermsOf<T>>::kThreads), (Shape
       }
 #pragma unroll
       for (int r = 0; r < N; ++r) l[r] = 0.f;
-      uint64_t nan_rows = 0;  // rows that see a NaN in element `token` of a value
+      uint32_t nan_rows = 0;  // rows that see a NaN in element `token` of a value
       // positions that every row sees: [all_lo, all_hi), and the first tokens
       const int all_hi = min(v.len, v.pos0 + 1);
       const int all_lo = p.window > 0 ? static_cast<int>(max(static_cast<int64_t>(v.pos0) + v.n - p.window, int64_t(0))) : 0;
@@ -564,17 +559,16 @@ __global__ void __launch_bounds__((Shape<DIM, N, kTermsOf<T>>::kThreads), (Shape
 #pragma unroll
           for (int c = 0; c < N; c += 16) {
             if (c >= rows) break;
-            constexpr int kParts = Sh::kStack ? kTerms : 1;
-            uint32_t part[kParts][16];
+            uint32_t part[kTerms][16];
 #pragma unroll
-            for (int x = 0; x < kParts; ++x) tmem_ld_32x16(t_s + x * N + c, part[x]);
+            for (int x = 0; x < kTerms; ++x) tmem_ld_32x16(t_s + x * N + c, part[x]);
             tmem_ld_wait();
             float s[16];
 #pragma unroll
             for (int j = 0; j < 16; ++j) {
-              s[j] = __uint_as_float(part[kParts - 1][j]);
+              s[j] = __uint_as_float(part[kTerms - 1][j]);
 #pragma unroll
-              for (int x = kParts - 2; x >= 0; --x) s[j] = fmaf(s[j], 1.f / kTermStep, __uint_as_float(part[x][j]));
+              for (int x = kTerms - 2; x >= 0; --x) s[j] = fmaf(s[j], 1.f / kTermStep, __uint_as_float(part[x][j]));
             }
 #pragma unroll
             for (int g = 0; g < 16; g += 8) {
@@ -916,14 +910,12 @@ cudaError_t launch_n(const CUtensorMap& tmK, const CUtensorMap& tmV, const Atten
 
 template <typename T, int DIM>
 cudaError_t launch_rows(const CUtensorMap& tmK, const CUtensorMap& tmV, const AttentionParams& p, int n, int blocks, cudaStream_t stream) {
-  if (n == 16) return launch_n<T, DIM, 16>(tmK, tmV, p, blocks, stream);
-  if (n == 32) return launch_n<T, DIM, 32>(tmK, tmV, p, blocks, stream);
-  return launch_n<T, DIM, 64>(tmK, tmV, p, blocks, stream);
+  return n == 16 ? launch_n<T, DIM, 16>(tmK, tmV, p, blocks, stream) : launch_n<T, DIM, 32>(tmK, tmV, p, blocks, stream);
 }
 
 }  // namespace
 
-int few_rows_padded(int rows) { return rows <= 16 ? 16 : rows <= 32 ? 32 : 64; }
+int few_rows_padded(int rows) { return rows <= 16 ? 16 : 32; }
 
 int few_rows_blocks(int dim, int rows_padded, bool bf16, int num_sms) {
   static_assert(Shape<128, 16, 2>::kBlocksPerSm == 2 && Shape<64, 16, 3>::kBlocksPerSm == 2 && Shape<128, 16, 3>::kBlocksPerSm == 1 &&
