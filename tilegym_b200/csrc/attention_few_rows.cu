@@ -21,6 +21,11 @@
 // Warp 0 copies pages (TMA, a ring of page pairs), warps 1 and 2 issue the two products, warps 3-6 do the softmax.  Where the shared
 // memory holds one block per SM only, four more warps share it: the two groups take pages in turn, each with references,
 // sums and an O^T of its own, which are joined when the unit ends (the softmax of 32 rows takes longer than copying the page).
+//
+// Bound: HBM up to 16 rows, the chain of the softmax from there.  Measured (8 cache heads of 128, bf16): 64 sequences of up to
+// 16000 tokens with 4 rows 172 us (1.1 GB, 0.97 of the copy bandwidth); 37 sequences of 8000 with 32 rows 162 us (0.57); one
+// sequence of 2001 tokens 12.6 us, of 32000 25 us.  Of 64 sequences of up to 8000 tokens (f16), equal shares counted in pages alone
+// took 164 us, with what units cost counted in 103.
 #include <cstdio>
 
 #include "tg_attention.cuh"

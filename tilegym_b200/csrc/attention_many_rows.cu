@@ -6,7 +6,7 @@
 //   S [128 rows, 128 tokens] = Q . K^T      kind::f8f6f4 on the cached bytes, q split into e4m3 terms (bf16: two hold it
 //                                           exactly) that the accumulator sums: the time of one 16-bit product, no conversion of K
 //   p = 2^(S * scale * log2 e + log2 v_scale - ref)   thread = row: no exchange between threads at all
-//   O [128 rows, dim]       += P . V        kind::f16: P in f16 from TMEM, V converted e4m3 -> f16 (exact) by two warps once
+//   O [128 rows, dim]       += P . V        kind::f16: P in f16 from TMEM, V converted e4m3 -> f16 (exact) by four warps once
 //                                           per page for both tiles
 //
 // The work goes by half pages (64 tokens): TMEM holds O of both tiles (2 x 128 columns) and two S buffers of 64 columns for
@@ -18,6 +18,10 @@
 // Warp 0 copies pages, warps 1 and 2 issue the tiles' score products and warp 3 the value products (a warp that issues is
 // held up until the tensor core has nearly caught up and then needs a few hundred clocks to find its next barriers ready:
 // with one warp for all the tensor core was idle 60 % of the time, with two 45 %), warps 4-7 convert values, warps 8-11 and 12-15 are the tiles' softmax.
+//
+// Bound: the chain scores -> softmax -> product of a half page (about 1700 clocks for both tiles; the products need 1250, the
+// exponentials 1024).  Measured (bf16, 32 heads on 8 of 128): 4 prompts of 300-2500 tokens on up to 5000 cached 245 us
+// (780 TFLOP/s of 1631 measured for a 16-bit GEMM; 351 with whole pages and one issuing warp), one of 4096 172 us.
 #include <cstdio>
 
 #include "tg_attention.cuh"
