@@ -23,7 +23,7 @@
 // sums and an O^T of its own, which are joined when the unit ends (the softmax of 32 rows takes longer than copying the page).
 //
 // Bound: HBM up to 16 rows, the chain of the softmax from there.  Measured (8 cache heads of 128, bf16): 64 sequences of up to
-// 16000 tokens with 4 rows 172 us (1.1 GB, 0.97 of the copy bandwidth); 37 sequences of 8000 with 32 rows 162 us (0.57); one
+// 16000 tokens with 4 rows 172 us (1.1 GB, 0.97 of the copy bandwidth); 37 sequences of 8000 with 32 rows 153 us (0.61); one
 // sequence of 2001 tokens 12.6 us, of 32000 25 us.  Of 64 sequences of up to 8000 tokens (f16), equal shares counted in pages alone
 // took 164 us, with what units cost counted in 103.
 #include <cstdio>
@@ -42,7 +42,7 @@ constexpr int kTermsOf = std::is_same<T, __half>::value ? 3 : 2;
 template <int DIM, int N, int TERMS>
 struct Shape {
   static constexpr int kTile = DIM * kPage;  // bytes of a key or value page
-  static constexpr int kP = TERMS * N * kPage;
+  static constexpr int kP = (TERMS * N + 31) / 32 * 32 * kPage;  // planes of [token][32 columns]
   static constexpr int kQ = TERMS * N * DIM;
   // two blocks share an SM where each still has a ring of three page pairs
   static constexpr int kBlocksPerSm = N == 16 && !(TERMS == 3 && DIM == 128) ? 2 : 1;
@@ -69,6 +69,15 @@ struct TileInfo {
   float ks, lv, inv_vs;
   int base;  // position of the page's first token; -1: no such page
 };
+
+// The operand P [columns][tokens] with the columns together: planes of 32 columns (32 bytes per token, tokens one after the
+// other, the two halves changing places every four tokens: the 32-byte swizzle), 4 KB from one plane to the next and 256 bytes
+// from one group of eight tokens to the next.  A thread, which has a token, writes eight columns at once; with the tokens
+// together every byte was a store of its own (32 rows, f16, dim 64, 37 sequences of 8000: 163 us, 190 that way).
+__device__ __forceinline__ uint64_t columns_desc(uint32_t smem_addr) {
+  return static_cast<uint64_t>((smem_addr >> 4) & 0x3FFFu) | (static_cast<uint64_t>((32 * kPage) >> 4) << 16) | (static_cast<uint64_t>(256u >> 4) << 32) |
+         (1ull << 46) | (6ull << 61);
+}
 
 // A bounded wait whose outcome is the same for the whole warp, which is converged behind it.
 template <bool kHint = false>
@@ -419,7 +428,7 @@ __global__ void __launch_bounds__((Shape<DIM, N, kTermsOf<T>>::kThreads), (Shape
     if (!ok && lane == 0) *p.status = kRoleMma * 1000 + site;
   } else if (warp == 2) {
     // ------------------------------------------------------------------------------------------ values
-    constexpr uint32_t idesc = make_idesc_e4m3_f32(128, kTerms * N);
+    constexpr uint32_t idesc = make_idesc_e4m3_f32(128, kTerms * N) | (1u << 16);  // B lies with its columns together
     const uint32_t p_addr = smem_u32(p_smem);
     int it = 0;
     while (left > 0 && ok) {
@@ -434,11 +443,11 @@ __global__ void __launch_bounds__((Shape<DIM, N, kTermsOf<T>>::kThreads), (Shape
         tc_fence_after();
         if (elect_one()) {
           const uint64_t a = make_kmajor_sw128_desc(smem_u32(smem + stage * 2 * Sh::kTile + Sh::kTile));
-          const uint64_t b = make_kmajor_sw128_desc(p_addr + buf * Sh::kP);
+          const uint64_t b = columns_desc(p_addr + buf * Sh::kP);
           const bool more = t - t0 >= kGroups;  // the group has an O^T of this unit already
 #pragma unroll
           for (int k = 0; k < kPage / 32; ++k)
-            mma_f8f6f4(tmem + 2 * Sh::kSCols + (kGroups == 2 ? buf * kTerms * N : 0), a + 2 * k, b + 2 * k, idesc, more || k > 0);
+            mma_f8f6f4(tmem + 2 * Sh::kSCols + (kGroups == 2 ? buf * kTerms * N : 0), a + 2 * k, b + 64 * k, idesc, more || k > 0);
           // the softmax has had S^T, so both of the stage's pages are done with
           tc_commit(b_empty + 8 * stage);
           tc_commit(b_pvdone + 8 * buf);
@@ -680,26 +689,27 @@ __global__ void __launch_bounds__((Shape<DIM, N, kTermsOf<T>>::kThreads), (Shape
         ++mine;
         // ---- P; its buffer is free once the product before the last has read it
         wait(b_pvdone + 8 * buf, ((it >> 1) & 1) ^ 1, 5);
-        const uint32_t pb = smem_u32(p_smem) + buf * Sh::kP + token;
+        const uint32_t pb = smem_u32(p_smem) + buf * Sh::kP + token * 32, flip = (token & 4) << 2;
 #pragma unroll
         for (int g = 0; g < N; g += 8) {
           if (g >= rows) break;
-          uint32_t term[4][kTerms];
+          uint32_t word[kTerms][2];
 #pragma unroll
           for (int j = 0; j < 8; j += 2) {
             const float e0 = exp2_approx(z[g + j]), e1 = exp2_approx(z[g + j + 1]);
             // the sums take p as it is: a page whose values are tiny beside the others' still counts in full
             l[g + j] = fmaf(e0, ti.inv_vs, l[g + j]);
             l[g + j + 1] = fmaf(e1, ti.inv_vs, l[g + j + 1]);
-            split_e4m3<kTerms>(e0, e1, kTermStep, term[j >> 1]);
+            uint32_t term[kTerms];
+            split_e4m3<kTerms>(e0, e1, kTermStep, term);
+#pragma unroll
+            for (int x = 0; x < kTerms; ++x) word[x][j >> 2] = (j & 2) ? word[x][j >> 2] | (term[x] << 16) : term[x];
           }
 #pragma unroll
-          for (int x = 0; x < kTerms; ++x)
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-              const uint32_t byte = (j & 1) ? term[j >> 1][x] >> 8 : term[j >> 1][x];
-              asm volatile("st.shared.u8 [%0], %1;" ::"r"((pb ^ (j << 4)) + (x * N + g + j) * kPage), "r"(byte) : "memory");
-            }
+          for (int x = 0; x < kTerms; ++x) {
+            const int col = x * N + g;
+            asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(pb + (col >> 5) * (32 * kPage) + ((col & 16) ^ flip) + (col & 8)), "r"(word[x][0]), "r"(word[x][1]) : "memory");
+          }
         }
         fence_proxy_async_smem();
         tc_fence_before();
