@@ -462,6 +462,34 @@ def test_attention_chunks_on_a_long_cache(dev, heads, group, dim, dtype, new, pa
     assert torch.equal(got, again)
 
 
+def test_attention_parts_follow_the_lengths_of_a_replay(dev):
+    """A captured chunk whose sequence grows and shrinks between replays, beside a second graph of the same call."""
+    g = gen(29)
+    n, lens = 100, [3000, 101, 1200, 100]
+    table, ref = make_kv([3000], 2, 128, g)
+    cache, t, cu = on(dev, ref), table.to(dev), i32([0, n]).to(dev)
+    length = i32([3000]).to(dev)
+    q = [torch.randn(n, 8, 128, generator=g).to(BF).to(dev) for _ in range(2)]
+    graphs, out = [], []
+    tg.paged_attention(q[0], cache, t, length, cu, max_q_len=n)
+    torch.cuda.synchronize()
+    for x in q:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            out.append(tg.paged_attention(x, cache, t, length, cu, max_q_len=n))
+    side = torch.cuda.Stream()
+    for now in lens:
+        length.fill_(now)
+        torch.cuda.synchronize()
+        graphs[0].replay()
+        with torch.cuda.stream(side):
+            graphs[1].replay()
+        torch.cuda.synchronize()
+        for x, got in zip(q, out):
+            check_attention(dev, x.cpu(), ref, table, [now], [n], got=got)
+            assert torch.equal(got, tg.paged_attention(x, cache, t, length, cu, max_q_len=n))
+
+
 def test_attention_nan_reaches_over_parts(dev):
     """A NaN in one part of the pages: of a key for the rows that see it, of a value for its element."""
     g = gen(28)
