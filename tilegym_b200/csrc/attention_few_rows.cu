@@ -5,14 +5,18 @@
 //
 //   S^T [128 tokens, R]  = K [128, dim] . Q^T           kind::f8f6f4, q = q1 + q2 (+ q3) in e4m3, summed by the accumulator
 //   p = 2^(S * scale * log2 e + log2 v_scale - ref)     thread = token; v_scale of the page rides in the exponent
-//   O^T [dim, R]        += V^T [dim, 128] . P           p = p1 + p2 (+ p3) in e4m3, the same way
+//   O^T [dim, R]        += V^T [dim, 128] . P           p = p1 + p2 + p3 (+ p4) in e5m2, beside V's e4m3
 //
-// The two factors that are not in the cache are split into e4m3 terms, each holding what the one before left: two hold a
-// bf16 q exactly and p to 2^-8, three (f16) both to 2^-12.  The terms are kept 16 times larger each (which moves the end of
-// e4m3's range out of reach) and stand side by side as rows of the operand, so a page is read once for all of them; their
-// columns of S^T and O^T are joined by the softmax and at the end.  `ref` is a running maximum of the exponent that is only moved when a p would leave the format (2^5 of
-// headroom), which rescales O^T in TMEM.  Keeping v_scale in the exponent keeps p at one magnitude whatever the pages'
-// scales are.
+// The two factors that are not in the cache are split into 8-bit terms, each holding what the one before left, which stand
+// side by side as rows of the operand, so a page is read once for all of them; their columns of S^T and O^T are joined by the
+// softmax and at the end.  q: e4m3, each term kept 16 times larger than the one before; two hold a bf16 exactly, three (f16) to
+// 2^-12.  p: rounded to f16, then cut into e5m2, which is f16's upper byte, 8 times larger each; three terms (bf16) hold it
+// to 2^-9, four (f16) hold the f16 whole.  p needs the range of f16, not of e4m3: where one token has most of a row's weight,
+// a long cache shares the rest among weights 2^-20 of the largest and below, and the sum counts them whatever becomes of them
+// in the product.  A row's largest p is kept between 2^9 and 2^14, so the terms keep their relative rounding down to 2^-23
+// of it and end at 2^-32 (2^-34 with four).
+// `ref` is a running maximum of the exponent that is only moved when a p would pass 2^14 (2^5 of headroom), which rescales O^T
+// in TMEM.  Keeping v_scale in the exponent keeps p at one magnitude whatever the pages' scales are.
 //
 // Work: the pages that the units (sequence, cache head) see are numbered through, each unit kUnitCost numbers in front of
 // them for what it costs to begin and end one, and every block takes an equal range of the numbers, wherever that begins
@@ -23,8 +27,8 @@
 // sums and an O^T of its own, which are joined when the unit ends (the softmax of 32 rows takes longer than copying the page).
 //
 // Bound: HBM up to 16 rows, the chain of the softmax from there.  Measured (8 cache heads of 128, bf16): 64 sequences of up to
-// 16000 tokens with 4 rows 172 us (1.1 GB, 0.97 of the copy bandwidth); 37 sequences of 8000 with 32 rows 153 us (0.61); one
-// sequence of 2001 tokens 12.6 us, of 32000 25 us.  Of 64 sequences of up to 8000 tokens (f16), equal shares counted in pages alone
+// 16000 tokens with 4 rows 173 us (1.1 GB, 0.97 of the copy bandwidth); 37 sequences of 8000 with 32 rows 160 us (0.58); one
+// sequence of 2001 tokens 12.7 us, of 32000 25 us.  Of 64 sequences of up to 8000 tokens (f16), equal shares counted in pages alone
 // took 164 us, with what units cost counted in 103.
 #include <cstdio>
 
@@ -33,21 +37,25 @@
 namespace tg {
 namespace {
 
-constexpr float kNominal = 3.f, kLimit = 8.f;  // p is kept times 2^3 and may reach 2^8 (e4m3 ends at 448) before ref moves
+constexpr float kNominal = 9.f, kLimit = 14.f;  // p is kept times 2^9 and may reach 2^14 (e5m2 ends at 2^15.8) before ref moves
 constexpr float kUnset = -1e30f;  // the reference of a row that has not seen a token yet
 
 template <typename T>
-constexpr int kTermsOf = std::is_same<T, __half>::value ? 3 : 2;
+constexpr int kTermsOf = std::is_same<T, __half>::value ? 3 : 2;  // of q; p has one more
 
 template <int DIM, int N, int TERMS>
 struct Shape {
   static constexpr int kTile = DIM * kPage;  // bytes of a key or value page
-  static constexpr int kP = (TERMS * N + 31) / 32 * 32 * kPage;  // planes of [token][32 columns]
+  static constexpr int kPTerms = TERMS + 1;
+  static constexpr int kP = (kPTerms * N + 31) / 32 * 32 * kPage;  // planes of [token][32 columns]
   static constexpr int kQ = TERMS * N * DIM;
   // two blocks share an SM where each still has a ring of three page pairs
   static constexpr int kBlocksPerSm = N == 16 && !(TERMS == 3 && DIM == 128) ? 2 : 1;
   static constexpr int kGroups = kBlocksPerSm == 2 ? 1 : 2;  // of four softmax warps
   static constexpr int kThreads = 96 + 128 * kGroups;
+  // Each group has a buffer of P.  One group with two buffers would not leave room for three page pairs, and gains nothing by
+  // them: the product of the page before is done long before this page's exponentials are.
+  static constexpr int kPAll = kGroups * kP;
   // A unit's queries, first references and result take about 8000 clocks; a page 2000 (one group, two blocks to share the
   // SM) or 1100.
   static constexpr int kUnitCost = kGroups == 1 ? 4 : 6;
@@ -55,14 +63,15 @@ struct Shape {
   static constexpr int kRowmul = 1024, kRef = kRowmul + N * 4, kWmax = kRef + kGroups * 2 * N * 4, kNan = kWmax + kGroups * 2 * 4 * N * 4;
   static constexpr int kMisc = kNan + (kGroups == 2 ? 2 * 128 * 4 : 0);
   // dim 64: the value operand is read as 128 rows, 64 of them whatever follows the page
-  static constexpr int kBudget = (kBlocksPerSm == 2 ? 113 : 226) * 1024 - 1024 - 2 * kP - kQ - kMisc;
+  static constexpr int kBudget = (kBlocksPerSm == 2 ? 113 : 226) * 1024 - 1024 - kPAll - kQ - kMisc;
   static constexpr int kStages = kBudget / (2 * kTile) > 8 ? 8 : kBudget / (2 * kTile);
-  static constexpr int kSmem = 1024 + kStages * 2 * kTile + 2 * kP + kQ + kMisc;
+  static constexpr int kSmem = 1024 + kStages * 2 * kTile + kPAll + kQ + kMisc;
   static constexpr int kSCols = TERMS * N;  // q's terms have columns of their own in S^T
-  static constexpr int kTmemUsed = 2 * kSCols + kGroups * TERMS * N;  // S^T twice and each group's O^T by term
+  static constexpr int kOCols = kPTerms * N;   // and p's in O^T
+  static constexpr int kTmemUsed = 2 * kSCols + kGroups * kOCols;  // S^T twice and each group's O^T by term
   static constexpr int kTmem = kTmemUsed <= 128 ? 128 : kTmemUsed <= 256 ? 256 : 512;
   static_assert(kStages >= 3, "the ring is too short to hide the latency of a page");
-  static_assert(2 * kP + kQ >= 8192, "the value operand of dim 64 reads 8 KB behind its page");
+  static_assert(kPAll + kQ >= 8192, "the value operand of dim 64 reads 8 KB behind its page");
 };
 
 struct TileInfo {
@@ -73,7 +82,8 @@ struct TileInfo {
 // The operand P [columns][tokens] with the columns together: planes of 32 columns (32 bytes per token, tokens one after the
 // other, the two halves changing places every four tokens: the 32-byte swizzle), 4 KB from one plane to the next and 256 bytes
 // from one group of eight tokens to the next.  A thread, which has a token, writes eight columns at once; with the tokens
-// together every byte was a store of its own (32 rows, f16, dim 64, 37 sequences of 8000: 163 us, 190 that way).
+// together every byte was a store of its own (32 rows, f16, dim 64, 37 sequences of 8000, with three terms: 163 us, 190 that way).
+// B's format is e5m2 (idesc bits 10-12), its columns lie together (bit 16).
 __device__ __forceinline__ uint64_t columns_desc(uint32_t smem_addr) {
   return static_cast<uint64_t>((smem_addr >> 4) & 0x3FFFu) | (static_cast<uint64_t>((32 * kPage) >> 4) << 16) | (static_cast<uint64_t>(256u >> 4) << 32) |
          (1ull << 46) | (6ull << 61);
@@ -83,6 +93,33 @@ __device__ __forceinline__ uint64_t columns_desc(uint32_t smem_addr) {
 template <bool kHint = false>
 __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile uint32_t* abort_flag) {
   return __all_sync(0xffffffffu, mbar_wait<kHint>(bar, parity, abort_flag));
+}
+
+// Eight values as sums of TERMS times eight e5m2 values, each term kPStep times larger than it is beside the one before.  e5m2 is
+// the upper byte of f16 and holds three significant bits: cutting a positive f16 there leaves less than a quarter of its leading
+// bit, exactly.  The last term is rounded to even; four hold all eleven bits, subnormal ones too.
+constexpr float kPStep = 8.f;
+template <int TERMS>
+__device__ __forceinline__ void split_e5m2(const float (&p)[8], uint32_t (&term)[TERMS][2]) {
+  uint32_t h[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) h[j] = pack_pair<__half>(p[2 * j], p[2 * j + 1]);
+#pragma unroll
+  for (int x = 0; x < TERMS; ++x) {
+    if (x + 1 == TERMS) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) h[j] += 0x007f007fu + ((h[j] >> 8) & 0x00010001u);
+    }
+    term[x][0] = __byte_perm(h[0], h[1], 0x7531);
+    term[x][1] = __byte_perm(h[2], h[3], 0x7531);
+    if (x + 1 == TERMS) break;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t cut = h[j] & 0xff00ff00u;
+      const __half2 rest = __hmul2(__hsub2(*reinterpret_cast<const __half2*>(&h[j]), *reinterpret_cast<const __half2*>(&cut)), __float2half2_rn(kPStep));
+      h[j] = *reinterpret_cast<const uint32_t*>(&rest);
+    }
+  }
 }
 
 __device__ __forceinline__ void load8(const float* src, float (&v)[8]) {
@@ -176,11 +213,11 @@ __global__ void __launch_bounds__((Shape<DIM, N, kTermsOf<T>>::kThreads), (Shape
     tg_attention_few_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const __grid_constant__ AttentionParams p) {
   constexpr int kTerms = kTermsOf<T>;
   using Sh = Shape<DIM, N, kTerms>;
-  constexpr int kStages = Sh::kStages, kGroups = Sh::kGroups, kThreads = Sh::kThreads;
+  constexpr int kStages = Sh::kStages, kGroups = Sh::kGroups, kThreads = Sh::kThreads, kPTerms = Sh::kPTerms, kOCols = Sh::kOCols;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* p_smem = smem + kStages * 2 * Sh::kTile;
-  uint8_t* q_smem = p_smem + 2 * Sh::kP;
+  uint8_t* q_smem = p_smem + Sh::kPAll;
   uint8_t* misc = q_smem + Sh::kQ;
   // misc: barriers, tile notes, row factors, exchanged maxima
   uint64_t* bars = reinterpret_cast<uint64_t*>(misc);
@@ -428,7 +465,7 @@ __global__ void __launch_bounds__((Shape<DIM, N, kTermsOf<T>>::kThreads), (Shape
     if (!ok && lane == 0) *p.status = kRoleMma * 1000 + site;
   } else if (warp == 2) {
     // ------------------------------------------------------------------------------------------ values
-    constexpr uint32_t idesc = make_idesc_e4m3_f32(128, kTerms * N) | (1u << 16);  // B lies with its columns together
+    constexpr uint32_t idesc = make_idesc_e4m3_f32(128, kOCols) | (1u << 10) | (1u << 16);
     const uint32_t p_addr = smem_u32(p_smem);
     int it = 0;
     while (left > 0 && ok) {
@@ -443,11 +480,11 @@ __global__ void __launch_bounds__((Shape<DIM, N, kTermsOf<T>>::kThreads), (Shape
         tc_fence_after();
         if (elect_one()) {
           const uint64_t a = make_kmajor_sw128_desc(smem_u32(smem + stage * 2 * Sh::kTile + Sh::kTile));
-          const uint64_t b = columns_desc(p_addr + buf * Sh::kP);
+          const uint64_t b = columns_desc(p_addr + (kGroups == 2 ? buf * Sh::kP : 0));
           const bool more = t - t0 >= kGroups;  // the group has an O^T of this unit already
 #pragma unroll
           for (int k = 0; k < kPage / 32; ++k)
-            mma_f8f6f4(tmem + 2 * Sh::kSCols + (kGroups == 2 ? buf * kTerms * N : 0), a + 2 * k, b + 64 * k, idesc, more || k > 0);
+            mma_f8f6f4(tmem + 2 * Sh::kSCols + (kGroups == 2 ? buf * kOCols : 0), a + 2 * k, b + 64 * k, idesc, more || k > 0);
           // the softmax has had S^T, so both of the stage's pages are done with
           tc_commit(b_empty + 8 * stage);
           tc_commit(b_pvdone + 8 * buf);
@@ -464,7 +501,7 @@ __global__ void __launch_bounds__((Shape<DIM, N, kTermsOf<T>>::kThreads), (Shape
     const int quarter = warp & 3, token = quarter * 32 + lane, at = (warp - 3) * 32 + lane, group = kGroups == 2 ? at >> 7 : 0;
     const int st = at & 127;
     const uint32_t lane_off = static_cast<uint32_t>(quarter * 32) << 16;
-    const uint32_t t_all = tmem + 2 * Sh::kSCols + lane_off, t_o = t_all + group * kTerms * N;
+    const uint32_t t_all = tmem + 2 * Sh::kSCols + lane_off, t_o = t_all + group * kOCols;
     float* refs = reinterpret_cast<float*>(misc + Sh::kRef);          // [group][copy][N]
     float* ref = refs + group * 2 * N;
     float* maxima = reinterpret_cast<float*>(misc + Sh::kWmax);       // [group][copy][4][N]: the warps' maxima, or sums, by row
@@ -667,12 +704,12 @@ __global__ void __launch_bounds__((Shape<DIM, N, kTermsOf<T>>::kThreads), (Shape
               *reinterpret_cast<float4*>(now + g + 4) = make_float4(top[4], top[5], top[6], top[7]);
             }
             if (mine > 0 && any) {
-              uint32_t o[kTerms][8];
+              uint32_t o[kPTerms][8];
 #pragma unroll
-              for (int x = 0; x < kTerms; ++x) tmem_ld_32x8(t_o + x * N + g, o[x]);
+              for (int x = 0; x < kPTerms; ++x) tmem_ld_32x8(t_o + x * N + g, o[x]);
               tmem_ld_wait();
 #pragma unroll
-              for (int x = 0; x < kTerms; ++x) {
+              for (int x = 0; x < kPTerms; ++x) {
 #pragma unroll
                 for (int j = 0; j < 8; ++j) o[x][j] = __float_as_uint(__uint_as_float(o[x][j]) * f[j]);
                 tmem_st_32x8(t_o + x * N + g, o[x]);
@@ -687,26 +724,23 @@ __global__ void __launch_bounds__((Shape<DIM, N, kTermsOf<T>>::kThreads), (Shape
           }
         }
         ++mine;
-        // ---- P; its buffer is free once the product before the last has read it
-        wait(b_pvdone + 8 * buf, ((it >> 1) & 1) ^ 1, 5);
-        const uint32_t pb = smem_u32(p_smem) + buf * Sh::kP + token * 32, flip = (token & 4) << 2;
+        // ---- P; its buffer is free once the group's product before has read it
+        wait(b_pvdone + 8 * ((it - kGroups) & 1), ((it - kGroups) >> 1) & 1, 5);
+        const uint32_t pb = smem_u32(p_smem) + group * Sh::kP + token * 32, flip = (token & 4) << 2;
 #pragma unroll
         for (int g = 0; g < N; g += 8) {
           if (g >= rows) break;
-          uint32_t word[kTerms][2];
+          float e[8];
 #pragma unroll
-          for (int j = 0; j < 8; j += 2) {
-            const float e0 = exp2_approx(z[g + j]), e1 = exp2_approx(z[g + j + 1]);
+          for (int j = 0; j < 8; ++j) {
+            e[j] = exp2_approx(z[g + j]);
             // the sums take p as it is: a page whose values are tiny beside the others' still counts in full
-            l[g + j] = fmaf(e0, ti.inv_vs, l[g + j]);
-            l[g + j + 1] = fmaf(e1, ti.inv_vs, l[g + j + 1]);
-            uint32_t term[kTerms];
-            split_e4m3<kTerms>(e0, e1, kTermStep, term);
-#pragma unroll
-            for (int x = 0; x < kTerms; ++x) word[x][j >> 2] = (j & 2) ? word[x][j >> 2] | (term[x] << 16) : term[x];
+            l[g + j] = fmaf(e[j], ti.inv_vs, l[g + j]);
           }
+          uint32_t word[kPTerms][2];
+          split_e5m2<kPTerms>(e, word);
 #pragma unroll
-          for (int x = 0; x < kTerms; ++x) {
+          for (int x = 0; x < kPTerms; ++x) {
             const int col = x * N + g;
             asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(pb + (col >> 5) * (32 * kPage) + ((col & 16) ^ flip) + (col & 8)), "r"(word[x][0]), "r"(word[x][1]) : "memory");
           }
@@ -771,9 +805,9 @@ __global__ void __launch_bounds__((Shape<DIM, N, kTermsOf<T>>::kThreads), (Shape
         float o[8], sum[8], base[8];
 #pragma unroll
         for (int x = 0; x < kGroups; ++x) {
-          uint32_t part[kTerms][8];
+          uint32_t part[kPTerms][8];
 #pragma unroll
-          for (int y = 0; y < kTerms; ++y) tmem_ld_32x8(t_all + (x * kTerms + y) * N + g, part[y]);
+          for (int y = 0; y < kPTerms; ++y) tmem_ld_32x8(t_all + x * kOCols + y * N + g, part[y]);
           float lx[8], rx[8];
           const float* sx = maxima + x * 8 * N + copy[x].x * 4 * N + g;
           load8(sx, lx);
@@ -788,9 +822,9 @@ __global__ void __launch_bounds__((Shape<DIM, N, kTermsOf<T>>::kThreads), (Shape
           tmem_ld_wait();
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
-            float ox = __uint_as_float(part[kTerms - 1][j]);
+            float ox = __uint_as_float(part[kPTerms - 1][j]);
 #pragma unroll
-            for (int y = kTerms - 2; y >= 0; --y) ox = fmaf(ox, 1.f / kTermStep, __uint_as_float(part[y][j]));
+            for (int y = kPTerms - 2; y >= 0; --y) ox = fmaf(ox, 1.f / kPStep, __uint_as_float(part[y][j]));
             if (!has[x]) {
               ox = 0.f;
               lx[j] = 0.f;
