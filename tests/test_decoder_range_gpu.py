@@ -73,7 +73,7 @@ def test_the_many_count_beside_one(dev, n, length, share, dim, dtype):
 
 
 # every score of the many alike: roundings that do not average out (2^-21.3 of the whole each at the longest)
-@pytest.mark.parametrize("n", [1, 8])
+@pytest.mark.parametrize("n", [1, 8, 9])
 @pytest.mark.parametrize("length,share", [(16000, 0.9), (131072, 0.95)])
 @pytest.mark.parametrize("dim,dtype", [(128, BF), (64, HF)])
 def test_the_many_count_where_they_are_alike(dev, n, length, share, dim, dtype):

@@ -11,8 +11,8 @@
 //
 // The work goes by half pages (64 tokens): TMEM holds O of both tiles (2 x 128 columns) and two S buffers of 64 columns for
 // each, P taking the place of the S it came from, so that the next scores are there when a softmax is done with the last
-// and the tensor core never waits for one tile alone.  `ref` is a running maximum that
-// moves only when a p would exceed 2^14 (f16 has room for that), which is when O is rescaled in TMEM.
+// and the tensor core never waits for one tile alone.  `ref` is a running maximum, less 8, that
+// moves only when a p would exceed 2^15 (f16 has room for that), which is when O is rescaled in TMEM.
 // Few blocks (a chunk of a prompt on a long cache, few heads) leave most SMs idle: there `splits` blocks share a block's pages,
 // each at least kMinPages, and a joining kernel adds their parts in order.
 // Warp 0 copies pages, warps 1 and 2 issue the tiles' score products and warp 3 the value products (a warp that issues is
@@ -20,8 +20,8 @@
 // with one warp for all the tensor core was idle 60 % of the time, with two 45 %), warps 4-7 convert values, warps 8-11 and 12-15 are the tiles' softmax.
 //
 // Bound: the chain scores -> softmax -> product of a half page (about 1700 clocks for both tiles; the products need 1250, the
-// exponentials 1024).  Measured (bf16, 32 heads on 8 of 128): 4 prompts of 300-2500 tokens on up to 5000 cached 245 us
-// (780 TFLOP/s of 1631 measured for a 16-bit GEMM; 351 with whole pages and one issuing warp), one of 4096 172 us.
+// exponentials 1024).  Measured (bf16, 32 heads on 8 of 128): 4 prompts of 300-2500 tokens on up to 5000 cached 250 us
+// (765 TFLOP/s of 1631 measured for a 16-bit GEMM; 351 with whole pages and one issuing warp), one of 4096 174 us.
 #include <cstdio>
 
 #include "tg_attention.cuh"
@@ -35,7 +35,9 @@ constexpr int kHalf = kPage / 2;  // tokens of a step
 constexpr int kPoly = 5;
 constexpr int kMinPages = 4;  // of a part: joining takes as long as three or four pages
 constexpr float kUnset = -1e30f;  // the reference of a row that has not seen a token yet
-constexpr float kHeadroom = 14.f;  // p may reach 2^14 before ref moves (f16 ends at 2^16)
+// A row's largest p is 2^8 when ref is set and may reach 2^15 before ref moves (f16 ends at 2^16): f16 keeps its relative
+// rounding down to 2^-22 of the largest.  A first token with most of the weight leaves the rest of a long cache there.
+constexpr float kNominal = 8.f, kLimit = 15.f;
 
 template <int DIM, int TERMS>
 struct Shape {
@@ -512,9 +514,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         const float most = max3(mx[1], mx[2], mx[2]), top = fmaf(most, f, lv);
         // the row sees a NaN (the sum keeps it)
         if (most != -INFINITY && (odd || !(top < INFINITY))) l = __uint_as_float(0x7fc00000u);
-        const bool move = top > ref + (ref == kUnset ? 0.f : kHeadroom);
+        const bool move = top > ref + (ref == kUnset ? 0.f : kLimit);
         if (__any_sync(0xffffffffu, move)) {
-          const float now = move ? top : ref, shrink = exp2_approx(ref - now);
+          const float now = move ? top - kNominal : ref, shrink = exp2_approx(ref - now);
           ref = now;
           l *= shrink;
           if (j + half > 0) {
@@ -710,7 +712,7 @@ cudaError_t launch(const CUtensorMap& tmK, const CUtensorMap& tmV, const Attenti
 
 int64_t many_rows_tiles(int64_t tokens, int64_t seqs, int group) { return tokens / (2 * (128 / group)) + seqs; }
 
-// As many parts as there are SMs for.  100 tokens on 32000, 32 heads on 8: 86 us, undivided 542; 500 tokens on 4000, 8 heads
+// As many parts as there are SMs for.  100 tokens on 32000, 32 heads on 8: 87 us, undivided 542; 500 tokens on 4000, 8 heads
 // on 2: 33 and 88; 1000 tokens on 4000, 32 heads on 8, are 136 blocks and stay whole (99 us).
 int many_rows_splits(int64_t tokens, int64_t seqs, int64_t heads, int group, int64_t max_pages, int num_sms) {
   const int64_t blocks = many_rows_tiles(tokens, seqs, group) * heads;

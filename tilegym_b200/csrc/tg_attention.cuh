@@ -23,7 +23,7 @@ struct AttentionParams {
 };
 
 // Few rows per (sequence, cache head): the cache's bytes are what counts.  37 sequences of 8000 tokens, 8 cache heads of 128,
-// with 32 rows each: 160 us, 223 with the kernel for many rows; with 64 rows 481 and 226.
+// with 32 rows each: 160 us, 226 with the kernel for many rows; with 64 rows 481 and 232.
 constexpr int kFewRowsMax = 32;
 int few_rows_padded(int rows);  // 16 or 32
 int few_rows_blocks(int dim, int rows_padded, bool bf16, int num_sms);
