@@ -594,6 +594,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         __syncwarp();
       }
+      // a row that has seen nothing: the polynomial's 2^-126 of hidden places is no sum (a NaN stays: the row has seen one)
+      if (ref == kUnset && l == l) l = 0.f;
       const float inv = l == 0.f ? 0.f : 1.0f / l;
       const int64_t slot = static_cast<int64_t>(blockIdx.x) * 256 + w * 128 + row;
       if (kSplit && parts > 1) p.part_ml[slot] = make_float2(ref, l);
