@@ -371,7 +371,7 @@ TG_API int32_t tg_plan_splits(int32_t kind, int64_t M, int64_t N, int64_t K, int
  *   (1 for an all-zero block),  Y = e4m3(y / s).
  * X, R [T, hidden] bf16 / f16 with any row pitch (a multiple of 16 bytes); hidden a multiple of 128 up to 65536; W [hidden]
  * in X's type or f32; Y [T, hidden] e4m3, S [T, hidden / 128] f32, H [T, hidden] contiguous.  R and H go together (both
- * null: h = x).  H may be the memory of X or of R. */
+ * null: h = x).  H may be the memory of X or of R where their rows are dense (a pitch of hidden); any other overlap is refused. */
 TG_API int32_t tg_rms_norm_quant(const TgTensorDesc* Y, const TgTensorDesc* S, const TgTensorDesc* H, const TgTensorDesc* X,
                                  const TgTensorDesc* R, const TgTensorDesc* W, float eps, float weight_offset, int32_t device_id,
                                  uint64_t stream);

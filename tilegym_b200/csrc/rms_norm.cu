@@ -178,6 +178,15 @@ extern "C" TG_API int32_t tg_rms_norm_quant(const TgTensorDesc* Y, const TgTenso
     if ((t->ptr & 15u) || (T > 1 && (t->strides[0] & 7))) return api_fail(TG_ERR_ALIGN, "rows of X and of the residual need 16-byte alignment");
   }
   if (T == 0) return TG_OK;
+  if (H != nullptr) {
+    // H's row t may lie on row t of an input, which its block has read by then, but not on rows that others have still to read
+    const uint64_t row = static_cast<uint64_t>(hidden) * 2, h_end = H->ptr + T * row;
+    for (const TgTensorDesc* t : in) {
+      const uint64_t end = t->ptr + static_cast<uint64_t>(T - 1) * static_cast<uint64_t>(t->strides[0]) * 2 + row;
+      if (t->ptr < h_end && H->ptr < end && !(t->ptr == H->ptr && (T == 1 || t->strides[0] == hidden)))
+        return api_fail(TG_ERR_ARGS, "H overlaps rows of X or of the residual: it may only take the place of dense ones");
+    }
+  }
   ScopedDevice guard(device_id);
   if (guard.err != cudaSuccess) {
     cudaGetLastError();
