@@ -32,3 +32,63 @@ def test_norm_refuses_a_sum_over_rows_that_are_still_read():
         for H, X, R, T in ((dense, dense, other, 4), (dense, other, dense, 4), (dense, dense, dense, 4), (other, pitched, shifted, 4),
                            (dense[:1], pitched[:1], other[:1], 1)):
             assert call(H, X, R, T) != -6
+
+
+# ------------------------------------------------------------------ FP8DecoderLayer.from_layer
+class Built(tg.FP8DecoderLayer):
+    """What from_layer found in a layer, without quantising it (which needs a GPU)."""
+
+    def __init__(self, weights, num_heads, num_kv_heads, head_dim, inv_freq, magnitude=1.0, **kwargs):
+        torch.nn.Module.__init__(self)
+        self.found = dict(kwargs, num_heads=num_heads, num_kv_heads=num_kv_heads)
+
+
+def plain_layer(norm=torch.nn.RMSNorm, **attention):
+    nn = torch.nn
+    m = nn.Module()
+    m.self_attn, m.mlp = nn.Module(), nn.Module()
+    a, p = m.self_attn, m.mlp
+    a.q_proj, a.k_proj, a.v_proj, a.o_proj = (nn.Linear(256, n, bias=False) for n in (256, 128, 128, 256))
+    p.gate_proj, p.up_proj, p.down_proj, p.act_fn = nn.Linear(256, 512, bias=False), nn.Linear(256, 512, bias=False), nn.Linear(512, 256, bias=False), nn.SiLU()
+    m.input_layernorm, m.post_attention_layernorm = norm(256, eps=1e-6), norm(256, eps=1e-6)
+    for name, value in attention.items():
+        setattr(a, name, value)
+    return m
+
+
+def built(layer, **kwargs):
+    return Built.from_layer(layer, 64, torch.ones(32, dtype=torch.float64), **kwargs).found
+
+
+class Config:
+    def __init__(self, **values):
+        self.__dict__.update(values)
+
+
+def test_layer_takes_over_the_sliding_window():
+    """Where a layer keeps its window: on the attention, or in the model's configuration, for every layer or for some."""
+    assert built(plain_layer()).get("window", 0) == 0
+    assert built(plain_layer(sliding_window=None, config=Config(sliding_window=512))).get("window", 0) == 0
+    assert built(plain_layer(sliding_window=512))["window"] == 512
+    assert built(plain_layer(config=Config(sliding_window=4096)))["window"] == 4096
+    assert built(plain_layer(config=Config(sliding_window=None))).get("window", 0) == 0
+    assert built(plain_layer(config=Config(sliding_window=64, use_sliding_window=False))).get("window", 0) == 0
+    kinds = Config(sliding_window=64, layer_types=["full_attention", "sliding_attention"])
+    assert built(plain_layer(config=kinds, layer_idx=0)).get("window", 0) == 0
+    assert built(plain_layer(config=kinds, layer_idx=1))["window"] == 64
+    # what the caller says holds
+    assert built(plain_layer(sliding_window=512), window=128, sinks=4)["window"] == 128
+    assert built(plain_layer(sliding_window=512), window=0)["window"] == 0
+    with pytest.raises(NotImplementedError, match="chunked_attention"):
+        built(plain_layer(config=Config(layer_types=["chunked_attention"]), layer_idx=0))
+
+
+def test_layer_takes_over_the_window_of_real_layers():
+    transformers = pytest.importorskip("transformers")
+    size = dict(hidden_size=256, intermediate_size=256, num_hidden_layers=2, num_attention_heads=4, num_key_value_heads=2, vocab_size=16)
+    mistral = transformers.MistralModel(transformers.MistralConfig(sliding_window=48, **size))
+    qwen = transformers.Qwen2Model(transformers.Qwen2Config(use_sliding_window=True, sliding_window=32, max_window_layers=1, **size))
+    llama = transformers.LlamaModel(transformers.LlamaConfig(**size))
+    assert [built(m).get("window", 0) for m in mistral.layers] == [48, 48]
+    assert [built(m).get("window", 0) for m in qwen.layers] == [0, 32]
+    assert [built(m).get("window", 0) for m in llama.layers] == [0, 0]

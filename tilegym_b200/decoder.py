@@ -46,6 +46,23 @@ def _refuse_other_layers(layer: nn.Module, head_dim: int) -> None:
         raise NotImplementedError("FP8DecoderLayer takes an MLP with silu")
 
 
+def _window_of(layer: nn.Module) -> int:
+    """The layer's sliding window (0: none): on its attention, or in the model's configuration for the layers that use it."""
+    att = layer.self_attn
+    config = getattr(att, "config", None)
+    kinds, index = getattr(config, "layer_types", None), getattr(att, "layer_idx", None)
+    kind = kinds[index] if kinds and index is not None else None
+    if kind not in (None, "full_attention", "sliding_attention"):
+        raise NotImplementedError(f"FP8DecoderLayer does not implement {kind}")
+    if hasattr(att, "sliding_window"):
+        window = att.sliding_window
+    elif kind == "full_attention" or not getattr(config, "use_sliding_window", True):
+        window = None
+    else:
+        window = getattr(config, "sliding_window", None)
+    return 0 if window is None else int(window)
+
+
 class FP8DecoderLayer(nn.Module):
     """Built by `from_layer` from a layer with `input_layernorm`, `self_attn.{q,k,v,o}_proj`, `post_attention_layernorm` and
     `mlp.{gate,up,down}_proj` (Llama, Mistral, Qwen2, ...).  Hidden and intermediate sizes must be multiples of 128,
@@ -86,9 +103,11 @@ class FP8DecoderLayer(nn.Module):
     @classmethod
     def from_layer(cls, layer: nn.Module, head_dim: int, inv_freq: torch.Tensor, magnitude: float = 1.0, eps: Optional[float] = None,
                    **kwargs) -> "FP8DecoderLayer":
-        """Quantises a layer whose weights are on a CUDA device.  kwargs go to the constructor (window, sinks, ...)."""
+        """Quantises a layer whose weights are on a CUDA device.  kwargs go to the constructor (window, sinks, ...); without
+        `window` the layer's own is taken over."""
         att, mlp = layer.self_attn, layer.mlp
         _refuse_other_layers(layer, head_dim)
+        kwargs.setdefault("window", _window_of(layer))
         parts = [att.q_proj, att.k_proj, att.v_proj]
         weights = {
             "norm1": layer.input_layernorm.weight, "norm2": layer.post_attention_layernorm.weight,
