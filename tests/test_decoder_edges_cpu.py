@@ -92,3 +92,55 @@ def test_layer_takes_over_the_window_of_real_layers():
     assert [built(m).get("window", 0) for m in mistral.layers] == [48, 48]
     assert [built(m).get("window", 0) for m in qwen.layers] == [0, 32]
     assert [built(m).get("window", 0) for m in llama.layers] == [0, 0]
+
+
+class Shifted(torch.nn.RMSNorm):
+    """A norm whose weight counts from one."""
+
+    def forward(self, x):
+        return torch.nn.functional.rms_norm(x, (x.shape[-1],), self.weight + 1, self.eps)
+
+
+def test_layer_refuses_what_it_would_compute_otherwise():
+    nn = torch.nn
+
+    def with_(owner, **values):
+        layer = plain_layer()
+        for name, value in values.items():
+            setattr({"layer": layer, "attention": layer.self_attn, "mlp": layer.mlp}[owner], name, value)
+        return layer
+
+    built(plain_layer())
+    for name in ("query_layernorm", "key_layernorm", "q_layernorm", "k_layernorm"):
+        with pytest.raises(NotImplementedError, match=name):
+            built(with_("attention", **{name: nn.RMSNorm(64)}))
+    for owner, name, value, harmless in (("layer", "residual_multiplier", 0.22, 1.0), ("layer", "use_parallel_residual", True, False),
+                                         ("attention", "use_rope", 0, 1), ("attention", "clip_qkv", 8.0, None)):
+        with pytest.raises(NotImplementedError, match=name):
+            built(with_(owner, **{name: value}))
+        built(with_(owner, **{name: harmless}))
+    with pytest.raises(NotImplementedError, match="clip_qkv"):
+        built(plain_layer(config=Config(clip_qkv=8.0)))
+
+
+def test_layer_refuses_norms_of_another_kind():
+    nn = torch.nn
+    with pytest.raises(NotImplementedError, match="input_layernorm"):
+        built(plain_layer(nn.LayerNorm))
+    with pytest.raises(NotImplementedError, match="input_layernorm"):
+        built(plain_layer(Shifted))
+    assert built(plain_layer(Shifted), weight_offset=1.0)["weight_offset"] == 1.0
+    # an epsilon that is not the first norm's; one that the caller passes holds
+    layer = plain_layer()
+    layer.post_attention_layernorm.eps = 1e-3
+    with pytest.raises(NotImplementedError, match="post_attention_layernorm"):
+        built(layer)
+    assert built(layer, eps=1e-4)["eps"] == 1e-4
+    for dtype in (torch.bfloat16, torch.float16):
+        assert built(plain_layer().to(dtype))["eps"] == 1e-6
+    # a holder of weights that cannot be called is taken as an RMS norm
+    layer = plain_layer()
+    layer.input_layernorm = nn.Module()
+    layer.input_layernorm.weight, layer.input_layernorm.eps = nn.Parameter(torch.ones(256)), 1e-5
+    layer.post_attention_layernorm.eps = 1e-5
+    assert built(layer)["eps"] == 1e-5

@@ -32,11 +32,19 @@ _FP8 = torch.float8_e4m3fn
 def _refuse_other_layers(layer: nn.Module, head_dim: int) -> None:
     """Layers that compute something else with the same projections would come out wrong without a word."""
     att, mlp = layer.self_attn, layer.mlp
-    for owner, names in ((att, ("q_norm", "k_norm", "sinks", "attn_logit_softcapping")),
+    for owner, names in ((att, ("q_norm", "k_norm", "query_layernorm", "key_layernorm", "q_layernorm", "k_layernorm", "sinks",
+                                "attn_logit_softcapping", "clip_qkv")),
+                         (getattr(att, "config", None), ("clip_qkv",)),
                          (layer, ("pre_feedforward_layernorm", "post_feedforward_layernorm"))):
         for name in names:
             if getattr(owner, name, None) is not None:
                 raise NotImplementedError(f"FP8DecoderLayer does not implement {name}")
+    if getattr(layer, "residual_multiplier", 1.0) != 1.0:
+        raise NotImplementedError("FP8DecoderLayer does not implement a residual_multiplier")
+    if getattr(layer, "use_parallel_residual", False):
+        raise NotImplementedError("FP8DecoderLayer does not implement use_parallel_residual")
+    if not getattr(att, "use_rope", True):
+        raise NotImplementedError("FP8DecoderLayer rotates queries and keys: the layer's use_rope is off")
     scaling = getattr(att, "scaling", None)
     if scaling is not None and abs(scaling * head_dim**0.5 - 1.0) > 1e-6:
         raise NotImplementedError(f"FP8DecoderLayer scales scores by head_dim^-0.5, not by {scaling}")
@@ -44,6 +52,24 @@ def _refuse_other_layers(layer: nn.Module, head_dim: int) -> None:
     probe = torch.linspace(-4.0, 4.0, 9)
     if act is not None and not torch.allclose(act(probe), nn.functional.silu(probe), atol=1e-6):
         raise NotImplementedError("FP8DecoderLayer takes an MLP with silu")
+
+
+def _refuse_other_norms(layer: nn.Module, eps: float, eps_given: bool, weight_offset: float) -> None:
+    """The layer's norms are tried on two rows, ordinary values and ones whose squares are as small as eps."""
+    for name in ("input_layernorm", "post_attention_layernorm"):
+        norm = getattr(layer, name)
+        if not callable(norm) or getattr(type(norm), "forward", None) is nn.Module.forward:
+            continue  # holds a weight and nothing else
+        w = norm.weight.detach()
+        x = torch.linspace(0.5, 2.0, w.numel(), device=w.device)  # a mean that is not zero
+        rows = torch.stack((x, x * (eps**0.5 if eps > 0 and not eps_given else 1.0))).to(w.dtype)
+        f = rows.float()
+        want = f * torch.rsqrt((f * f).mean(-1, keepdim=True) + eps) * (w.float() + weight_offset)
+        with torch.no_grad():
+            got = norm(rows).float()
+        # two roundings to 16 bits
+        if got.shape != want.shape or not torch.allclose(got, want, rtol=2.0**-6, atol=1e-6):
+            raise NotImplementedError(f"{name} is not an RMS norm of weight + {weight_offset} and eps {eps}")
 
 
 def _window_of(layer: nn.Module) -> int:
@@ -119,8 +145,10 @@ class FP8DecoderLayer(nn.Module):
         if any((p.bias is None) != (parts[0].bias is None) for p in parts):
             raise NotImplementedError("q_proj, k_proj and v_proj must all have a bias or none")
         bias = None if parts[0].bias is None else torch.cat([p.bias for p in parts])
-        if eps is None:
+        eps_given = eps is not None
+        if not eps_given:
             eps = getattr(layer.input_layernorm, "variance_epsilon", None) or getattr(layer.input_layernorm, "eps", None) or 1e-6
+        _refuse_other_norms(layer, eps, eps_given, kwargs.get("weight_offset", 0.0))
         return cls(weights, att.q_proj.out_features // head_dim, att.k_proj.out_features // head_dim, head_dim, inv_freq, magnitude,
                    eps=eps, qkv_bias=bias, o_bias=att.o_proj.bias, **kwargs)
 
