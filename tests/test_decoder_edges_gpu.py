@@ -47,3 +47,33 @@ def test_rows_that_see_nothing_are_zero_whatever_the_scales(dev, exponent, n, le
     assert bool((got[:empty] == 0).all())
     if exponent < 7 or dtype == BF:  # f16 ends at 2^16
         assert bool(got[empty:].isfinite().all()) and bool((got[empty:] != 0).any(-1).all())
+
+
+# ------------------------------------------------------------------ kv_cache_write
+@pytest.mark.parametrize("scale", [1.5 * 2.0**-5, 1.0000001 * 2.0**-4, 1.75, 3e-9, 1.9 * 2.0**-30, 2.0**127, 1.5 * 2.0**100])
+@pytest.mark.parametrize("new", [1, 3, 60])
+@pytest.mark.parametrize("dim,dtype", [(64, BF), (128, HF)])
+def test_append_to_a_page_whose_scale_is_no_power_of_two(dev, scale, new, dim, dtype):
+    """Scales are fp32, positive: a page that came from elsewhere may have any.  New tokens are right under the scale that the
+    page keeps, earlier ones under the one that it moves to.
+
+    A byte is off by half a step, 2^-4 of the value or 2^-10 of the scale, and the quotient in front of it by 2^-23."""
+    g = torch.Generator().manual_seed(new + dim)
+    past = 50
+    cache = make_cache(2, 2, dim, new)
+    cache[2].fill_(scale)
+    cache[3].fill_(scale)
+    before = [x[:, :past].clone() for x in D.cache_values(cache, i32([1]), past + new)]
+    k, v = (torch.randn(new, 2, dim, generator=g).to(dtype) for _ in "kv")
+    table, lens = i32([[1]]), i32([past + new])
+    got = on(dev, cache)
+    tg.kv_cache_write(got, k.to(dev), v.to(dev), table.to(dev), lens.to(dev), i32([0, new]).to(dev))
+    back = [c.cpu() for c in got]
+    for x, old, after, s in zip((k, v), before, D.cache_values(back, i32([1]), past + new), (back[2], back[3])):
+        want = torch.cat((old, x.double().transpose(0, 1)), 1)
+        s = s[1, :, None, None].double()
+        bound = torch.clamp(want.abs() * 2.0**-4, min=2.0**-10 * s) * (1 + 2.0**-20)
+        assert bool(((after - want).abs() <= bound).all()), float(((after - want).abs() / bound).max())
+        # a scale that is large enough is kept, and with it the earlier bytes
+        if scale > 2.0**-6:
+            assert bool((s == torch.tensor(scale, dtype=torch.float32).double()).all()) and torch.equal(after[:, :past], old)

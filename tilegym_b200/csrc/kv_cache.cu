@@ -269,7 +269,7 @@ __device__ __forceinline__ void write_tile(const WriteParams& p, const WriteTile
     __syncthreads();  // the scale is read by all before it is written, old bytes are moved before new ones arrive
   }
   if (threadIdx.x == 0) *scale = s;
-  const float r = pow2_reciprocal(s);
+  const float r = 1.0f / s;  // exact but for a kept scale that is no power of two
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
     if (i * kWriteThreads + static_cast<int>(threadIdx.x) >= count) continue;
@@ -383,7 +383,7 @@ __device__ __forceinline__ void write_append(const WriteParams& p, const WriteTi
     __syncwarp();
   }
   if (lane == 0) *scale = s;
-  const float r = pow2_reciprocal(s);
+  const float r = 1.0f / s;  // as in write_tile
   for (int t = at.t0; t < at.t1; ++t) {
     if (at.t1 - at.t0 > 1) token(t, v);  // a single token is still in registers
     uint32_t q = q8_cast2<kQ8E4M3>(v[0] * r, v[1] * r, 0.f, 0.f);
