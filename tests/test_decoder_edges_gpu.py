@@ -1,6 +1,7 @@
 """Calls of the decoder operators at the edges of what their documentation allows."""
 
-import math
+import threading
+import time
 
 import pytest
 import torch
@@ -77,3 +78,36 @@ def test_append_to_a_page_whose_scale_is_no_power_of_two(dev, scale, new, dim, d
         # a scale that is large enough is kept, and with it the earlier bytes
         if scale > 2.0**-6:
             assert bool((s == torch.tensor(scale, dtype=torch.float32).double()).all()) and torch.equal(after[:, :past], old)
+
+
+# ------------------------------------------------------------------ host side
+@pytest.mark.parametrize("call", ["norm", "rope", "write", "attention"])
+def test_a_full_launch_queue_holds_up_its_own_thread_only(dev, call):
+    """A thread whose launches wait for room behind a long kernel (half a second or so) leaves the interpreter to the others."""
+    x, w = torch.ones(1, 128, dtype=BF, device=dev), torch.ones(128, dtype=BF, device=dev)
+    q, kv, at = torch.ones(1, 2, 64, dtype=BF, device=dev), torch.ones(1, 1, 64, dtype=BF, device=dev), torch.zeros(1, dtype=torch.int64, device=dev)
+    f, _ = tg.rope_frequencies(64, device=dev)
+    cache, table, lens = tg.FP8KVCache.empty(1, 1, 64, dev), i32([[0]]).to(dev), i32([1]).to(dev)
+    calls = {"norm": lambda: tg.rms_norm_quant(x, w), "rope": lambda: tg.apply_rope(q, kv, at, f),
+             "write": lambda: tg.kv_cache_write(cache, kv, kv, table, lens), "attention": lambda: tg.paged_attention(q, cache, table, lens)}
+    calls[call]()
+    torch.cuda.synchronize()
+
+    def launch():
+        torch.cuda.set_device(dev)
+        torch.cuda._sleep(1_000_000_000)
+        for _ in range(3000):  # more than the queue holds
+            calls[call]()
+
+    thread = threading.Thread(target=launch)
+    longest, last = 0.0, time.perf_counter()
+    start = last
+    thread.start()
+    while thread.is_alive():
+        time.sleep(0.001)
+        now = time.perf_counter()
+        longest, last = max(longest, now - last), now
+    thread.join()
+    torch.cuda.synchronize()
+    assert last - start > 0.2, "the queue was never full"
+    assert longest < 0.1, f"this thread stood still for {longest:.2f} s"

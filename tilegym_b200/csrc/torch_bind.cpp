@@ -70,6 +70,12 @@ bool heads(const Tensor& t, int64_t dev) {
 }
 bool table(const Tensor& t, int64_t dev) { return on(t, dev) && t.scalar_type() == at::kInt && t.is_contiguous(); }
 uint64_t stream_of(int64_t dev) { return reinterpret_cast<uint64_t>(c10::cuda::getCurrentCUDAStream(static_cast<c10::DeviceIndex>(dev)).stream()); }
+// The C call without the interpreter's lock: a launch may wait for room in a full queue, and other threads go on meanwhile.
+template <typename F>
+int32_t unlocked(F&& call) {
+  py::gil_scoped_release released;
+  return call();
+}
 Tensor like(const Tensor& t) { return at::empty(t.sizes(), t.options()); }
 
 struct Cache {
@@ -99,8 +105,10 @@ py::object rms_norm_quant(const Tensor& x, const Tensor& w, double eps, const Op
     dh.emplace(h, rows, hidden);
     dr.emplace(*residual, rows, hidden);
   }
-  const int32_t rc = tg_rms_norm_quant(dy.p, ds.p, dh ? dh->p : nullptr, dx.p, dr ? dr->p : nullptr, dw.p, static_cast<float>(eps),
-                                       static_cast<float>(offset), static_cast<int32_t>(dev), stream_of(dev));
+  const int32_t rc = unlocked([&] {
+    return tg_rms_norm_quant(dy.p, ds.p, dh ? dh->p : nullptr, dx.p, dr ? dr->p : nullptr, dw.p, static_cast<float>(eps),
+                             static_cast<float>(offset), static_cast<int32_t>(dev), stream_of(dev));
+  });
   if (rc != TG_OK) return py::none();
   if (residual) return py::make_tuple(y, s, h);
   return py::make_tuple(y, s);
@@ -116,8 +124,10 @@ py::object apply_rope(const Tensor& q, const OptTensor& k, const Tensor& positio
   const Tensor qo = inplace ? q : like(q);
   const OptTensor ko = !k ? OptTensor() : OptTensor(inplace ? *k : like(*k));
   const Desc dqo(qo), dko(ko), dq(q), dk(k), dp(positions), df(inv_freq);
-  const int32_t rc = tg_apply_rope(dqo.p, dko.p, dq.p, dk.p, dp.p, df.p, interleaved, static_cast<float>(magnitude), static_cast<int32_t>(dev),
-                                   stream_of(dev));
+  const int32_t rc = unlocked([&] {
+    return tg_apply_rope(dqo.p, dko.p, dq.p, dk.p, dp.p, df.p, interleaved, static_cast<float>(magnitude), static_cast<int32_t>(dev),
+                         stream_of(dev));
+  });
   if (rc != TG_OK) return py::none();
   return py::make_tuple(qo, ko);
 }
@@ -134,8 +144,10 @@ py::object kv_cache_write(const Tensor& kc, const Tensor& vc, const Tensor& ks, 
   const OptTensor qo = q ? OptTensor(like(*q)) : OptTensor();
   const Cache c(kc, vc, ks, vs);
   const Desc dk(k), dv(v), dt(block_table), dl(seq_lens), dc(cu), dqo(qo), dq(q), df(inv_freq);
-  const int32_t rc = tg_kv_cache_write(c.k.p, c.v.p, c.ks.p, c.vs.p, dk.p, dv.p, dt.p, dl.p, dc.p, dqo.p, dq.p, df.p, interleaved,
-                                       static_cast<float>(magnitude), static_cast<int32_t>(dev), stream_of(dev));
+  const int32_t rc = unlocked([&] {
+    return tg_kv_cache_write(c.k.p, c.v.p, c.ks.p, c.vs.p, dk.p, dv.p, dt.p, dl.p, dc.p, dqo.p, dq.p, df.p, interleaved,
+                             static_cast<float>(magnitude), static_cast<int32_t>(dev), stream_of(dev));
+  });
   if (rc != TG_OK) return py::none();
   return py::make_tuple(qo);
 }
@@ -153,10 +165,12 @@ py::object paged_attention(const Tensor& q, const Tensor& kc, const Tensor& vc, 
   if (workspace_bytes > 0) ws = at::empty({workspace_bytes}, q.options().dtype(at::kByte));
   const Cache c(kc, vc, ks, vs);
   const Desc dq(q), dout(o), dt(block_table), dl(seq_lens), dc(cu);
-  const int32_t rc = tg_paged_attention(dout.p, dq.p, c.k.p, c.v.p, c.ks.p, c.vs.p, dt.p, dl.p, dc.p, static_cast<int32_t>(max_q_len),
-                                        static_cast<float>(scale), static_cast<int32_t>(window), static_cast<int32_t>(sinks),
-                                        workspace_bytes > 0 ? reinterpret_cast<uint64_t>(ws.data_ptr()) : 0, static_cast<uint64_t>(workspace_bytes),
-                                        static_cast<int32_t>(dev), stream_of(dev));
+  const int32_t rc = unlocked([&] {
+    return tg_paged_attention(dout.p, dq.p, c.k.p, c.v.p, c.ks.p, c.vs.p, dt.p, dl.p, dc.p, static_cast<int32_t>(max_q_len),
+                              static_cast<float>(scale), static_cast<int32_t>(window), static_cast<int32_t>(sinks),
+                              workspace_bytes > 0 ? reinterpret_cast<uint64_t>(ws.data_ptr()) : 0, static_cast<uint64_t>(workspace_bytes),
+                              static_cast<int32_t>(dev), stream_of(dev));
+  });
   if (rc != TG_OK) return py::none();
   return py::cast(o);
 }
