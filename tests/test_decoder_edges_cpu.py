@@ -144,3 +144,60 @@ def test_layer_refuses_norms_of_another_kind():
     layer.input_layernorm.weight, layer.input_layernorm.eps = nn.Parameter(torch.ones(256)), 1e-5
     layer.post_attention_layernorm.eps = 1e-5
     assert built(layer)["eps"] == 1e-5
+
+
+# ------------------------------------------------------------------ the extension is optional
+@pytest.fixture
+def bind_build(tmp_path, monkeypatch):
+    """The build module with nothing to compile but the extension, into a folder of its own, by a compiler that the test plays."""
+    import types
+
+    from tilegym_b200 import build
+
+    for name, path in (("LIB_PATH", "lib.so"), ("BIND_PATH", "_bind.so")):
+        monkeypatch.setattr(build, name, str(tmp_path / path))
+    monkeypatch.setattr(build, "OBJ_DIR", str(tmp_path / "build"))
+    monkeypatch.setattr(build, "SOURCES", [])
+    (tmp_path / "lib.so").write_bytes(b"")
+    calls, result = [], types.SimpleNamespace(returncode=0, stdout="", stderr="no such header")
+
+    def run(cmd, **_):
+        calls.append(cmd)
+        if result.returncode == 0:
+            (tmp_path / "_bind.so").write_bytes(b"built")
+        return result
+
+    monkeypatch.setattr(build.subprocess, "run", run)
+    return build, calls, result, tmp_path / "_bind.so"
+
+
+def test_build_goes_on_without_the_extension(bind_build, capsys):
+    """Where torch's headers or g++ are missing the library is built all the same, and an extension of an older build, which may
+    call it otherwise, is not left beside it."""
+    build, calls, result, bind = bind_build
+    bind.write_bytes(b"old")
+    result.returncode = 1
+    assert build.build(force=False) == build.LIB_PATH
+    assert len(calls) == 1 and not bind.exists()
+    assert "without" in capsys.readouterr().err
+
+
+def test_extension_is_rebuilt_for_another_torch(bind_build, monkeypatch):
+    build, calls, _, bind = bind_build
+    build.build()
+    assert len(calls) == 1 and bind.exists()
+    build.build()
+    assert len(calls) == 1
+    monkeypatch.setattr(torch, "__version__", "9.9.9")
+    build.build()
+    assert len(calls) == 2
+
+
+def test_extension_of_another_torch_is_not_called(monkeypatch):
+    import types
+
+    fake = types.SimpleNamespace(torch_version="9.9.9")
+    assert _lib.usable_extension(fake) is None and _lib.usable_extension(None) is None
+    fake.torch_version = torch.__version__
+    assert _lib.usable_extension(fake) is fake
+    assert _lib.fast is None or _lib.fast.torch_version == torch.__version__

@@ -71,6 +71,14 @@ try:
 except ImportError:
     fast = None
 
+
+def usable_extension(module):
+    """`module` where it was built for the torch that runs, else None."""
+    return module if getattr(module, "torch_version", None) == torch.__version__ else None
+
+
+fast = usable_extension(fast)
+
 # name -> (restype, argtypes); the list the symbol-export test walks.
 _P = ctypes.c_char_p  # const TgTensorDesc*, passed as the packed bytes of desc()
 SIGNATURES = {

@@ -75,23 +75,33 @@ def build(force: bool = False, verbose: bool = False) -> str:
         if r.returncode != 0:
             sys.stderr.write(r.stdout + r.stderr)
             raise RuntimeError("link failed")
-    build_bind(force)
+    try:
+        build_bind(force)
+    except Exception as e:  # g++, torch's headers: the library does without
+        if os.path.exists(BIND_PATH):
+            os.remove(BIND_PATH)  # of an older build, which may call the library otherwise
+        sys.stderr.write(f"{e}: the library is built without the extension; decode-sized calls go through ctypes\n")
     return LIB_PATH
 
 
 def build_bind(force: bool = False) -> str:
-    src = os.path.join(CSRC, "torch_bind.cpp")
-    if not force and _newer(BIND_PATH, [src, os.path.join(PKG_DIR, "..", "include", "tilegym_b200.h")]):
-        return BIND_PATH
     import sysconfig
 
     import torch
+
+    src = os.path.join(CSRC, "torch_bind.cpp")
+    stamp = os.path.join(OBJ_DIR, "bind.torch")  # the version that it was built for
+    if not force and _newer(BIND_PATH, [src, os.path.join(PKG_DIR, "..", "include", "tilegym_b200.h")]) and os.path.exists(stamp):
+        with open(stamp) as f:
+            if f.read() == torch.__version__:
+                return BIND_PATH
 
     root = os.path.dirname(os.path.abspath(torch.__file__))
     cuda = os.path.dirname(os.path.dirname(os.path.realpath(_nvcc())))
     include = [os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api", "include"),
                os.path.join(cuda, "include"), sysconfig.get_paths()["include"]]
     cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
+           f'-DTG_TORCH_VERSION="{torch.__version__}"',
            src, "-o", BIND_PATH] + [f"-I{p}" for p in include]
     cmd += [f"-L{os.path.join(root, 'lib')}", f"-L{PKG_DIR}", "-l:libtilegym_b200.so", "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python",
             "-Wl,-rpath,$ORIGIN"]
@@ -99,6 +109,8 @@ def build_bind(force: bool = False) -> str:
     if r.returncode != 0:
         sys.stderr.write(r.stdout + r.stderr)
         raise RuntimeError("g++ failed on torch_bind.cpp")
+    with open(stamp, "w") as f:
+        f.write(torch.__version__)
     return BIND_PATH
 
 

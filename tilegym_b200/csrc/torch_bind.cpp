@@ -178,6 +178,7 @@ py::object paged_attention(const Tensor& q, const Tensor& kc, const Tensor& vc, 
 }  // namespace
 
 PYBIND11_MODULE(_bind, m) {
+  m.attr("torch_version") = TG_TORCH_VERSION;  // the one it was built for: it is not called under another
   m.def("rms_norm_quant", &rms_norm_quant);
   m.def("apply_rope", &apply_rope);
   m.def("kv_cache_write", &kv_cache_write);
