@@ -201,3 +201,19 @@ def test_extension_of_another_torch_is_not_called(monkeypatch):
     fake.torch_version = torch.__version__
     assert _lib.usable_extension(fake) is fake
     assert _lib.fast is None or _lib.fast.torch_version == torch.__version__
+
+
+# ------------------------------------------------------------------ derivatives
+def test_operators_have_no_forward_derivative_either():
+    from torch.autograd import forward_ad
+
+    from tilegym_b200 import ops
+
+    with forward_ad.dual_level():
+        x = forward_ad.make_dual(torch.zeros(2, 128), torch.ones(2, 128))
+        with pytest.raises(RuntimeError, match="no backward"):
+            ops._no_grad_inputs(None, x)
+        with torch.no_grad(), pytest.raises(RuntimeError, match="no backward"):  # which has no say in tangents
+            ops._no_grad_inputs(x)
+        ops._no_grad_inputs(torch.zeros(2, 128), forward_ad.unpack_dual(x).primal)
+    ops._no_grad_inputs(torch.zeros(2, 128))

@@ -5,12 +5,14 @@ import time
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 from oracle import decoder_ref as D
 
 pytestmark = pytest.mark.gpu
 
 import tilegym_b200 as tg  # noqa: E402
+from tilegym_b200 import _lib  # noqa: E402
 
 F8 = torch.float8_e4m3fn
 BF, HF = torch.bfloat16, torch.float16
@@ -111,3 +113,26 @@ def test_a_full_launch_queue_holds_up_its_own_thread_only(dev, call):
     torch.cuda.synchronize()
     assert last - start > 0.2, "the queue was never full"
     assert longest < 0.1, f"this thread stood still for {longest:.2f} s"
+
+
+# ------------------------------------------------------------------ derivatives
+@pytest.mark.parametrize("extension", [True, False])
+def test_tangents_are_refused(dev, extension, monkeypatch):
+    """A result that silently loses a derivative is refused, in forward mode too."""
+    if not extension:
+        monkeypatch.setattr(_lib, "fast", None)
+    x, w = torch.ones(1, 128, dtype=BF, device=dev), torch.ones(128, dtype=BF, device=dev)
+    q, kv, at = torch.ones(1, 2, 64, dtype=BF, device=dev), torch.ones(1, 1, 64, dtype=BF, device=dev), torch.zeros(1, dtype=torch.int64, device=dev)
+    f, _ = tg.rope_frequencies(64, device=dev)
+    cache, table, lens = tg.FP8KVCache.empty(1, 1, 64, dev), i32([[0]]).to(dev), i32([1]).to(dev)
+    with forward_ad.dual_level():
+        def dual(t):
+            return forward_ad.make_dual(t, torch.ones_like(t))
+
+        for call in (lambda: tg.rms_norm_quant(dual(x), w), lambda: tg.rms_norm_quant(x, w, residual=dual(x)), lambda: tg.apply_rope(dual(q), kv, at, f),
+                     lambda: tg.apply_rope(q, dual(kv), at, f), lambda: tg.kv_cache_write(cache, dual(kv), kv, table, lens),
+                     lambda: tg.kv_cache_write(cache, kv, dual(kv), table, lens), lambda: tg.kv_cache_write(cache, kv, kv, table, lens, inv_freq=f, q=dual(q)),
+                     lambda: tg.paged_attention(dual(q), cache, table, lens)):
+            with pytest.raises(RuntimeError, match="no backward"):
+                call()
+        tg.paged_attention(q, cache, table, lens)  # the others are served

@@ -63,7 +63,7 @@ struct Desc {
 
 bool is_16bit(const Tensor& t) { return t.scalar_type() == at::kBFloat16 || t.scalar_type() == at::kHalf; }
 bool aligned(const Tensor& t) { return (reinterpret_cast<uint64_t>(t.data_ptr()) & 15u) == 0; }
-bool wants_grad(const Tensor& t) { return t.requires_grad() && at::GradMode::is_enabled(); }
+bool wants_grad(const Tensor& t) { return (t.requires_grad() && at::GradMode::is_enabled()) || t._fw_grad(0).defined(); }  // or has a tangent
 bool on(const Tensor& t, int64_t dev) { return t.is_cuda() && t.get_device() == dev; }
 bool heads(const Tensor& t, int64_t dev) {
   return on(t, dev) && t.dim() == 3 && is_16bit(t) && t.stride(2) == 1 && t.stride(0) % 8 == 0 && t.stride(1) % 8 == 0 && aligned(t) && !wants_grad(t);

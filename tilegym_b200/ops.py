@@ -13,6 +13,7 @@ import math
 from typing import Dict, List, Optional, Tuple
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -329,9 +330,11 @@ def per_token_group_quant_8bit(
 
 
 def _no_grad_inputs(*tensors: Optional[torch.Tensor]) -> None:
-    """The package has forward kernels only: a result that silently cuts the graph is refused."""
+    """The package has forward kernels only: a result that silently cuts the graph, or loses a tangent, is refused."""
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
         raise RuntimeError("tilegym_b200 operators have no backward: call them under torch.no_grad() or detach the inputs")
+    if any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise RuntimeError("tilegym_b200 operators have no backward and no forward-mode derivative: pass the primal values")
 
 
 def rms_norm_quant(
