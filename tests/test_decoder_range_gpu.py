@@ -2,10 +2,12 @@
 are far below the largest one and still make the answer.
 
 Tolerance: half a step of the output, and of sum p |v| the probabilities' own rounding and 32-bit noise, whatever the length
-of the cache.  A probability is rounded to f16 (2^-12) or to 9 bits (2^-9), and no finer than 2^-25 or 2^-23 where its row's
-largest is 2^8 or more: 2^-33 and 2^-31 of the largest.  The many have 2^-21.3 of the largest each, on the mean, in the
-longest case here, so that what ends there is at most 2^-11.7 or 2^-9.7 of them, and the rest within its rounding:
-PROBABILITY is a bound for both together.
+of the cache.
+A probability is rounded to f16, half a step 2^-11, and in the kernel for few rows of bf16 to nine bits, 2^-9.  Below f16's
+normal range that is 2^-25, and 2^-23 for the nine bits, where the row's largest is at least 2^8 (many rows) or 2^9 (few).
+The many have 2^-21.3 of the largest each, on the mean, in the longest case here: 2^-13.3 and 2^-12.3, so that what ends is at
+most 2^-11.7 (f16) and 2^-10.7 + 2^-12.7 (nine bits) of their sum.  Together: f16 2^-11 + 2^-11.7, bf16
+2^-9 + 2^-11 + 2^-10.7 + 2^-12.7 < 2^-8.
 A logit is a sum of 128 products in 32 bits, off by at most 128 * 2^-24 of the sum of their magnitudes (`size`), which
 moves a probability by as much, relative; numerator and denominator: 2^-16 * size.  exp, sums and rescaling: 2^-14."""
 
@@ -19,10 +21,11 @@ from oracle import decoder_ref as D
 pytestmark = pytest.mark.gpu
 
 import tilegym_b200 as tg  # noqa: E402
+from test_decoder_gpu import cumulative, gen, make_kv, on  # noqa: E402
 
 F8 = torch.float8_e4m3fn
 BF, HF = torch.bfloat16, torch.float16
-PROBABILITY = {BF: 2.0**-8, HF: 2.0**-11}
+PROBABILITY = {BF: 2.0**-8, HF: 2.0**-11 + 2.0**-11.7}
 
 
 def i32(x):
@@ -91,3 +94,21 @@ def test_the_many_count_in_a_large_batch(dev, length, share, dim, n, group, dtyp
     got = tg.paged_attention(q.repeat(copies, 1, 1).to(dev), tg.FP8KVCache(*(c.to(dev) for c in cache)), table.repeat(copies, 1).to(dev),
                              i32([length] * copies).to(dev), cu.to(dev), max_q_len=n)
     compare(got.cpu().unflatten(0, (copies, n)), q, cache, table, length)
+
+
+@pytest.mark.parametrize("new,past,window,sinks", [([1] * 5, [0, 130, 900, 3000, 5000], 0, 0), ([4, 1, 3], [0, 2500, 127], 0, 0), ([4, 2, 4], [3000, 700, 5], 600, 4),
+                                                   ([60, 1, 130], [3000, 200, 0], 0, 0), ([300, 7], [1000, 2000], 700, 130)])
+@pytest.mark.parametrize("heads,group,dim,dtype", [(2, 4, 128, BF), (1, 8, 64, HF), (2, 1, 64, BF), (1, 5, 128, HF)])
+def test_ordinary_batches_keep_the_same_bound(dev, new, past, window, sinks, heads, group, dim, dtype):
+    """Pages of different scales, foreign bytes behind the ends.  v_scale rides in the exponent, so p * v_scale is what ends, at
+    2^-31 of a row's largest, and it meets the values' bytes."""
+    g = gen(sum(new) + sum(past) + dim)
+    lens = [a + b for a, b in zip(new, past)]
+    table, ref = make_kv(lens, heads, dim, g)
+    q = torch.randn(sum(new), heads * group, dim, generator=g).to(dtype)
+    cu = cumulative(new)
+    got = tg.paged_attention(q.to(dev), on(dev, ref), table.to(dev), i32(lens).to(dev), cu.to(dev), max_q_len=max(new), window=window, sinks=sinks)
+    o, mag, size, coarse = D.ref_attention(q, ref, table, i32(lens), cu, window=window, sinks=sinks)
+    tiny = 2.0**-25 if dtype == HF else 0.0
+    bound = torch.finfo(dtype).eps / 2 * o.abs() + (PROBABILITY[dtype] + 2.0**-16 * size + 2.0**-14) * mag + 2.0**-31 * coarse + tiny
+    assert bool(((got.cpu().double() - o).abs() <= bound).all())
