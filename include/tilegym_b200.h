@@ -389,7 +389,7 @@ TG_API int32_t tg_apply_rope(const TgTensorDesc* Qo, const TgTensorDesc* Ko, con
  * seq_lens int32 [seqs]: tokens of each sequence INCLUDING the new ones; cu_seqlens int32 [seqs + 1]: sequence b's new
  * tokens are rows [cu[b], cu[b + 1]) of the batch, its last positions (null: one row per sequence).  Entries of these
  * tables are read on the device: pages outside [0, pages) and positions below 0 or past the table are neither read nor
- * written.  A page that is written belongs to one sequence.
+ * written.  A page that is written belongs to one sequence, once.
  *
  * write: K, V [T, heads, D] bf16 / f16.  Scale of a (page, head): smallest 2^e, -60 <= e <= 60, with amax / 2^e <= 448 over
  * the finite new values; a page that holds earlier tokens keeps the larger of its scale and the new one, and moves its

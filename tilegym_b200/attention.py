@@ -29,7 +29,8 @@ _16BIT = (torch.bfloat16, torch.float16)
 
 class FP8KVCache(NamedTuple):
     """k [pages, kv_heads, 128, head_dim] and v [pages, kv_heads, head_dim, 128] (values lie [dim][token]) in
-    float8_e4m3fn, k_scale / v_scale [pages, kv_heads] fp32, positive.  A value is its byte times its block's scale."""
+    float8_e4m3fn, k_scale / v_scale [pages, kv_heads] fp32, positive (what `kv_cache_write` sets is a power of two).  A value
+    is its byte times its block's scale."""
 
     k: torch.Tensor
     v: torch.Tensor
@@ -213,7 +214,7 @@ def kv_cache_write(
     the earlier bytes are moved to it.  NaN stays NaN, infinities saturate, and neither counts for the scale.  Only the
     new tokens' bytes (and the earlier ones of a page whose scale grew) are written.  Rows of the batch outside
     cu_seqlens, positions outside the table and pages outside the cache are left alone (their rows of q are unspecified).
-    A page that is written must belong to one sequence.
+    A page that is written must belong to one sequence and stand once in its row of the table.
     """
     if _lib.fast is not None:
         result = _lib.fast.kv_cache_write(*cache, k, v, block_table, seq_lens, cu_seqlens, inv_freq, q, interleaved, magnitude)
@@ -249,7 +250,7 @@ def kv_cache_read(
     max_len: int,
     dtype: torch.dtype = torch.bfloat16,
 ) -> Tuple[torch.Tensor, torch.Tensor]:
-    """(k, v), each (seqs, max_len, kv_heads, head_dim) in `dtype` (bf16: exact), with zeros behind a sequence's length
+    """(k, v), each (seqs, max_len, kv_heads, head_dim) in `dtype` (bf16: exact under power-of-two scales), with zeros behind a sequence's length
     (and where the table has no page of the cache)."""
     dev = ops._need_cuda(*cache, block_table, seq_lens)
     if dtype not in _16BIT:
@@ -287,8 +288,8 @@ def paged_attention(
     positions j <= i; with window > 0 of those only j > i - window or j < sinks.  scale: of the products, positive
     (1 / sqrt(head_dim) by default).  max_q_len bounds the new tokens of any sequence (1 without cu_seqlens, else the
     batch's token count by default); saying that it is small selects the kernel for few rows, and rows beyond it are not
-    computed.  A token that sees nothing (a sequence of length 0 in a padded batch) gets zeros; rows outside cu_seqlens
-    are not written.
+    computed.  One kernel serves the whole batch: single tokens beside a chunk of a prompt are faster as two calls.  A token that
+    sees nothing (a sequence of length 0 in a padded batch) gets zeros; rows outside cu_seqlens are not written.
     """
     dev = ops._cuda_index(q, *cache, block_table, seq_lens, cu_seqlens, out)
     if q.dim() != 3:
