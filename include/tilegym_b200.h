@@ -377,7 +377,7 @@ TG_API int32_t tg_rms_norm_quant(const TgTensorDesc* Y, const TgTensorDesc* S, c
                                  uint64_t stream);
 
 /* Rotary positions of Q [T, heads, D] and K [T, heads, D] (K / Ko may be null), bf16 / f16, D a multiple of 16 up to 512,
- * any token and head pitch that keeps 16-byte alignment; the outputs may be the inputs.  inv_freq: f64 [R / 2] radians per
+ * any token and head pitch that keeps 16-byte alignment; the outputs may be the inputs (with their pitches).  inv_freq: f64 [R / 2] radians per
  * position, R <= D a multiple of 16; elements from R on are copied.  interleaved 0: pairs (i, i + R / 2), 1: (2 i, 2 i + 1).
  * positions: int32 / int64 [T], any value.  cos and sin are multiplied by `magnitude`. */
 TG_API int32_t tg_apply_rope(const TgTensorDesc* Qo, const TgTensorDesc* Ko, const TgTensorDesc* Q, const TgTensorDesc* K,

@@ -217,3 +217,29 @@ def test_operators_have_no_forward_derivative_either():
             ops._no_grad_inputs(x)
         ops._no_grad_inputs(torch.zeros(2, 128), forward_ad.unpack_dual(x).primal)
     ops._no_grad_inputs(torch.zeros(2, 128))
+
+
+# ------------------------------------------------------------------ outputs in the place of inputs
+def test_outputs_in_the_place_of_inputs_lie_as_they_do():
+    """apply_rope and paged_attention may write over what they read where every head lies on itself; the same memory under other
+    pitches would be read by one warp or block after another has written it."""
+    L = _lib.lib()
+    memory = torch.zeros(4 * 4 * 64, dtype=BF)
+    q = memory.view(4, 4, 64)
+    other = memory.as_strided((4, 4, 64), (64, 256, 1))  # heads in front of tokens
+    pos, f = torch.zeros(4, dtype=torch.int64), torch.ones(32, dtype=torch.float64)
+    spare = torch.zeros(4, 4, 64, dtype=BF)
+
+    def rope(Qo, Q, Ko=None, K=None):
+        return L.tg_apply_rope(_d(Qo), _d(Ko), _d(Q), _d(K), _d(pos), _d(f), 0, 1.0, 0, 0)
+
+    c = tg.FP8KVCache.empty(4, 4, 64, device="cpu")
+    table, lens = torch.zeros(4, 1, dtype=torch.int32), torch.ones(4, dtype=torch.int32)
+
+    def attend(O, Q):
+        return L.tg_paged_attention(_d(O), _d(Q), *map(_d, c), _d(table), _d(lens), None, 1, 0.125, 0, 0, 0, 0, 0, 0)
+
+    assert rope(other, q) == -6 and rope(spare, spare, other, q) == -6
+    assert attend(other, q) == -6
+    if not torch.cuda.is_available():  # these get as far as the device
+        assert rope(q, q) != -6 and rope(spare, q, q, q) != -6 and attend(q, q) != -6 and attend(other, other) != -6

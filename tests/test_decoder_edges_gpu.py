@@ -52,6 +52,21 @@ def test_rows_that_see_nothing_are_zero_whatever_the_scales(dev, exponent, n, le
         assert bool(got[empty:].isfinite().all()) and bool((got[empty:] != 0).any(-1).all())
 
 
+@pytest.mark.parametrize("new,past,heads,group", [([1], [3000], 2, 4), ([1] * 400, [200] * 400, 2, 4), ([4, 8], [2000, 100], 1, 4), ([100], [4000], 1, 4), ([300, 70], [0, 500], 4, 2)])
+def test_out_may_be_the_queries(dev, new, past, heads, group):
+    lens = [a + b for a, b in zip(new, past)]
+    pages = [-(-n // 128) for n in lens]
+    cache = on(dev, make_cache(max(pages), heads, 64, len(new)))
+    table = torch.arange(max(pages), dtype=torch.int32).repeat(len(new), 1)  # read only: pages are shared
+    big = torch.randn(sum(new), 3, heads * group, 64, generator=torch.Generator().manual_seed(7)).to(BF).to(dev)
+    q = big[:, 1]
+    args = cache, table.to(dev), i32(lens).to(dev), i32([sum(new[:b]) for b in range(len(new) + 1)]).to(dev)
+    want = tg.paged_attention(q, *args, max_q_len=max(new))
+    around = big[:, ::2].clone()
+    assert tg.paged_attention(q, *args, max_q_len=max(new), out=q) is q
+    assert torch.equal(q, want) and torch.equal(big[:, ::2], around)
+
+
 # ------------------------------------------------------------------ kv_cache_write
 @pytest.mark.parametrize("scale", [1.5 * 2.0**-5, 1.0000001 * 2.0**-4, 1.75, 3e-9, 1.9 * 2.0**-30, 2.0**127, 1.5 * 2.0**100])
 @pytest.mark.parametrize("new", [1, 3, 60])

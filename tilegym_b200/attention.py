@@ -289,7 +289,7 @@ def paged_attention(
     (1 / sqrt(head_dim) by default).  max_q_len bounds the new tokens of any sequence (1 without cu_seqlens, else the
     batch's token count by default); saying that it is small selects the kernel for few rows, and rows beyond it are not
     computed.  One kernel serves the whole batch: single tokens beside a chunk of a prompt are faster as two calls.  A token that
-    sees nothing (a sequence of length 0 in a padded batch) gets zeros; rows outside cu_seqlens are not written.
+    sees nothing (a sequence of length 0 in a padded batch) gets zeros; rows outside cu_seqlens are not written.  out may be q.
     """
     dev = ops._cuda_index(q, *cache, block_table, seq_lens, cu_seqlens, out)
     if q.dim() != 3:

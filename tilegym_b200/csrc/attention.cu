@@ -50,6 +50,7 @@ extern "C" TG_API int32_t tg_paged_attention(const TgTensorDesc* O, const TgTens
     return api_fail(TG_ERR_ARGS, "the query heads must be a multiple of the cache's heads, at most 64 times as many");
   if ((rc = check_heads(Q, "q: [tokens, heads, head_dim of the cache], 16-byte aligned", T, heads, D, Q->dtype)) != TG_OK) return rc;
   if ((rc = check_heads_out(O, "output: shape and type of q, 16-byte aligned", T, heads, D, Q->dtype)) != TG_OK) return rc;
+  if ((rc = check_heads_place(O, Q)) != TG_OK) return rc;
   if (max_q_len < 1) return api_fail(TG_ERR_ARGS, "max_q_len must be at least 1");
   if (window < 0 || sinks < 0) return api_fail(TG_ERR_ARGS, "window and sinks must not be negative");
   if (sinks > 0 && window == 0) return api_fail(TG_ERR_ARGS, "sinks only mean something under a window");

@@ -572,11 +572,13 @@ extern "C" TG_API int32_t tg_apply_rope(const TgTensorDesc* Qo, const TgTensorDe
   int32_t rc;
   if ((rc = check_heads(Q, "q: rows of a head dense, pitches and pointer 16-byte aligned", T, Q->shape[1], D, Q->dtype)) != TG_OK) return rc;
   if ((rc = check_heads_out(Qo, "q output: shape and type of q, 16-byte aligned", T, Q->shape[1], D, Q->dtype)) != TG_OK) return rc;
+  if ((rc = check_heads_place(Qo, Q)) != TG_OK) return rc;
   p.q = heads_of(Q, Qo);
   if (K != nullptr) {
     if (K->ndim != 3 || K->shape[1] < 1 || K->shape[1] > 65536) return api_fail(TG_ERR_ARGS, "k must be [tokens, heads, head_dim]");
     if ((rc = check_heads(K, "k: tokens, head_dim and type of q, 16-byte aligned", T, K->shape[1], D, Q->dtype)) != TG_OK) return rc;
     if ((rc = check_heads_out(Ko, "k output: shape and type of k, 16-byte aligned", T, K->shape[1], D, Q->dtype)) != TG_OK) return rc;
+    if ((rc = check_heads_place(Ko, K)) != TG_OK) return rc;
     p.k = heads_of(K, Ko);
     if (T > 0 && Ko->ptr == Qo->ptr) return api_fail(TG_ERR_ARGS, "q and k must not be written to the same place");
   }
@@ -629,6 +631,7 @@ extern "C" TG_API int32_t tg_kv_cache_write(const TgTensorDesc* Kc, const TgTens
     if (Q->ndim != 3 || Q->shape[1] < 1 || Q->shape[1] > 65536) return api_fail(TG_ERR_ARGS, "q must be [tokens, heads, head_dim]");
     if ((rc = check_heads(Q, "q: tokens, head_dim and type of k, 16-byte aligned", T, Q->shape[1], D, K->dtype)) != TG_OK) return rc;
     if ((rc = check_heads_out(Qo, "q output: shape and type of q, 16-byte aligned", T, Q->shape[1], D, K->dtype)) != TG_OK) return rc;
+    if ((rc = check_heads_place(Qo, Q)) != TG_OK) return rc;
     p.q = heads_of(Q, Qo);
   }
   if (T == 0 || p.c.seqs == 0) return TG_OK;

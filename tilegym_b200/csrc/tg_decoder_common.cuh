@@ -72,6 +72,14 @@ inline int32_t check_heads_out(const TgTensorDesc* t, const char* what, int64_t 
   return TG_OK;
 }
 
+// An output that takes its input's place: every head on itself.
+inline int32_t check_heads_place(const TgTensorDesc* out, const TgTensorDesc* in) {
+  if (out->ptr != in->ptr || in->shape[0] < 1) return TG_OK;
+  if ((in->shape[0] > 1 && out->strides[0] != in->strides[0]) || (in->shape[1] > 1 && out->strides[1] != in->strides[1]))
+    return api_fail(TG_ERR_ARGS, "an output in the place of its input must have the same pitches");
+  return TG_OK;
+}
+
 inline int32_t check_dense_nd(const TgTensorDesc* t, const char* what, int32_t dtype, int nd, const int64_t* shape, unsigned align) {
   if (t == nullptr) return api_fail(TG_ERR_NULL, what);
   if (t->dtype != dtype) return api_fail(TG_ERR_DTYPE, what);
